@@ -70,9 +70,8 @@ __device__ __forceinline__ float aql_erf(float x) {
 
 // Pair form for the GEGLU epilogues (scripts/lib/original_unet.py:721-729, F.gelu exact form), which are VALU-bound: ~10k cycles of
 // activation per 128 x 160 tile next to a 5-step K loop.  A&S 7.1.28: erf(x) = 1 - (1 + a1 x + ... + a6 x^6)^-16, |error| <= 3e-7,
-// ONE transcendental (v_rcp) per element instead of two (v_rcp + v_exp), and every other operation -- six FMAs, four squarings -- on
-// TWO elements per instruction (v_pk_fma_f32 / v_pk_mul_f32: the two bf16 halves of a 32-bit word).  Per element ~11 issue slots
-// instead of ~19.  Large |x|: the 16th power overflows to +inf, its reciprocal is 0, erf = +-1 (no NaN: inf * inf = inf).
+// ONE transcendental (v_rcp) per element instead of two (v_rcp + v_exp); the other operations -- six FMAs, four squarings -- are written
+// on the two bf16 halves of a 32-bit word.  The library is built without packed-fp32 instructions (Makefile), so they issue one by one.  Large |x|: the 16th power overflows to +inf, its reciprocal is 0, erf = +-1 (no NaN: inf * inf = inf).
 // Used by the fused epilogues AND the stand-alone geglu kernels, so the two paths stay bit-identical to each other (packed lanes are
 // independent IEEE operations: the pairing does not matter).
 typedef float aql_f32x2_t __attribute__((ext_vector_type(2)));

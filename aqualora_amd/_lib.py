@@ -61,6 +61,11 @@ SIGNATURES = {
     "aql_groupnorm_silu_bwd": [c_p, c_p, c_i, c_i, c_i, c_p, c_p, c_i, c_p, c_p, c_p, c_p, c_p],
     "aql_layernorm_fwd": [c_p, c_l, c_i, c_p, c_p, c_f, c_p, c_p, c_p],
     "aql_layernorm_bwd": [c_p, c_p, c_l, c_i, c_p, c_p, c_p, c_p, c_p],
+    "aql_layernorm_train_scratch_floats": [c_l, c_i],
+    "aql_layernorm_train_fwd": [c_p, c_i, c_l, c_i, c_l, c_p, c_p, c_i, c_f, c_p, c_l, c_p, c_p, c_p, c_p],
+    "aql_layernorm_train_bwd": [c_p, c_p, c_p, c_p, c_p, c_i, c_l, c_i, c_l, c_l, c_l, c_p, c_i, c_p, c_p, c_l, c_p, c_p, c_p, c_l, c_p],
+    "aql_act8_pack": [c_p, c_i, c_l, c_i, c_l, c_p, c_p, c_p],
+    "aql_act8_unpack": [c_p, c_p, c_l, c_i, c_p, c_i, c_l, c_p],
     # X ldx M rps row0 S nstage | W ldw bias Adown Bup T Ts res ldr out ldo keep ln gamma beta eps stats nout ldn nout_row0 | stream
     "aql_lora_chain_fwd": [c_p, c_l, c_l, c_i, c_l, c_p, c_i] + [c_p] * 21 + [c_p],
     "aql_lora_chain_fwd_r320": [c_p, c_l, c_l, c_i, c_l, c_p, c_i] + [c_p] * 21 + [c_p],

@@ -2019,6 +2019,153 @@ def layernorm_res(x2d, gamma, beta, eps=1e-5):
     return LayerNormFn.apply(x2d, gamma, beta, eps, True)
 
 
+# ------------------------------------------------------------------- 8-bit activation checkpoints
+_ACT_DT = {torch.bfloat16: 0, torch.float32: 1}
+
+
+def _here(t, name):
+    """The kernels run on the current device's current stream: a tensor of another device is refused, not followed."""
+    _req(t, name)
+    if t.device.index != torch.cuda.current_device():
+        raise L.AqlError(f"{name}: tensor on {t.device}, but the current device is cuda:{torch.cuda.current_device()}; "
+                         "wrap the call in torch.cuda.device(...)")
+    if DUAL is not None and _full(t) is not None:
+        raise L.AqlError(f"{name} does not take twin batches")
+    return t
+
+
+def _rows2d(t, name):
+    """-> (t, row stride) with unit column stride and rows that do not overlap (a copy where t has neither)."""
+    if t.dim() != 2:
+        raise ValueError(f"{name}: expected [rows, columns], got {tuple(t.shape)}")
+    M, C = t.shape
+    if M <= 1:
+        t = t if t.is_contiguous() else t.contiguous()
+        return t, C
+    if t.stride(1) != 1 or t.stride(0) < C:
+        t = t.contiguous()
+    return t, t.stride(0)
+
+
+class Act8:
+    """An activation kept in 8 bits: int8 codes and one power-of-two step per 32 columns of a row (csrc/aql_act8.cuh), 1.03 bytes per value.
+    ``codes`` uint8 [M, Cp] (two's complement), ``exps`` uint8 [M, Cp / 32] (step = 2^(exp - 127)), Cp = C rounded up to 32."""
+
+    def __init__(self, codes, exps, shape, dtype):
+        self.codes, self.exps, self.shape, self.dtype = codes, exps, tuple(shape), dtype
+
+    def unpack(self, dtype=None):
+        """The values that the codes stand for, in the packed tensor's shape and type (or fp32 / bf16 on request: exact in both)."""
+        dtype = self.dtype if dtype is None else dtype
+        if dtype not in _ACT_DT:
+            raise ValueError(f"Act8.unpack: bfloat16 or float32, not {dtype}")
+        _here(self.codes, "Act8.unpack")
+        C = self.shape[-1]
+        out = torch.empty(self.shape, dtype=dtype, device=self.codes.device)
+        L.call("aql_act8_unpack", self.codes.data_ptr(), self.exps.data_ptr(), self.codes.shape[0], C, out.data_ptr(), _ACT_DT[dtype], C, L.stream_ptr())
+        return out
+
+
+def _act8_alloc(M, C, device):
+    Cp = (C + 31) // 32 * 32
+    return torch.empty(M, Cp, dtype=torch.uint8, device=device), torch.empty(M, Cp // 32, dtype=torch.uint8, device=device)
+
+
+def act8_pack(x):
+    """bf16 / fp32 ``x`` [..., C] -> Act8.  A value is off by at most half its block's step, 2^e / 2 with 63.75 2^e < max|block| (blocks whose
+    magnitudes reach from 2^-120 to 2^127); a block with an infinity or a NaN comes back as NaN.  No gradient flows through it."""
+    if x.dtype not in _ACT_DT:
+        raise ValueError(f"act8_pack: bfloat16 or float32, not {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"act8_pack: expected [..., columns], got {tuple(x.shape)}")
+    _here(x, "act8_pack")
+    C = x.shape[-1]
+    x2, ld = _rows2d(x.detach().reshape(-1, C), "act8_pack")
+    codes, exps = _act8_alloc(x2.shape[0], C, x.device)
+    L.call("aql_act8_pack", x2.data_ptr(), _ACT_DT[x.dtype], x2.shape[0], C, ld, codes.data_ptr(), exps.data_ptr(), L.stream_ptr())
+    return Act8(codes, exps, x.shape, x.dtype)
+
+
+# ------------------------------------------------------------------- LayerNorm with weight gradients
+class LayerNormTrainFn(torch.autograd.Function):
+    """LayerNorm whose gamma / beta are trained (``layernorm`` is the frozen form): dgamma, dbeta summed over the rows in fp32 in a fixed
+    order.  ``ckpt8``: the backward pass keeps x in 8 bits and computes xh = (x8 - mean) rstd from the codes."""
+
+    @staticmethod
+    def forward(ctx, x, gamma, beta, eps, ckpt8, passthrough):
+        M, C = x.shape
+        x2, ldx = _rows2d(x, "layernorm_train")
+        y = torch.empty(M, C, dtype=x.dtype, device=x.device)
+        stats = torch.empty(M, 2, dtype=torch.float32, device=x.device)
+        codes, exps = _act8_alloc(M, C, x.device) if ckpt8 else (None, None)
+        L.call("aql_layernorm_train_fwd", x2.data_ptr(), _ACT_DT[x.dtype], M, C, ldx, gamma.data_ptr(), L.ptr(beta), _ACT_DT[gamma.dtype], float(eps),
+               y.data_ptr(), C, stats.data_ptr(), L.ptr(codes), L.ptr(exps), L.stream_ptr())
+        ctx.save_for_backward(None if ckpt8 else x2, codes, exps, gamma, stats)
+        ctx.has_beta = beta is not None
+        if passthrough:
+            return y, x.view_as(x)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dres=None):
+        x2, codes, exps, gamma, stats = ctx.saved_tensors
+        _here(dy, "layernorm_train backward")
+        M, C = dy.shape
+        _, want_g, want_b = ctx.needs_input_grad[:3]
+        want_b = want_b and ctx.has_beta
+        dx = torch.empty(M, C, dtype=dy.dtype, device=dy.device)
+        if M == 0:
+            z = torch.zeros(C, dtype=gamma.dtype, device=dy.device)
+            return dx, z if want_g else None, z.clone() if want_b else None, None, None, None
+        dy, lddy = _rows2d(dy, "layernorm_train")
+        lddres = 0
+        if dres is not None:
+            dres, lddres = _rows2d(dres, "layernorm_train")
+        dg = torch.empty(C, dtype=torch.float32, device=dy.device) if want_g else None
+        db = torch.empty(C, dtype=torch.float32, device=dy.device) if want_b else None
+        n = L.call_raw("aql_layernorm_train_scratch_floats", M, C)
+        scratch = torch.empty(n, dtype=torch.float32, device=dy.device)
+        L.call("aql_layernorm_train_bwd", L.ptr(x2), L.ptr(codes), L.ptr(exps), dy.data_ptr(), L.ptr(dres), _ACT_DT[dy.dtype], M, C,
+               C if x2 is None or M == 1 else x2.stride(0), lddy, lddres, gamma.data_ptr(), _ACT_DT[gamma.dtype], stats.data_ptr(), dx.data_ptr(), C,
+               L.ptr(dg), L.ptr(db), scratch.data_ptr(), n, L.stream_ptr())
+        if dg is not None and gamma.dtype != torch.float32:
+            dg = dg.to(gamma.dtype)
+        if db is not None and gamma.dtype != torch.float32:
+            db = db.to(gamma.dtype)
+        return dx, dg, db, None, None, None
+
+
+def _layernorm_train(x2d, gamma, beta, eps, ckpt8, passthrough):
+    if x2d.dim() != 2:
+        raise ValueError(f"layernorm_train: expected [rows, columns], got {tuple(x2d.shape)}")
+    if x2d.dtype not in _ACT_DT:
+        raise ValueError(f"layernorm_train: bfloat16 or float32 rows, not {x2d.dtype}")
+    C = x2d.shape[1]
+    for p, n in ((gamma, "gamma"), (beta, "beta")):
+        if p is None and n == "beta":
+            continue
+        if tuple(p.shape) != (C,) or p.dtype not in _ACT_DT or p.device != x2d.device or (C > 1 and p.stride(0) != 1):
+            raise ValueError(f"layernorm_train: {n} must be a contiguous bfloat16 / float32 [{C}] on {x2d.device}")
+        if p.dtype != gamma.dtype:
+            raise ValueError("layernorm_train: gamma and beta must have the same type")
+    if not 1 <= C <= 8192:
+        raise ValueError(f"layernorm_train: 1 to 8192 columns, not {C}")
+    _here(x2d, "layernorm_train")
+    return LayerNormTrainFn.apply(x2d, gamma, beta, eps, bool(ckpt8), passthrough)
+
+
+def layernorm_train(x2d, gamma, beta=None, eps=1e-5, ckpt8=False):
+    """LayerNorm over the columns of ``x2d`` [M, C] (bf16 or fp32, C <= 8192) with gradients for x, gamma and beta (bf16 or fp32 [C]).
+    ``ckpt8`` keeps x in 8 bits for the backward pass (1.03 bytes per value instead of 2 or 4)."""
+    return _layernorm_train(x2d, gamma, beta, eps, ckpt8, False)
+
+
+def layernorm_train_res(x2d, gamma, beta=None, eps=1e-5, ckpt8=False):
+    """-> (normalised, x2d) with the residual gradient folded into the backward kernel (the form of ``layernorm_res``)."""
+    return _layernorm_train(x2d, gamma, beta, eps, ckpt8, True)
+
+
 class GegluFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h2d):

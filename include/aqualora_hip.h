@@ -220,6 +220,21 @@ int aql_groupnorm_silu_fwd(const bf16_t* x, int B, int HW, int C, const bf16_t* 
 int aql_groupnorm_silu_bwd(const bf16_t* x, const bf16_t* dy, int B, int HW, int C, const bf16_t* gamma,
                            const bf16_t* beta, int silu, const float* stats, const bf16_t* dres, bf16_t* dx,
                            float* scratch, aql_stream_t stream);
+/* LayerNorm that trains its own weights (csrc/aql_lnorm_train.hip): rows of any width up to 8192 and any row stride (`ldx`, elements),
+ * element alignment; dtype / param_dtype 0 = bf16, 1 = fp32 (of x, y, dy, dres, dx / of gamma, beta); beta may be null.  stats: [M][2] fp32 (mean, rstd).
+ * codes / exps (both or neither): 8-bit checkpoint of x (aql_act8_pack's layout), written by the forward pass, read by the backward pass in
+ * the place of x (pass x = null there).  dgamma / dbeta: fp32 [C], overwritten, each may be null.  scratch: fp32,
+ * aql_layernorm_train_scratch_floats(M, C) elements.  The same bits on every call (no atomics).                                          */
+int aql_layernorm_train_scratch_floats(long M, int C);
+int aql_layernorm_train_fwd(const void* x, int dtype, long M, int C, long ldx, const void* gamma, const void* beta, int param_dtype, float eps,
+                            void* y, long ldy, float* stats, uint8_t* codes, uint8_t* exps, aql_stream_t stream);
+int aql_layernorm_train_bwd(const void* x, const uint8_t* codes, const uint8_t* exps, const void* dy, const void* dres, int dtype, long M, int C,
+                            long ldx, long lddy, long lddres, const void* gamma, int param_dtype, const float* stats, void* dx, long lddx,
+                            float* dgamma, float* dbeta, float* scratch, long scratch_floats, aql_stream_t stream);
+/* 8-bit activation checkpoint (csrc/aql_act8.hip).  codes: [M][Cp] int8, exps: [M][Cp / 32], Cp = C rounded up to a multiple of 32 (the codes
+ * of the columns C..Cp-1 are 0); block value = code * 2^(exp - 127), exp = 255: the block held an infinity or a NaN and stands for NaN.  */
+int aql_act8_pack(const void* x, int dtype, long M, int C, long ldx, uint8_t* codes, uint8_t* exps, aql_stream_t stream);
+int aql_act8_unpack(const uint8_t* codes, const uint8_t* exps, long M, int C, void* out, int dtype, long ldo, aql_stream_t stream);
 int aql_layernorm_fwd(const bf16_t* x, long M, int C, const bf16_t* gamma, const bf16_t* beta, float eps, bf16_t* y,
                       float* stats, aql_stream_t stream);
 int aql_layernorm_bwd(const bf16_t* x, const bf16_t* dy, long M, int C, const bf16_t* gamma, const float* stats,

@@ -1,0 +1,171 @@
+"""Many owners' low-rank adapters on one frozen model: the weights of one projection's adapters (`AdapterBank`) and the description of which
+rows belong to whom (`RequestPlan`), the two handles of `ops.adapter_linear`.
+
+A watermark LoRA that has been baked for an owner (`inference.create_watermark_lora`) is an ordinary LoRA with matrices of its own.  Fusing it
+into the weights serves one owner per model copy; `ops.lora_linear` shares one pair of matrices between all samples.  Here every request of a
+batch names its adapter, and the batch still runs the shared projection as one product."""
+import numpy as np
+import torch
+import torch.nn as nn
+
+from . import _lib as L
+
+MAX_RANK = 1024
+
+
+class AdapterBank:
+    """G adapters of one projection [N, K], stacked at one rank.
+
+    ``down`` [G, r, K] and ``up`` [G, N, r] in bf16 or fp32; ``ranks[g]`` <= r says how much of adapter g is used (None: all of it), ``scales[g]``
+    multiplies it (None: 1).  The kernels read bf16 copies laid out once.  ``trainable``: ``down`` / ``up`` become fp32 parameters, their
+    gradients are fp32, and the copies follow after an optimizer step: `refresh` lays them out again when the parameters' versions
+    have changed (ops.adapter_linear calls it; writes through ``.data`` need ``refresh(force=True)``)."""
+
+    def __init__(self, down, up, ranks=None, scales=None, trainable=False, device="cuda"):
+        dev = torch.device(device)
+        if dev.type != "cuda":
+            raise L.AqlError("AdapterBank needs an MI355X (cuda device); there is no CPU path")
+        if down.dim() != 3 or up.dim() != 3 or down.shape[0] != up.shape[0] or down.shape[1] != up.shape[2]:
+            raise ValueError(f"AdapterBank: down [G, r, K] and up [G, N, r], not {tuple(down.shape)} and {tuple(up.shape)}")
+        for t in (down, up):
+            if t.dtype not in (torch.bfloat16, torch.float32):
+                raise ValueError(f"AdapterBank: bfloat16 or float32 weights, not {t.dtype}")
+        self.G, self.rank, self.K = down.shape
+        self.N = up.shape[1]
+        if not (1 <= self.G <= 65535 and 1 <= self.rank <= MAX_RANK and self.K % 8 == 0 and self.N % 8 == 0 and self.K and self.N):
+            raise ValueError(f"AdapterBank: 1 to 65535 adapters of rank 1 to {MAX_RANK} on sides that are multiples of 8, "
+                             f"not {self.G} of rank {self.rank} on [{self.N}, {self.K}]")
+        self.ranks = [self.rank] * self.G if ranks is None else [int(r) for r in ranks]
+        self.scales = [1.0] * self.G if scales is None else [float(s) for s in scales]
+        if len(self.ranks) != self.G or len(self.scales) != self.G or not all(0 <= r <= self.rank for r in self.ranks):
+            raise ValueError("AdapterBank: one rank of at most r and one scale for each adapter")
+        self.R = (self.rank + 7) // 8 * 8
+        self.trainable, self.device = bool(trainable), dev
+        self.ranks_dev = torch.tensor(self.ranks, dtype=torch.int32, device=dev)
+        self.scales_dev = torch.tensor(self.scales, dtype=torch.float32, device=dev)
+        self._live = torch.arange(self.R, device=dev)[None] < self.ranks_dev[:, None]      # [G, R]
+        z = lambda *s: torch.zeros(s, dtype=torch.bfloat16, device=dev)  # noqa: E731
+        self.a, self.b = z(self.G, self.R, self.K), z(self.G, self.N, self.R)
+        self.at = self.bt = None        # [G, K, R], [G, R, N]: the backward pass's operands, laid out when one first needs them
+        self._ver = None
+        self.serial = 0                 # counts the layouts: a backward pass refuses weights that changed since its forward pass
+        if trainable:
+            self.down = nn.Parameter(down.detach().to(device=dev, dtype=torch.float32, copy=True))
+            self.up = nn.Parameter(up.detach().to(device=dev, dtype=torch.float32, copy=True))
+        else:
+            self.down, self.up = down.detach().to(dev), up.detach().to(dev)
+        self.refresh()
+
+    @classmethod
+    def from_layers(cls, layers, trainable=False, device="cuda"):
+        """From LoRA layers (lora.LoRALinearLayer / LoRAConv2dLayer, 1x1) of one projection; ``network_alpha / rank`` becomes the scale."""
+        ranks = [int(ly.rank) for ly in layers]
+        r = max(ranks)
+        downs, ups, scales = [], [], []
+        for ly in layers:
+            d = ly.down.weight.detach().reshape(ly.rank, -1).float()
+            u = ly.up.weight.detach().reshape(-1, ly.rank).float()
+            downs.append(nn.functional.pad(d, (0, 0, 0, r - ly.rank)))
+            ups.append(nn.functional.pad(u, (0, r - ly.rank)))
+            alpha = getattr(ly, "network_alpha", None)
+            scales.append(1.0 if alpha is None else float(alpha) / ly.rank)
+        return cls(torch.stack(downs), torch.stack(ups), ranks=ranks, scales=scales, trainable=trainable, device=device)
+
+    def parameters(self):
+        return [self.down, self.up] if self.trainable else []
+
+    @torch.no_grad()
+    def refresh(self, force=False):
+        ver = (self.down._version, self.up._version)
+        if ver == self._ver and not force:
+            return
+        r, live = self.rank, self._live
+        # in place: a captured graph keeps reading these buffers
+        self.a[:, :r].copy_(torch.where(live[:, :r, None], self.down, torch.zeros((), dtype=self.down.dtype, device=self.device)))
+        self.b[:, :, :r].copy_(torch.where(live[:, None, :r], self.up, torch.zeros((), dtype=self.up.dtype, device=self.device)))
+        if self.at is not None:
+            self.at.copy_(self.a.transpose(1, 2))
+            self.bt.copy_(self.b.transpose(1, 2))
+        self._ver = ver
+        self.serial += 1
+
+    def transposed(self):
+        """(B^T [G, R, N], A^T [G, K, R]): the stacks as the backward-data pass reads them."""
+        if self.at is None:
+            self.at = self.a.transpose(1, 2).contiguous()
+            self.bt = self.b.transpose(1, 2).contiguous()
+        return self.bt, self.at
+
+
+class RequestPlan:
+    """Which rows use which adapter: request i has ``lengths[i]`` rows (None: all requests have the same number, whatever the rows of the call) and
+    adapter ``adapters[i]`` (-1: none).  Requests follow each other in the rows.  The tables are built on the host once and live on the device;
+    one plan serves every projection of a model, and calls with any number of rows per request when ``lengths`` is None."""
+
+    def __init__(self, adapters, lengths=None, device="cuda"):
+        dev = torch.device(device)
+        if dev.type != "cuda":
+            raise L.AqlError("RequestPlan needs an MI355X (cuda device); there is no CPU path")
+        ids = np.asarray([int(a) for a in adapters], dtype=np.int64)
+        if ids.size and ids.min() < -1:
+            raise ValueError("RequestPlan: adapters are numbered from 0; -1 is none")
+        self.equal = lengths is None
+        self.requests = int(ids.size)
+        n = np.ones(ids.size, dtype=np.int64) if self.equal else np.asarray([int(x) for x in lengths], dtype=np.int64)
+        if n.size != ids.size or (n.size and n.min() < 0):
+            raise ValueError("RequestPlan: one length of 0 or more for each request")
+        self.units = int(n.sum())
+        if self.units >= (1 << 31) - 256:
+            raise ValueError("RequestPlan: too many rows")
+        ids, n = ids[n > 0], n[n > 0]
+        first = np.flatnonzero(np.r_[True, ids[1:] != ids[:-1]]) if ids.size else np.zeros(0, dtype=np.int64)
+        begin = np.r_[0, np.cumsum(n)]
+        self._start = np.r_[begin[first], self.units] if ids.size else np.zeros(1, dtype=np.int64)     # [n + 1], neighbours of one adapter joined
+        seg = ids[first] if ids.size else ids
+        self.max_id = int(seg.max()) if seg.size else -1
+        self.nseg = int(seg.size) if self.max_id >= 0 else 0       # no adapters at all: no segments
+        size = np.diff(self._start)
+        # sorted order of the rows that have an adapter, for the weight gradients
+        order = np.argsort(seg, kind="stable")
+        order = order[seg[order] >= 0]
+        used, count_at = np.unique(seg[order], return_index=True)
+        pos = np.r_[0, np.cumsum(size[order])]
+        slot = np.full(max(self.max_id + 1, 1), -1, dtype=np.int64)
+        slot[used] = np.arange(used.size)
+        self.nsorted, self.nused, self.nslot, self.live_units = int(order.size), int(used.size), int(slot.size), int(pos[-1])
+        parts = dict(start=self._start, id=seg, seg_start=self._start[order] if order.size else order, seg_pos=pos,
+                     used_pos=np.r_[pos[count_at], pos[-1]] if used.size else pos, used_id=used, slot=slot)
+        flat = np.concatenate([p.astype(np.int32) for p in parts.values()])
+        self.device = dev
+        self.table = torch.from_numpy(flat).to(dev)
+        at = self.table.data_ptr()
+        self._ptr = {}
+        for k, p in parts.items():
+            self._ptr[k] = at
+            at += 4 * p.size
+        self._slots = {}
+        self.fwd_ptrs = (self._ptr["start"], self._ptr["id"])
+        self.grad_ptrs = tuple(self._ptr[k] for k in ("seg_start", "seg_pos", "used_pos", "used_id", "slot"))
+
+    def unit(self, rows):
+        """Rows per table unit for a call on ``rows`` rows."""
+        if not self.equal:
+            if rows != self.units:
+                raise ValueError(f"RequestPlan: the requests have {self.units} rows, the call {rows}")
+            return 1
+        if self.requests == 0:
+            if rows:
+                raise ValueError(f"RequestPlan: no requests for {rows} rows")
+            return 1
+        if rows % self.requests:
+            raise ValueError(f"RequestPlan: {rows} rows do not divide among {self.requests} equal requests")
+        return max(1, rows // self.requests)
+
+    def slots(self, unit):
+        """The most segments that meet in 16 consecutive rows [16 i, 16 i + 16)."""
+        s = self._slots.get(unit)
+        if s is None:
+            inner = self._start[1:-1] * unit
+            inner = inner[inner % 16 != 0] // 16
+            s = self._slots[unit] = 1 + (int(np.unique(inner, return_counts=True)[1].max()) if inner.size else 0)
+        return s

@@ -2166,6 +2166,139 @@ def layernorm_train_res(x2d, gamma, beta=None, eps=1e-5, ckpt8=False):
     return _layernorm_train(x2d, gamma, beta, eps, ckpt8, True)
 
 
+# ------------------------------------------------------------------- many requests' adapters beside one projection
+def _stream(t):
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+def _gemm_rows(t):
+    """-> (t, row stride): rows as the matrix kernels read them -- unit column stride, 16-byte aligned, a multiple of 8 elements apart."""
+    C = t.shape[1]
+    if t.shape[0] <= 1:
+        t = t if t.is_contiguous() else t.contiguous()
+        ld = C
+    else:
+        if t.stride(1) != 1 or t.stride(0) < C or t.stride(0) % 8 or t.stride(0) >= 1 << 21:
+            t = t.contiguous()
+        ld = t.stride(0)
+    if t.data_ptr() & 15:
+        t = t.clone(memory_format=torch.contiguous_format)
+        ld = C
+    return t, ld
+
+
+def _adapter_product(x, ldx, w, bias, res, ldr, a, b, bank, plan, unit, N, K):
+    """One pass of aql_adapter_linear -> (y [M, N], T [M, R] or None)."""
+    M = x.shape[0]
+    y = torch.empty(M, N, dtype=torch.bfloat16, device=x.device)
+    T = torch.empty(M, bank.R, dtype=torch.float32, device=x.device) if plan.nseg else None
+    L.call("aql_adapter_linear", x.data_ptr(), ldx, w.data_ptr(), K, None if bias is None else bias.data_ptr(),
+           None if res is None else res.data_ptr(), ldr, y.data_ptr(), N, M, N, K, a.data_ptr(), b.data_ptr(), bank.ranks_dev.data_ptr(),
+           bank.scales_dev.data_ptr(), bank.R, plan.fwd_ptrs[0], plan.fwd_ptrs[1], plan.nseg, unit, plan.slots(unit),
+           None if T is None else T.data_ptr(), _stream(x))
+    return y, T
+
+
+def _adapter_down(x, ldx, codes, exps, M, K, a, bank, plan, unit, like):
+    T = torch.empty(M, bank.R, dtype=torch.float32, device=like.device)
+    L.call("aql_adapter_down", None if x is None else x.data_ptr(), ldx, L.ptr(codes), L.ptr(exps), M, K, a.data_ptr(), bank.ranks_dev.data_ptr(),
+           bank.scales_dev.data_ptr(), bank.R, plan.fwd_ptrs[0], plan.fwd_ptrs[1], plan.nseg, unit, plan.slots(unit), T.data_ptr(), _stream(like))
+    return T
+
+
+def _adapter_wgrad(u, v, ldv, codes, exps, M, C, trans, bank, plan, unit, like):
+    """fp32 gradient of a stack: [G, r, C], or [G, C, r] with ``trans``."""
+    r = bank.rank
+    out = torch.empty((bank.G, C, r) if trans else (bank.G, r, C), dtype=torch.float32, device=like.device)
+    rows = plan.live_units * unit
+    n = L.call_raw("aql_adapter_wgrad_scratch_floats", rows, plan.nused, C, bank.R)
+    if n < 0:
+        raise L.AqlError("adapter_linear: the weight gradients' workspace passes 2^31 elements; train fewer rows or adapters per call")
+    scratch = torch.empty(n, dtype=torch.float32, device=like.device)
+    L.call("aql_adapter_wgrad", L.ptr(u), bank.R, L.ptr(v), ldv, L.ptr(codes), L.ptr(exps), M, C, bank.G, r, bank.ranks_dev.data_ptr(), *plan.grad_ptrs,
+           plan.nsorted, plan.nused, plan.nslot, unit, rows, int(trans), out.data_ptr(), scratch.data_ptr() if n else None, n, _stream(like))
+    return out
+
+
+class AdapterLinearFn(torch.autograd.Function):
+    """Y = X.W^T + b + residual + s_g (X.A_g^T).B_g^T with g by request (adapters.AdapterBank, adapters.RequestPlan).  Gradients: dX, dA, dB (fp32), residual.
+    ``ckpt8``: the backward pass keeps X in 8 bits -- T is computed again from the codes, and dA and dB see their values in the place of X."""
+
+    @staticmethod
+    def forward(ctx, x2d, down, up, residual, packed, bank, plan, unit, ckpt8):
+        x, ldx = _gemm_rows(x2d)
+        res, ldr = (None, 0) if residual is None else _gemm_rows(residual)
+        y, T = _adapter_product(x, ldx, packed.w, packed.bias, res, ldr, bank.a, bank.b, bank, plan, unit, packed.N, packed.K)
+        ctx.packed, ctx.bank, ctx.plan, ctx.unit, ctx.serial, ctx.ckpt8 = packed, bank, plan, unit, bank.serial, ckpt8
+        ctx.train = bank.trainable and (ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
+        codes = exps = None
+        if not ctx.train:
+            x = T = None
+        elif ckpt8:
+            M, K = x.shape
+            codes, exps = _act8_alloc(M, K, x.device)
+            L.call("aql_act8_pack", x.data_ptr(), 0, M, K, ldx, codes.data_ptr(), exps.data_ptr(), _stream(x))
+            x = T = None
+        ctx.save_for_backward(x, T, codes, exps)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        _here(dy, "adapter_linear backward")
+        x, T, codes, exps = ctx.saved_tensors
+        packed, bank, plan, unit = ctx.packed, ctx.bank, ctx.plan, ctx.unit
+        want_x, want_a, want_b, want_r = ctx.needs_input_grad[:4]
+        if bank.serial != ctx.serial:
+            raise L.AqlError("adapter_linear: the bank's weights changed between the forward pass and its backward pass")
+        dy2, lddy = _gemm_rows(dy)
+        M, N, K = dy2.shape[0], packed.N, packed.K
+        dx = dA = dB = dT = None
+        if M == 0:
+            zeros = lambda p: torch.zeros_like(p, dtype=torch.float32)  # noqa: E731
+            return (dy.new_empty(0, K), zeros(bank.down) if want_a else None, zeros(bank.up) if want_b else None, dy if want_r else None) + (None,) * 5
+        if want_x:
+            bt, at = bank.transposed()
+            dx, dT = _adapter_product(dy2, lddy, packed.wt, None, None, 0, bt, at, bank, plan, unit, K, N)
+        if ctx.train:
+            if want_a:
+                if dT is None and plan.nseg:
+                    dT = _adapter_down(dy2, lddy, None, None, M, N, bank.transposed()[0], bank, plan, unit, dy2)
+                dA = _adapter_wgrad(dT, x, 0 if x is None else (K if M <= 1 else x.stride(0)), codes, exps, M, K, False, bank, plan, unit, dy2)
+            if want_b:
+                if T is None and plan.nseg:
+                    T = _adapter_down(None, 0, codes, exps, M, K, bank.a, bank, plan, unit, dy2)
+                dB = _adapter_wgrad(T, dy2, lddy, None, None, M, N, True, bank, plan, unit, dy2)
+        return dx, dA, dB, (dy if want_r else None), None, None, None, None, None
+
+
+def adapter_linear(x2d, packed, bank, plan, residual=None, ckpt8=False):
+    """``x2d`` [M, K] bf16 through ``packed`` (PackedLinear, K and N multiples of 8) with every request's own adapter -> [M, N] bf16.
+    ``bank``: adapters.AdapterBank of this projection; ``plan``: adapters.RequestPlan whose requests make up the M rows; ``residual`` [M, N] is
+    added before the one rounding.  Differentiable in x2d, residual and a trainable bank's down / up; ``ckpt8`` keeps x2d in 8 bits for the latter."""
+    if x2d.dim() != 2 or x2d.dtype != torch.bfloat16:
+        raise ValueError(f"adapter_linear: expected bfloat16 [rows, {packed.K}], got {x2d.dtype} {tuple(x2d.shape)}")
+    M, K = x2d.shape
+    N = packed.N
+    if K != packed.K or bank.K != K or bank.N != N:
+        raise ValueError(f"adapter_linear: input of width {K}, projection [{packed.N}, {packed.K}], adapters on [{bank.N}, {bank.K}]")
+    if plan.max_id >= bank.G:
+        raise ValueError(f"adapter_linear: the plan names adapter {plan.max_id}, the bank has {bank.G}")
+    unit = plan.unit(M)
+    if residual is not None and (tuple(residual.shape) != (M, N) or residual.dtype != torch.bfloat16):
+        raise ValueError(f"adapter_linear: residual must be bfloat16 [{M}, {N}], not {residual.dtype} {tuple(residual.shape)}")
+    _here(x2d, "adapter_linear")
+    if bank.a.device != x2d.device or plan.table.device != x2d.device or packed.w.device != x2d.device or (residual is not None and residual.device != x2d.device):
+        raise ValueError("adapter_linear: input, projection, adapters, plan and residual must live on one device")
+    bank.refresh()
+    if torch.is_grad_enabled() and (x2d.requires_grad or (residual is not None and residual.requires_grad) or
+                                    (bank.trainable and (bank.down.requires_grad or bank.up.requires_grad))):
+        return AdapterLinearFn.apply(x2d, bank.down, bank.up, residual, packed, bank, plan, unit, bool(ckpt8))
+    x, ldx = _gemm_rows(x2d)
+    res, ldr = (None, 0) if residual is None else _gemm_rows(residual)
+    return _adapter_product(x, ldx, packed.w, packed.bias, res, ldr, bank.a, bank.b, bank, plan, unit, N, K)[0]
+
+
 class GegluFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h2d):

@@ -212,6 +212,30 @@ def load():
     return lib
 
 
+TORCH_LIB_PATH = os.path.join(_HERE, "csrc", "libaqualora_torch.so")
+_native = None
+
+
+def native():
+    """The autograd binding of the training operators (csrc/aql_torch.cpp): a Python module next to the kernel library, loaded once."""
+    global _native
+    if _native is None:
+        load()
+        if not os.path.exists(TORCH_LIB_PATH):
+            raise AqlError(f"{TORCH_LIB_PATH} not found: build it with `python -c 'import __graft_entry__ as g; g.build()'` "
+                           "(or `make -C aqualora_amd/csrc`). There is no fallback path.")
+        import importlib.machinery
+        import importlib.util
+        loader = importlib.machinery.ExtensionFileLoader("aqualora_torch", TORCH_LIB_PATH)
+        mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("aqualora_torch", loader))
+        loader.exec_module(mod)
+        if mod.abi_version() != ABI_VERSION:
+            raise AqlError(f"{TORCH_LIB_PATH} calls a kernel library of AQL_ABI_VERSION {mod.abi_version()}, this binding expects {ABI_VERSION}: rebuild")
+        mod.set_error_class(AqlError)
+        _native = mod
+    return _native
+
+
 def check(status, what=""):
     if status != 0:
         msg = load().aql_last_error().decode("utf-8", "replace")

@@ -19,7 +19,8 @@ class AdapterBank:
     ``down`` [G, r, K] and ``up`` [G, N, r] in bf16 or fp32; ``ranks[g]`` <= r says how much of adapter g is used (None: all of it), ``scales[g]``
     multiplies it (None: 1).  The kernels read bf16 copies laid out once.  ``trainable``: ``down`` / ``up`` become fp32 parameters, their
     gradients are fp32, and the copies follow after an optimizer step: `refresh` lays them out again when the parameters' versions
-    have changed (ops.adapter_linear calls it; writes through ``.data`` need ``refresh(force=True)``)."""
+    have changed (ops.adapter_linear calls it; writes through ``.data``, and an optimizer step inside a captured graph, need
+    ``refresh(force=True)`` behind them)."""
 
     def __init__(self, down, up, ranks=None, scales=None, trainable=False, device="cuda"):
         dev = torch.device(device)
@@ -39,22 +40,25 @@ class AdapterBank:
         self.scales = [1.0] * self.G if scales is None else [float(s) for s in scales]
         if len(self.ranks) != self.G or len(self.scales) != self.G or not all(0 <= r <= self.rank for r in self.ranks):
             raise ValueError("AdapterBank: one rank of at most r and one scale for each adapter")
-        self.R = (self.rank + 7) // 8 * 8
+        self.R = (self.rank + 7) // 8 * 8    # the stacks' rank
         self.trainable, self.device = bool(trainable), dev
-        self.ranks_dev = torch.tensor(self.ranks, dtype=torch.int32, device=dev)
-        self.scales_dev = torch.tensor(self.scales, dtype=torch.float32, device=dev)
-        self._live = torch.arange(self.R, device=dev)[None] < self.ranks_dev[:, None]      # [G, R]
-        z = lambda *s: torch.zeros(s, dtype=torch.bfloat16, device=dev)  # noqa: E731
-        self.a, self.b = z(self.G, self.R, self.K), z(self.G, self.N, self.R)
-        self.at = self.bt = None        # [G, K, R], [G, R, N]: the backward pass's operands, laid out when one first needs them
+        h = self.handle = L.native().Bank()  # what the kernels' binding reads
+        h.G, h.r, h.R, h.K, h.N, h.trainable = self.G, self.rank, self.R, self.K, self.N, self.trainable
+        h.ranks = torch.tensor(self.ranks, dtype=torch.int32, device=dev)
+        h.scales = torch.tensor(self.scales, dtype=torch.float32, device=dev)
+        self._live = torch.arange(self.rank, device=dev)[None] < h.ranks[:, None]      # [G, r]
+        h.a = torch.zeros(self.G, self.R, self.K, dtype=torch.bfloat16, device=dev)
+        h.b = torch.zeros(self.G, self.N, self.R, dtype=torch.bfloat16, device=dev)
+        self._transposed = False
         self._ver = None
-        self.serial = 0                 # counts the layouts: a backward pass refuses weights that changed since its forward pass
         if trainable:
             self.down = nn.Parameter(down.detach().to(device=dev, dtype=torch.float32, copy=True))
             self.up = nn.Parameter(up.detach().to(device=dev, dtype=torch.float32, copy=True))
         else:
             self.down, self.up = down.detach().to(dev), up.detach().to(dev)
         self.refresh()
+        if trainable:
+            self.lay_out_transposed()
 
     @classmethod
     def from_layers(cls, layers, trainable=False, device="cuda"):
@@ -74,27 +78,31 @@ class AdapterBank:
     def parameters(self):
         return [self.down, self.up] if self.trainable else []
 
-    @torch.no_grad()
     def refresh(self, force=False):
         ver = (self.down._version, self.up._version)
         if ver == self._ver and not force:
             return
-        r, live = self.rank, self._live
-        # in place: a captured graph keeps reading these buffers
-        self.a[:, :r].copy_(torch.where(live[:, :r, None], self.down, torch.zeros((), dtype=self.down.dtype, device=self.device)))
-        self.b[:, :, :r].copy_(torch.where(live[:, None, :r], self.up, torch.zeros((), dtype=self.up.dtype, device=self.device)))
-        if self.at is not None:
-            self.at.copy_(self.a.transpose(1, 2))
-            self.bt.copy_(self.b.transpose(1, 2))
+        h, r, live = self.handle, self.rank, self._live
+        with torch.no_grad():                # in place: a captured graph keeps reading these buffers
+            h.a[:, :r].copy_(torch.where(live[:, :, None], self.down, torch.zeros((), dtype=self.down.dtype, device=self.device)))
+            h.b[:, :, :r].copy_(torch.where(live[:, None, :], self.up, torch.zeros((), dtype=self.up.dtype, device=self.device)))
+            if self._transposed:
+                h.at.copy_(h.a.transpose(1, 2))
+                h.bt.copy_(h.b.transpose(1, 2))
         self._ver = ver
-        self.serial += 1
+        h.serial += 1                        # a backward pass refuses weights that changed since its forward pass
 
-    def transposed(self):
-        """(B^T [G, R, N], A^T [G, K, R]): the stacks as the backward-data pass reads them."""
-        if self.at is None:
-            self.at = self.a.transpose(1, 2).contiguous()
-            self.bt = self.b.transpose(1, 2).contiguous()
-        return self.bt, self.at
+    def lay_out_transposed(self):
+        """B^T [G, R, N] and A^T [G, K, R], the stacks as the backward-data pass reads them: at once for a trainable bank, for others when an input
+        first asks for a gradient."""
+        if self._transposed:
+            return
+        if torch.cuda.is_current_stream_capturing():
+            raise L.AqlError("AdapterBank: call lay_out_transposed() before capturing a pass that differentiates a frozen bank's input")
+        h = self.handle
+        h.at, h.bt = h.a.transpose(1, 2).contiguous(), h.b.transpose(1, 2).contiguous()
+        torch.cuda.current_stream(self.device).synchronize()      # once: later calls may come on other streams
+        self._transposed = True
 
 
 class RequestPlan:
@@ -120,11 +128,10 @@ class RequestPlan:
         ids, n = ids[n > 0], n[n > 0]
         first = np.flatnonzero(np.r_[True, ids[1:] != ids[:-1]]) if ids.size else np.zeros(0, dtype=np.int64)
         begin = np.r_[0, np.cumsum(n)]
-        self._start = np.r_[begin[first], self.units] if ids.size else np.zeros(1, dtype=np.int64)     # [n + 1], neighbours of one adapter joined
+        start = np.r_[begin[first], self.units] if ids.size else np.zeros(1, dtype=np.int64)     # [n + 1], neighbours of one adapter joined
         seg = ids[first] if ids.size else ids
         self.max_id = int(seg.max()) if seg.size else -1
-        self.nseg = int(seg.size) if self.max_id >= 0 else 0       # no adapters at all: no segments
-        size = np.diff(self._start)
+        size = np.diff(start)
         # sorted order of the rows that have an adapter, for the weight gradients
         order = np.argsort(seg, kind="stable")
         order = order[seg[order] >= 0]
@@ -132,40 +139,13 @@ class RequestPlan:
         pos = np.r_[0, np.cumsum(size[order])]
         slot = np.full(max(self.max_id + 1, 1), -1, dtype=np.int64)
         slot[used] = np.arange(used.size)
-        self.nsorted, self.nused, self.nslot, self.live_units = int(order.size), int(used.size), int(slot.size), int(pos[-1])
-        parts = dict(start=self._start, id=seg, seg_start=self._start[order] if order.size else order, seg_pos=pos,
+        parts = dict(start=start, id=seg, seg_start=start[order] if order.size else order, seg_pos=pos,
                      used_pos=np.r_[pos[count_at], pos[-1]] if used.size else pos, used_id=used, slot=slot)
         flat = np.concatenate([p.astype(np.int32) for p in parts.values()])
-        self.device = dev
-        self.table = torch.from_numpy(flat).to(dev)
-        at = self.table.data_ptr()
-        self._ptr = {}
-        for k, p in parts.items():
-            self._ptr[k] = at
-            at += 4 * p.size
-        self._slots = {}
-        self.fwd_ptrs = (self._ptr["start"], self._ptr["id"])
-        self.grad_ptrs = tuple(self._ptr[k] for k in ("seg_start", "seg_pos", "used_pos", "used_id", "slot"))
-
-    def unit(self, rows):
-        """Rows per table unit for a call on ``rows`` rows."""
-        if not self.equal:
-            if rows != self.units:
-                raise ValueError(f"RequestPlan: the requests have {self.units} rows, the call {rows}")
-            return 1
-        if self.requests == 0:
-            if rows:
-                raise ValueError(f"RequestPlan: no requests for {rows} rows")
-            return 1
-        if rows % self.requests:
-            raise ValueError(f"RequestPlan: {rows} rows do not divide among {self.requests} equal requests")
-        return max(1, rows // self.requests)
-
-    def slots(self, unit):
-        """The most segments that meet in 16 consecutive rows [16 i, 16 i + 16)."""
-        s = self._slots.get(unit)
-        if s is None:
-            inner = self._start[1:-1] * unit
-            inner = inner[inner % 16 != 0] // 16
-            s = self._slots[unit] = 1 + (int(np.unique(inner, return_counts=True)[1].max()) if inner.size else 0)
-        return s
+        h = self.handle = L.native().Plan()  # what the kernels' binding reads
+        self.table = h.table = torch.from_numpy(flat).to(dev)
+        h.at = np.r_[0, np.cumsum([p.size for p in parts.values()])[:-1]].tolist()
+        h.start = start.tolist()
+        h.units, h.requests, h.live_units, h.equal, h.max_id = self.units, self.requests, int(pos[-1]), self.equal, self.max_id
+        h.nseg = int(seg.size) if self.max_id >= 0 else 0              # no adapters at all: no segments
+        h.nsorted, h.nused, h.nslot = int(order.size), int(used.size), int(slot.size)

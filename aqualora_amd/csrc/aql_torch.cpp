@@ -1,0 +1,413 @@
+// Autograd binding of the training operators (LayerNorm with weight gradients, 8-bit checkpoints, adapters of many requests): argument checks,
+// output allocation, the calls of the C ABI, and the backward nodes, in C++.
+//
+// Why not Python like the other wrappers: these operators are short (8-30 us each way at a few thousand rows), and a Python backward node costs
+// more than that on the host -- it runs on the engine's device thread, where it has to take the interpreter lock for every line.  Measured for a
+// LayerNorm forward + backward of 64 x 320: 155 us of host time with Python nodes (17 us forward alone).
+// No kernel is here: everything below ends in an aql_* entry point of libaqualora_hip.so.
+#include <torch/extension.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPStream.h>
+
+#include <cstdlib>
+#include <memory>
+#include <optional>
+#include <string>
+#include <unordered_map>
+#include <vector>
+
+#include "../../include/aqualora_hip.h"
+
+namespace py = pybind11;
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+namespace {
+
+struct AqlErr : std::runtime_error {   // becomes aqualora_amd._lib.AqlError in Python
+  using std::runtime_error::runtime_error;
+};
+py::handle aql_error_class;
+
+bool debug_sync() {
+  static const bool on = [] { const char* e = std::getenv("AQL_DEBUG_SYNC"); return e && *e; }();
+  return on;
+}
+void ran(int rc, const char* name, aql_stream_t st) {
+  if (rc) throw AqlErr(std::string(name) + " failed with status " + std::to_string(rc) + ": " + aql_last_error());
+  if (debug_sync()) {   // the debugging aid of _lib.call: name the entry point that faulted
+    std::fprintf(stderr, "[aql] %s\n", name);
+    std::fflush(stderr);
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing((hipStream_t)st, &cs) == hipSuccess && cs == hipStreamCaptureStatusNone) (void)hipDeviceSynchronize();
+  }
+}
+[[noreturn]] void bad_value(const std::string& s) { throw py::value_error(s); }
+std::string shape_of(const Tensor& t) {
+  std::string s = "[";
+  for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
+  return s + "]";
+}
+
+// the kernels run on the current device's current stream: a tensor of another device is refused, not followed
+void here(const Tensor& t, const char* name) {
+  if (!t.is_cuda()) throw AqlErr(std::string(name) + ": the HIP path needs a GPU tensor; there is no CPU fallback");
+  if (t.get_device() != c10::hip::current_device())
+    throw AqlErr(std::string(name) + ": tensor on device " + std::to_string(t.get_device()) + ", but the current device is " +
+                 std::to_string(c10::hip::current_device()) + "; wrap the call in torch.cuda.device(...)");
+}
+aql_stream_t stream_of(const Tensor& t) { return (aql_stream_t)c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+
+int dt(const Tensor& t) { return t.scalar_type() == at::kBFloat16 ? 0 : 1; }
+bool bf16_or_f32(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat; }
+template <class T = void>
+T* ptr(const Tensor& t) { return t.defined() ? (T*)t.data_ptr() : nullptr; }
+
+struct Rows {
+  Tensor t;
+  long ld = 0;
+};
+// rows with unit column stride that do not overlap
+Rows rows2d(const Tensor& t) {
+  const long M = t.size(0), C = t.size(1);
+  if (M <= 1) return {t.is_contiguous() ? t : t.contiguous(), C};
+  if (t.stride(1) != 1 || t.stride(0) < C) return {t.contiguous(), C};
+  return {t, t.stride(0)};
+}
+// rows as the matrix kernels read them: 16-byte aligned, a multiple of 8 elements apart
+Rows gemm_rows(const Tensor& t) {
+  Rows r = rows2d(t);
+  if (r.ld % 8 || r.ld >= (1L << 21) || ((uintptr_t)r.t.data_ptr() & 15)) r = {r.t.clone(at::MemoryFormat::Contiguous), t.size(1)};
+  return r;
+}
+
+// gradients of a backward pass under create_graph: they carry a node that refuses a second backward pass
+variable_list once(variable_list grads, const char* name) {
+  if (!at::GradMode::is_enabled()) return grads;
+  at::AutoGradMode off(false);
+  variable_list in;
+  for (auto& g : grads)
+    if (g.defined()) in.push_back(g.detach().set_requires_grad(true));
+  if (in.empty()) return grads;
+  auto err = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " has no second derivative", (int64_t)in.size());
+  auto out = (*err)(std::move(in));
+  size_t k = 0;
+  for (auto& g : grads)
+    if (g.defined()) g = out[k++];
+  return grads;
+}
+
+// ------------------------------------------------------------------------------------------------------------------ 8-bit checkpoint
+std::pair<Tensor, Tensor> act8_alloc(long M, long C, const Tensor& like) {
+  const long Cp = (C + 31) / 32 * 32;
+  const auto opt = like.options().dtype(at::kByte).requires_grad(false);
+  return {at::empty({M, Cp}, opt), at::empty({M, Cp / 32}, opt)};
+}
+
+std::pair<Tensor, Tensor> act8_pack(const Tensor& x) {
+  if (!bf16_or_f32(x)) bad_value(std::string("act8_pack: bfloat16 or float32, not ") + c10::toString(x.scalar_type()));
+  if (x.dim() < 1 || x.size(-1) == 0) bad_value("act8_pack: expected [..., columns], got " + shape_of(x));
+  here(x, "act8_pack");
+  at::AutoGradMode off(false);
+  const long C = x.size(-1);
+  const Rows r = rows2d(x.numel() ? x.reshape({-1, C}) : x.reshape({0, C}));
+  auto [codes, exps] = act8_alloc(r.t.size(0), C, x);
+  const auto st = stream_of(x);
+  ran(aql_act8_pack(r.t.data_ptr(), dt(x), r.t.size(0), (int)C, r.ld, ptr<uint8_t>(codes), ptr<uint8_t>(exps), st), "aql_act8_pack", st);
+  return {codes, exps};
+}
+
+Tensor act8_unpack(const Tensor& codes, const Tensor& exps, std::vector<int64_t> shape, bool bf16) {
+  here(codes, "Act8.unpack");
+  const long C = shape.back();
+  Tensor out = at::empty(shape, codes.options().dtype(bf16 ? at::kBFloat16 : at::kFloat));
+  const auto st = stream_of(codes);
+  ran(aql_act8_unpack(ptr<uint8_t>(codes), ptr<uint8_t>(exps), codes.size(0), (int)C, out.data_ptr(), bf16 ? 0 : 1, C, st), "aql_act8_unpack", st);
+  return out;
+}
+
+// -------------------------------------------------------------------------------------------------------- LayerNorm with weight gradients
+struct LayerNormTrain : torch::autograd::Function<LayerNormTrain> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& gamma, const std::optional<Tensor>& beta_, double eps, bool ckpt8, bool passthrough) {
+    const Tensor beta = beta_ ? *beta_ : Tensor();
+    const long M = x.size(0), C = x.size(1);
+    const Rows r = rows2d(x);
+    Tensor y = at::empty({M, C}, x.options()), stats = at::empty({M, 2}, x.options().dtype(at::kFloat)), codes, exps;
+    if (ckpt8) std::tie(codes, exps) = act8_alloc(M, C, x);
+    const auto st = stream_of(x);
+    ran(aql_layernorm_train_fwd(r.t.data_ptr(), dt(x), M, (int)C, r.ld, gamma.data_ptr(), ptr(beta), dt(gamma), (float)eps, y.data_ptr(), C,
+                                ptr<float>(stats), ptr<uint8_t>(codes), ptr<uint8_t>(exps), st), "aql_layernorm_train_fwd", st);
+    ctx->save_for_backward({ckpt8 ? Tensor() : r.t, codes, exps, gamma, stats});
+    ctx->saved_data["beta"] = beta.defined();
+    if (passthrough) return {y, x.view_as(x)};
+    return {y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &x = s[0], &codes = s[1], &exps = s[2], &gamma = s[3], &stats = s[4];
+    const long M = stats.size(0), C = gamma.size(0);
+    const bool want_g = ctx->needs_input_grad(1), want_b = ctx->saved_data["beta"].toBool() && ctx->needs_input_grad(2);
+    if (!g[0].defined()) {   // only the pass-through output was used
+      const Tensor z;
+      return {g.size() > 1 ? g[1] : z, z, z, z, z, z};
+    }
+    here(g[0], "layernorm_train backward");
+    Tensor dx, dg, db;
+    {
+      at::AutoGradMode off(false);
+      const auto f32 = g[0].options().dtype(at::kFloat);
+      dx = at::empty({M, C}, g[0].options());
+      if (M == 0) {
+        if (want_g) dg = at::zeros({C}, f32);
+        if (want_b) db = at::zeros({C}, f32);
+      } else {
+        const Rows dy = rows2d(g[0]);
+        Rows dres;
+        if (g.size() > 1 && g[1].defined()) dres = rows2d(g[1]);
+        if (want_g) dg = at::empty({C}, f32);
+        if (want_b) db = at::empty({C}, f32);
+        const long n = aql_layernorm_train_scratch_floats(M, (int)C);
+        const Tensor scratch = at::empty({n}, f32);
+        const auto st = stream_of(dx);
+        ran(aql_layernorm_train_bwd(ptr(x), ptr<uint8_t>(codes), ptr<uint8_t>(exps), dy.t.data_ptr(), ptr(dres.t), dt(dx), M, (int)C,
+                                    x.defined() && M > 1 ? x.stride(0) : C, dy.ld, dres.ld, gamma.data_ptr(), dt(gamma), ptr<float>(stats), dx.data_ptr(), C,
+                                    ptr<float>(dg), ptr<float>(db), ptr<float>(scratch), n, st), "aql_layernorm_train_bwd", st);
+      }
+      if (gamma.scalar_type() != at::kFloat) {
+        if (dg.defined()) dg = dg.to(gamma.scalar_type());
+        if (db.defined()) db = db.to(gamma.scalar_type());
+      }
+    }
+    return once({dx, dg, db, Tensor(), Tensor(), Tensor()}, "layernorm_train");
+  }
+};
+
+py::object layernorm_train(const Tensor& x, const Tensor& gamma, const std::optional<Tensor>& beta_, double eps, bool ckpt8, bool passthrough) {
+  if (x.dim() != 2) bad_value("layernorm_train: expected [rows, columns], got " + shape_of(x));
+  if (!bf16_or_f32(x)) bad_value(std::string("layernorm_train: bfloat16 or float32 rows, not ") + c10::toString(x.scalar_type()));
+  const long C = x.size(1);
+  const Tensor beta = beta_ ? *beta_ : Tensor();
+  for (const Tensor* p : {&gamma, &beta}) {
+    if (!p->defined()) continue;
+    if (p->dim() != 1 || p->size(0) != C || !bf16_or_f32(*p) || p->device() != x.device() || (C > 1 && p->stride(0) != 1))
+      bad_value("layernorm_train: gamma and beta must be contiguous bfloat16 / float32 [" + std::to_string(C) + "] on " + x.device().str());
+    if (p->scalar_type() != gamma.scalar_type()) bad_value("layernorm_train: gamma and beta must have the same type");
+  }
+  if (C < 1 || C > 8192) bad_value("layernorm_train: 1 to 8192 columns, not " + std::to_string(C));
+  here(x, "layernorm_train");
+  variable_list out = LayerNormTrain::apply(x, gamma, beta_, eps, ckpt8, passthrough);
+  if (passthrough) return py::make_tuple(out[0], out[1]);
+  return py::cast(out[0]);
+}
+
+// ------------------------------------------------------------------------------------------------------- adapters of many requests
+struct Bank {   // the device side of adapters.AdapterBank
+  Tensor a, b, at, bt, ranks, scales;
+  long G = 0, r = 0, R = 0, K = 0, N = 0, serial = 0;
+  bool trainable = false;
+};
+
+struct Plan {   // the device side of adapters.RequestPlan
+  Tensor table;
+  std::vector<long> start;   // host copy, in units
+  long units = 0, requests = 0, live_units = 0;
+  int nseg = 0, nsorted = 0, nused = 0, nslot = 0, max_id = -1;
+  bool equal = false;
+  std::vector<long> at;      // offsets of start, id, seg_start, seg_pos, used_pos, used_id, slot in the table
+  std::unordered_map<long, int> slots_by_unit;
+
+  const int* part(int k) const { return (const int*)table.data_ptr() + at[k]; }
+  long unit(long rows) const {   // rows per table unit for a call on `rows` rows
+    if (!equal) {
+      if (rows != units) bad_value("RequestPlan: the requests have " + std::to_string(units) + " rows, the call " + std::to_string(rows));
+      return 1;
+    }
+    if (requests == 0) {
+      if (rows) bad_value("RequestPlan: no requests for " + std::to_string(rows) + " rows");
+      return 1;
+    }
+    if (rows % requests) bad_value("RequestPlan: " + std::to_string(rows) + " rows do not divide among " + std::to_string(requests) + " equal requests");
+    return std::max(1L, rows / requests);
+  }
+  int slots(long unit) {   // the most segments that meet in 16 rows [16 i, 16 i + 16)
+    auto it = slots_by_unit.find(unit);
+    if (it != slots_by_unit.end()) return it->second;
+    int most = 0, count = 0;
+    long tile = -1;
+    for (size_t k = 1; k + 1 < start.size(); ++k) {
+      const long row = start[k] * unit;
+      if (row % 16 == 0) continue;
+      count = row / 16 == tile ? count + 1 : 1;
+      tile = row / 16;
+      most = std::max(most, count);
+    }
+    return slots_by_unit[unit] = 1 + most;
+  }
+};
+
+struct Call : torch::CustomClassHolder {   // what a backward pass of adapter_linear needs besides tensors
+  std::shared_ptr<Bank> bank;
+  std::shared_ptr<Plan> plan;
+  Tensor w, wt, bias;
+  long unit = 1, serial = 0, M = 0, N = 0, K = 0;
+  bool train = false, residual = false;
+};
+
+// one pass of aql_adapter_linear -> (y [M, N], T [M, R] or undefined)
+std::pair<Tensor, Tensor> product(const Rows& x, const Tensor& w, const Tensor& bias, const Rows& res, const Tensor& a, const Tensor& b, const Bank& bank,
+                                  Plan& plan, long unit, long N, long K) {
+  const long M = x.t.size(0);
+  Tensor y = at::empty({M, N}, x.t.options().requires_grad(false)), T;
+  if (plan.nseg) T = at::empty({M, bank.R}, x.t.options().dtype(at::kFloat).requires_grad(false));
+  const auto st = stream_of(y);
+  ran(aql_adapter_linear(ptr<bf16_t>(x.t), x.ld, ptr<bf16_t>(w), K, ptr<bf16_t>(bias), ptr<bf16_t>(res.t), res.ld, ptr<bf16_t>(y), N, M, (int)N, (int)K,
+                         ptr<bf16_t>(a), ptr<bf16_t>(b), ptr<int>(bank.ranks), ptr<float>(bank.scales), (int)bank.R, plan.part(0), plan.part(1), plan.nseg,
+                         (int)unit, plan.slots(unit), ptr<float>(T), st), "aql_adapter_linear", st);
+  return {y, T};
+}
+
+Tensor down(const Rows& x, const Tensor& codes, const Tensor& exps, long M, long K, const Tensor& a, const Bank& bank, Plan& plan, long unit) {
+  Tensor T = at::empty({M, bank.R}, a.options().dtype(at::kFloat));
+  const auto st = stream_of(T);
+  ran(aql_adapter_down(ptr<bf16_t>(x.t), x.ld, ptr<uint8_t>(codes), ptr<uint8_t>(exps), M, (int)K, ptr<bf16_t>(a), ptr<int>(bank.ranks), ptr<float>(bank.scales),
+                       (int)bank.R, plan.part(0), plan.part(1), plan.nseg, (int)unit, plan.slots(unit), ptr<float>(T), st), "aql_adapter_down", st);
+  return T;
+}
+
+// fp32 gradient of a stack: [G, r, C], or [G, C, r] with `trans`
+Tensor wgrad(const Tensor& u, const Rows& v, const Tensor& codes, const Tensor& exps, long M, long C, bool trans, const Bank& bank, const Plan& plan, long unit) {
+  const auto f32 = bank.scales.options();
+  Tensor out = trans ? at::empty({bank.G, C, bank.r}, f32) : at::empty({bank.G, bank.r, C}, f32);
+  const long rows = plan.live_units * unit;
+  const int n = aql_adapter_wgrad_scratch_floats(rows, plan.nused, (int)C, (int)bank.R);
+  if (n < 0) throw AqlErr("adapter_linear: the weight gradients' workspace passes 2^31 elements; train fewer rows or adapters per call");
+  const Tensor scratch = at::empty({n}, f32);
+  const auto st = stream_of(out);
+  ran(aql_adapter_wgrad(ptr<float>(u), (int)bank.R, ptr<bf16_t>(v.t), v.ld, ptr<uint8_t>(codes), ptr<uint8_t>(exps), M, (int)C, (int)bank.G, (int)bank.r,
+                        ptr<int>(bank.ranks), plan.part(2), plan.part(3), plan.part(4), plan.part(5), plan.part(6), plan.nsorted, plan.nused, plan.nslot, (int)unit,
+                        rows, trans, ptr<float>(out), n ? ptr<float>(scratch) : nullptr, n, st), "aql_adapter_wgrad", st);
+  return out;
+}
+
+struct AdapterLinear : torch::autograd::Function<AdapterLinear> {
+  // ckpt8: the backward pass keeps X in 8 bits -- T is computed again from the codes, and dA and dB see their values in the place of X
+  static Tensor forward(AutogradContext* ctx, const Tensor& x2d, const Tensor& /*down*/, const Tensor& /*up*/, const std::optional<Tensor>& residual,
+                        c10::intrusive_ptr<Call> c, bool ckpt8, bool train) {
+    Rows x = gemm_rows(x2d), res;
+    if ((c->residual = residual.has_value())) res = gemm_rows(*residual);
+    auto [y, T] = product(x, c->w, c->bias, res, c->bank->a, c->bank->b, *c->bank, *c->plan, c->unit, c->N, c->K);
+    Tensor codes, exps, keep = x.t;
+    c->train = train;
+    if (!train) {
+      keep = T = Tensor();
+    } else if (ckpt8) {
+      std::tie(codes, exps) = act8_alloc(c->M, c->K, y);
+      const auto st = stream_of(y);
+      ran(aql_act8_pack(x.t.data_ptr(), 0, c->M, (int)c->K, x.ld, ptr<uint8_t>(codes), ptr<uint8_t>(exps), st), "aql_act8_pack", st);
+      keep = T = Tensor();
+    }
+    ctx->save_for_backward({keep, T, codes, exps});
+    ctx->saved_data["call"] = c10::IValue::make_capsule(c);
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto c = c10::static_intrusive_pointer_cast<Call>(ctx->saved_data["call"].toCapsule());
+    const Bank& bank = *c->bank;
+    const variable_list s = ctx->get_saved_variables();
+    const bool want_x = ctx->needs_input_grad(0), want_a = ctx->needs_input_grad(1), want_b = ctx->needs_input_grad(2), want_r = c->residual && ctx->needs_input_grad(3);
+    variable_list out(7);
+    if (!g[0].defined()) return out;
+    here(g[0], "adapter_linear backward");
+    if (bank.serial != c->serial) throw AqlErr("adapter_linear: the bank's weights changed between the forward pass and its backward pass");
+    {
+      at::AutoGradMode off(false);
+      if (c->M == 0) {
+        if (want_x) out[0] = at::empty({0, c->K}, g[0].options());
+        if (want_a) out[1] = at::zeros({bank.G, bank.r, bank.K}, bank.scales.options());
+        if (want_b) out[2] = at::zeros({bank.G, bank.N, bank.r}, bank.scales.options());
+      } else {
+        const Rows dy = gemm_rows(g[0]);
+        Tensor dT, T = s[1];
+        Rows x;
+        if (s[0].defined()) x = {s[0], c->M > 1 ? s[0].stride(0) : c->K};
+        if (want_x) std::tie(out[0], dT) = product(dy, c->wt, Tensor(), Rows(), bank.bt, bank.at, bank, *c->plan, c->unit, c->K, c->N);
+        if (c->train) {
+          if (want_a) {
+            if (!dT.defined() && c->plan->nseg) dT = down(dy, Tensor(), Tensor(), c->M, c->N, bank.bt, bank, *c->plan, c->unit);
+            out[1] = wgrad(dT, x, s[2], s[3], c->M, c->K, false, bank, *c->plan, c->unit);
+          }
+          if (want_b) {
+            if (!T.defined() && c->plan->nseg) T = down(Rows(), s[2], s[3], c->M, c->K, bank.a, bank, *c->plan, c->unit);
+            out[2] = wgrad(T, dy, Tensor(), Tensor(), c->M, c->N, true, bank, *c->plan, c->unit);
+          }
+        }
+      }
+      if (want_r) out[3] = g[0];
+    }
+    return once(std::move(out), "adapter_linear");
+  }
+};
+
+Tensor adapter_linear(const Tensor& x, const Tensor& w, const Tensor& wt, const std::optional<Tensor>& bias_, const std::shared_ptr<Bank>& bank,
+                      const std::shared_ptr<Plan>& plan, const Tensor& down, const Tensor& up,
+                      const std::optional<Tensor>& residual_, bool ckpt8) {
+  const long N = w.size(0), K = w.size(1);
+  if (x.dim() != 2 || x.scalar_type() != at::kBFloat16)
+    bad_value("adapter_linear: expected bfloat16 [rows, " + std::to_string(K) + "], got " + c10::toString(x.scalar_type()) + " " + shape_of(x));
+  const long M = x.size(0);
+  if (x.size(1) != K || bank->K != K || bank->N != N)
+    bad_value("adapter_linear: input " + shape_of(x) + ", projection [" + std::to_string(N) + ", " + std::to_string(K) + "], adapters on [" +
+              std::to_string(bank->N) + ", " + std::to_string(bank->K) + "]");
+  if (plan->max_id >= bank->G)
+    bad_value("adapter_linear: the plan names adapter " + std::to_string(plan->max_id) + ", the bank has " + std::to_string(bank->G));
+  const long unit = plan->unit(M);
+  const Tensor res = residual_ ? *residual_ : Tensor(), bias = bias_ ? *bias_ : Tensor();
+  if (res.defined() && (res.dim() != 2 || res.size(0) != M || res.size(1) != N || res.scalar_type() != at::kBFloat16))
+    bad_value("adapter_linear: residual must be bfloat16 [" + std::to_string(M) + ", " + std::to_string(N) + "], not " + shape_of(res));
+  here(x, "adapter_linear");
+  if (bank->a.device() != x.device() || plan->table.device() != x.device() || w.device() != x.device() || (res.defined() && res.device() != x.device()))
+    bad_value("adapter_linear: input, projection, adapters, plan and residual must live on one device");
+  const bool train = bank->trainable && at::GradMode::is_enabled() && (down.requires_grad() || up.requires_grad());
+  if (at::GradMode::is_enabled() && (train || x.requires_grad() || (res.defined() && res.requires_grad()))) {
+    auto c = c10::make_intrusive<Call>();
+    c->bank = bank, c->plan = plan, c->w = w, c->wt = wt, c->bias = bias, c->unit = unit, c->serial = bank->serial, c->M = M, c->N = N, c->K = K;
+    return AdapterLinear::apply(x, down, up, residual_, c, ckpt8, train);
+  }
+  Rows r;
+  if (res.defined()) r = gemm_rows(res);
+  return product(gemm_rows(x), w, bias, r, bank->a, bank->b, *bank, *plan, unit, N, K).first;
+}
+
+}  // namespace
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  m.def("set_error_class", [](py::object cls) { aql_error_class = cls.release(); });
+  py::register_exception_translator([](std::exception_ptr p) {
+    try {
+      if (p) std::rethrow_exception(p);
+    } catch (const AqlErr& e) {
+      PyErr_SetString(aql_error_class.ptr() ? aql_error_class.ptr() : PyExc_RuntimeError, e.what());
+    }
+  });
+  m.def("abi_version", [] { return aql_abi_version(); });
+  m.def("act8_pack", &act8_pack);
+  m.def("act8_unpack", &act8_unpack);
+  m.def("layernorm_train", &layernorm_train);
+  m.def("adapter_linear", &adapter_linear);
+  py::class_<Bank, std::shared_ptr<Bank>>(m, "Bank")
+      .def(py::init<>())
+      .def_readwrite("a", &Bank::a).def_readwrite("b", &Bank::b).def_readwrite("at", &Bank::at).def_readwrite("bt", &Bank::bt)
+      .def_readwrite("ranks", &Bank::ranks).def_readwrite("scales", &Bank::scales)
+      .def_readwrite("G", &Bank::G).def_readwrite("r", &Bank::r).def_readwrite("R", &Bank::R).def_readwrite("K", &Bank::K).def_readwrite("N", &Bank::N)
+      .def_readwrite("serial", &Bank::serial).def_readwrite("trainable", &Bank::trainable);
+  py::class_<Plan, std::shared_ptr<Plan>>(m, "Plan")
+      .def(py::init<>())
+      .def_readwrite("table", &Plan::table).def_readwrite("start", &Plan::start).def_readwrite("at", &Plan::at)
+      .def_readwrite("units", &Plan::units).def_readwrite("requests", &Plan::requests).def_readwrite("live_units", &Plan::live_units)
+      .def_readwrite("nseg", &Plan::nseg).def_readwrite("nsorted", &Plan::nsorted).def_readwrite("nused", &Plan::nused).def_readwrite("nslot", &Plan::nslot)
+      .def_readwrite("max_id", &Plan::max_id).def_readwrite("equal", &Plan::equal)
+      .def("unit", &Plan::unit).def("slots", &Plan::slots);
+}

@@ -2019,32 +2019,13 @@ def layernorm_res(x2d, gamma, beta, eps=1e-5):
     return LayerNormFn.apply(x2d, gamma, beta, eps, True)
 
 
-# ------------------------------------------------------------------- 8-bit activation checkpoints
-_ACT_DT = {torch.bfloat16: 0, torch.float32: 1}
-
-
-def _here(t, name):
-    """The kernels run on the current device's current stream: a tensor of another device is refused, not followed."""
-    _req(t, name)
-    if t.device.index != torch.cuda.current_device():
-        raise L.AqlError(f"{name}: tensor on {t.device}, but the current device is cuda:{torch.cuda.current_device()}; "
-                         "wrap the call in torch.cuda.device(...)")
-    if DUAL is not None and _full(t) is not None:
-        raise L.AqlError(f"{name} does not take twin batches")
-    return t
-
-
-def _rows2d(t, name):
-    """-> (t, row stride) with unit column stride and rows that do not overlap (a copy where t has neither)."""
-    if t.dim() != 2:
-        raise ValueError(f"{name}: expected [rows, columns], got {tuple(t.shape)}")
-    M, C = t.shape
-    if M <= 1:
-        t = t if t.is_contiguous() else t.contiguous()
-        return t, C
-    if t.stride(1) != 1 or t.stride(0) < C:
-        t = t.contiguous()
-    return t, t.stride(0)
+# ------------------------------------------------------------------- training operators bound in C++ (csrc/aql_torch.cpp)
+def _plain(t, name):
+    """These operators know nothing of held-back finalize launches and twin batches."""
+    if _PENDING or DUAL is not None:
+        _req(t, name)
+        if t.is_cuda and _full(t) is not None:
+            raise L.AqlError(f"{name} does not take twin batches")
 
 
 class Act8:
@@ -2052,251 +2033,48 @@ class Act8:
     ``codes`` uint8 [M, Cp] (two's complement), ``exps`` uint8 [M, Cp / 32] (step = 2^(exp - 127)), Cp = C rounded up to 32."""
 
     def __init__(self, codes, exps, shape, dtype):
-        self.codes, self.exps, self.shape, self.dtype = codes, exps, tuple(shape), dtype
+        self.codes, self.exps, self.shape, self.dtype = codes, exps, shape, dtype
 
     def unpack(self, dtype=None):
         """The values that the codes stand for, in the packed tensor's shape and type (or fp32 / bf16 on request: exact in both)."""
         dtype = self.dtype if dtype is None else dtype
-        if dtype not in _ACT_DT:
+        if dtype is not torch.bfloat16 and dtype is not torch.float32:
             raise ValueError(f"Act8.unpack: bfloat16 or float32, not {dtype}")
-        _here(self.codes, "Act8.unpack")
-        C = self.shape[-1]
-        out = torch.empty(self.shape, dtype=dtype, device=self.codes.device)
-        L.call("aql_act8_unpack", self.codes.data_ptr(), self.exps.data_ptr(), self.codes.shape[0], C, out.data_ptr(), _ACT_DT[dtype], C, L.stream_ptr())
-        return out
-
-
-def _act8_alloc(M, C, device):
-    Cp = (C + 31) // 32 * 32
-    return torch.empty(M, Cp, dtype=torch.uint8, device=device), torch.empty(M, Cp // 32, dtype=torch.uint8, device=device)
+        return L.native().act8_unpack(self.codes, self.exps, self.shape, dtype is torch.bfloat16)
 
 
 def act8_pack(x):
     """bf16 / fp32 ``x`` [..., C] -> Act8.  A value is off by at most half its block's step, 2^e / 2 with 63.75 2^e < max|block| (blocks whose
     magnitudes reach from 2^-120 to 2^127); a block with an infinity or a NaN comes back as NaN.  No gradient flows through it."""
-    if x.dtype not in _ACT_DT:
-        raise ValueError(f"act8_pack: bfloat16 or float32, not {x.dtype}")
-    if x.dim() < 1 or x.shape[-1] == 0:
-        raise ValueError(f"act8_pack: expected [..., columns], got {tuple(x.shape)}")
-    _here(x, "act8_pack")
-    C = x.shape[-1]
-    x2, ld = _rows2d(x.detach().reshape(-1, C), "act8_pack")
-    codes, exps = _act8_alloc(x2.shape[0], C, x.device)
-    L.call("aql_act8_pack", x2.data_ptr(), _ACT_DT[x.dtype], x2.shape[0], C, ld, codes.data_ptr(), exps.data_ptr(), L.stream_ptr())
-    return Act8(codes, exps, x.shape, x.dtype)
-
-
-# ------------------------------------------------------------------- LayerNorm with weight gradients
-class LayerNormTrainFn(torch.autograd.Function):
-    """LayerNorm whose gamma / beta are trained (``layernorm`` is the frozen form): dgamma, dbeta summed over the rows in fp32 in a fixed
-    order.  ``ckpt8``: the backward pass keeps x in 8 bits and computes xh = (x8 - mean) rstd from the codes."""
-
-    @staticmethod
-    def forward(ctx, x, gamma, beta, eps, ckpt8, passthrough):
-        M, C = x.shape
-        x2, ldx = _rows2d(x, "layernorm_train")
-        y = torch.empty(M, C, dtype=x.dtype, device=x.device)
-        stats = torch.empty(M, 2, dtype=torch.float32, device=x.device)
-        codes, exps = _act8_alloc(M, C, x.device) if ckpt8 else (None, None)
-        L.call("aql_layernorm_train_fwd", x2.data_ptr(), _ACT_DT[x.dtype], M, C, ldx, gamma.data_ptr(), L.ptr(beta), _ACT_DT[gamma.dtype], float(eps),
-               y.data_ptr(), C, stats.data_ptr(), L.ptr(codes), L.ptr(exps), L.stream_ptr())
-        ctx.save_for_backward(None if ckpt8 else x2, codes, exps, gamma, stats)
-        ctx.has_beta = beta is not None
-        if passthrough:
-            return y, x.view_as(x)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy, dres=None):
-        x2, codes, exps, gamma, stats = ctx.saved_tensors
-        _here(dy, "layernorm_train backward")
-        M, C = dy.shape
-        _, want_g, want_b = ctx.needs_input_grad[:3]
-        want_b = want_b and ctx.has_beta
-        dx = torch.empty(M, C, dtype=dy.dtype, device=dy.device)
-        if M == 0:
-            z = torch.zeros(C, dtype=gamma.dtype, device=dy.device)
-            return dx, z if want_g else None, z.clone() if want_b else None, None, None, None
-        dy, lddy = _rows2d(dy, "layernorm_train")
-        lddres = 0
-        if dres is not None:
-            dres, lddres = _rows2d(dres, "layernorm_train")
-        dg = torch.empty(C, dtype=torch.float32, device=dy.device) if want_g else None
-        db = torch.empty(C, dtype=torch.float32, device=dy.device) if want_b else None
-        n = L.call_raw("aql_layernorm_train_scratch_floats", M, C)
-        scratch = torch.empty(n, dtype=torch.float32, device=dy.device)
-        L.call("aql_layernorm_train_bwd", L.ptr(x2), L.ptr(codes), L.ptr(exps), dy.data_ptr(), L.ptr(dres), _ACT_DT[dy.dtype], M, C,
-               C if x2 is None or M == 1 else x2.stride(0), lddy, lddres, gamma.data_ptr(), _ACT_DT[gamma.dtype], stats.data_ptr(), dx.data_ptr(), C,
-               L.ptr(dg), L.ptr(db), scratch.data_ptr(), n, L.stream_ptr())
-        if dg is not None and gamma.dtype != torch.float32:
-            dg = dg.to(gamma.dtype)
-        if db is not None and gamma.dtype != torch.float32:
-            db = db.to(gamma.dtype)
-        return dx, dg, db, None, None, None
-
-
-def _layernorm_train(x2d, gamma, beta, eps, ckpt8, passthrough):
-    if x2d.dim() != 2:
-        raise ValueError(f"layernorm_train: expected [rows, columns], got {tuple(x2d.shape)}")
-    if x2d.dtype not in _ACT_DT:
-        raise ValueError(f"layernorm_train: bfloat16 or float32 rows, not {x2d.dtype}")
-    C = x2d.shape[1]
-    for p, n in ((gamma, "gamma"), (beta, "beta")):
-        if p is None and n == "beta":
-            continue
-        if tuple(p.shape) != (C,) or p.dtype not in _ACT_DT or p.device != x2d.device or (C > 1 and p.stride(0) != 1):
-            raise ValueError(f"layernorm_train: {n} must be a contiguous bfloat16 / float32 [{C}] on {x2d.device}")
-        if p.dtype != gamma.dtype:
-            raise ValueError("layernorm_train: gamma and beta must have the same type")
-    if not 1 <= C <= 8192:
-        raise ValueError(f"layernorm_train: 1 to 8192 columns, not {C}")
-    _here(x2d, "layernorm_train")
-    return LayerNormTrainFn.apply(x2d, gamma, beta, eps, bool(ckpt8), passthrough)
+    _plain(x, "act8_pack")
+    codes, exps = L.native().act8_pack(x)
+    return Act8(codes, exps, tuple(x.shape), x.dtype)
 
 
 def layernorm_train(x2d, gamma, beta=None, eps=1e-5, ckpt8=False):
-    """LayerNorm over the columns of ``x2d`` [M, C] (bf16 or fp32, C <= 8192) with gradients for x, gamma and beta (bf16 or fp32 [C]).
-    ``ckpt8`` keeps x in 8 bits for the backward pass (1.03 bytes per value instead of 2 or 4)."""
-    return _layernorm_train(x2d, gamma, beta, eps, ckpt8, False)
+    """LayerNorm over the columns of ``x2d`` [M, C] (bf16 or fp32, C <= 8192, any row stride) whose weights are trained (``layernorm`` is the frozen
+    form): gradients for x, gamma and beta (bf16 or fp32 [C]), the latter summed over the rows in fp32 in a fixed order.  ``ckpt8`` keeps x in
+    8 bits for the backward pass (1.03 bytes per value instead of 2 or 4), which then sees (x8 - mean) rstd."""
+    _plain(x2d, "layernorm_train")
+    return L.native().layernorm_train(x2d, gamma, beta, eps, ckpt8, False)
 
 
 def layernorm_train_res(x2d, gamma, beta=None, eps=1e-5, ckpt8=False):
     """-> (normalised, x2d) with the residual gradient folded into the backward kernel (the form of ``layernorm_res``)."""
-    return _layernorm_train(x2d, gamma, beta, eps, ckpt8, True)
-
-
-# ------------------------------------------------------------------- many requests' adapters beside one projection
-def _stream(t):
-    return torch._C._cuda_getCurrentRawStream(t.device.index)
-
-
-def _gemm_rows(t):
-    """-> (t, row stride): rows as the matrix kernels read them -- unit column stride, 16-byte aligned, a multiple of 8 elements apart."""
-    C = t.shape[1]
-    if t.shape[0] <= 1:
-        t = t if t.is_contiguous() else t.contiguous()
-        ld = C
-    else:
-        if t.stride(1) != 1 or t.stride(0) < C or t.stride(0) % 8 or t.stride(0) >= 1 << 21:
-            t = t.contiguous()
-        ld = t.stride(0)
-    if t.data_ptr() & 15:
-        t = t.clone(memory_format=torch.contiguous_format)
-        ld = C
-    return t, ld
-
-
-def _adapter_product(x, ldx, w, bias, res, ldr, a, b, bank, plan, unit, N, K):
-    """One pass of aql_adapter_linear -> (y [M, N], T [M, R] or None)."""
-    M = x.shape[0]
-    y = torch.empty(M, N, dtype=torch.bfloat16, device=x.device)
-    T = torch.empty(M, bank.R, dtype=torch.float32, device=x.device) if plan.nseg else None
-    L.call("aql_adapter_linear", x.data_ptr(), ldx, w.data_ptr(), K, None if bias is None else bias.data_ptr(),
-           None if res is None else res.data_ptr(), ldr, y.data_ptr(), N, M, N, K, a.data_ptr(), b.data_ptr(), bank.ranks_dev.data_ptr(),
-           bank.scales_dev.data_ptr(), bank.R, plan.fwd_ptrs[0], plan.fwd_ptrs[1], plan.nseg, unit, plan.slots(unit),
-           None if T is None else T.data_ptr(), _stream(x))
-    return y, T
-
-
-def _adapter_down(x, ldx, codes, exps, M, K, a, bank, plan, unit, like):
-    T = torch.empty(M, bank.R, dtype=torch.float32, device=like.device)
-    L.call("aql_adapter_down", None if x is None else x.data_ptr(), ldx, L.ptr(codes), L.ptr(exps), M, K, a.data_ptr(), bank.ranks_dev.data_ptr(),
-           bank.scales_dev.data_ptr(), bank.R, plan.fwd_ptrs[0], plan.fwd_ptrs[1], plan.nseg, unit, plan.slots(unit), T.data_ptr(), _stream(like))
-    return T
-
-
-def _adapter_wgrad(u, v, ldv, codes, exps, M, C, trans, bank, plan, unit, like):
-    """fp32 gradient of a stack: [G, r, C], or [G, C, r] with ``trans``."""
-    r = bank.rank
-    out = torch.empty((bank.G, C, r) if trans else (bank.G, r, C), dtype=torch.float32, device=like.device)
-    rows = plan.live_units * unit
-    n = L.call_raw("aql_adapter_wgrad_scratch_floats", rows, plan.nused, C, bank.R)
-    if n < 0:
-        raise L.AqlError("adapter_linear: the weight gradients' workspace passes 2^31 elements; train fewer rows or adapters per call")
-    scratch = torch.empty(n, dtype=torch.float32, device=like.device)
-    L.call("aql_adapter_wgrad", L.ptr(u), bank.R, L.ptr(v), ldv, L.ptr(codes), L.ptr(exps), M, C, bank.G, r, bank.ranks_dev.data_ptr(), *plan.grad_ptrs,
-           plan.nsorted, plan.nused, plan.nslot, unit, rows, int(trans), out.data_ptr(), scratch.data_ptr() if n else None, n, _stream(like))
-    return out
-
-
-class AdapterLinearFn(torch.autograd.Function):
-    """Y = X.W^T + b + residual + s_g (X.A_g^T).B_g^T with g by request (adapters.AdapterBank, adapters.RequestPlan).  Gradients: dX, dA, dB (fp32), residual.
-    ``ckpt8``: the backward pass keeps X in 8 bits -- T is computed again from the codes, and dA and dB see their values in the place of X."""
-
-    @staticmethod
-    def forward(ctx, x2d, down, up, residual, packed, bank, plan, unit, ckpt8):
-        x, ldx = _gemm_rows(x2d)
-        res, ldr = (None, 0) if residual is None else _gemm_rows(residual)
-        y, T = _adapter_product(x, ldx, packed.w, packed.bias, res, ldr, bank.a, bank.b, bank, plan, unit, packed.N, packed.K)
-        ctx.packed, ctx.bank, ctx.plan, ctx.unit, ctx.serial, ctx.ckpt8 = packed, bank, plan, unit, bank.serial, ckpt8
-        ctx.train = bank.trainable and (ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
-        codes = exps = None
-        if not ctx.train:
-            x = T = None
-        elif ckpt8:
-            M, K = x.shape
-            codes, exps = _act8_alloc(M, K, x.device)
-            L.call("aql_act8_pack", x.data_ptr(), 0, M, K, ldx, codes.data_ptr(), exps.data_ptr(), _stream(x))
-            x = T = None
-        ctx.save_for_backward(x, T, codes, exps)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        _here(dy, "adapter_linear backward")
-        x, T, codes, exps = ctx.saved_tensors
-        packed, bank, plan, unit = ctx.packed, ctx.bank, ctx.plan, ctx.unit
-        want_x, want_a, want_b, want_r = ctx.needs_input_grad[:4]
-        if bank.serial != ctx.serial:
-            raise L.AqlError("adapter_linear: the bank's weights changed between the forward pass and its backward pass")
-        dy2, lddy = _gemm_rows(dy)
-        M, N, K = dy2.shape[0], packed.N, packed.K
-        dx = dA = dB = dT = None
-        if M == 0:
-            zeros = lambda p: torch.zeros_like(p, dtype=torch.float32)  # noqa: E731
-            return (dy.new_empty(0, K), zeros(bank.down) if want_a else None, zeros(bank.up) if want_b else None, dy if want_r else None) + (None,) * 5
-        if want_x:
-            bt, at = bank.transposed()
-            dx, dT = _adapter_product(dy2, lddy, packed.wt, None, None, 0, bt, at, bank, plan, unit, K, N)
-        if ctx.train:
-            if want_a:
-                if dT is None and plan.nseg:
-                    dT = _adapter_down(dy2, lddy, None, None, M, N, bank.transposed()[0], bank, plan, unit, dy2)
-                dA = _adapter_wgrad(dT, x, 0 if x is None else (K if M <= 1 else x.stride(0)), codes, exps, M, K, False, bank, plan, unit, dy2)
-            if want_b:
-                if T is None and plan.nseg:
-                    T = _adapter_down(None, 0, codes, exps, M, K, bank.a, bank, plan, unit, dy2)
-                dB = _adapter_wgrad(T, dy2, lddy, None, None, M, N, True, bank, plan, unit, dy2)
-        return dx, dA, dB, (dy if want_r else None), None, None, None, None, None
+    _plain(x2d, "layernorm_train")
+    return L.native().layernorm_train(x2d, gamma, beta, eps, ckpt8, True)
 
 
 def adapter_linear(x2d, packed, bank, plan, residual=None, ckpt8=False):
-    """``x2d`` [M, K] bf16 through ``packed`` (PackedLinear, K and N multiples of 8) with every request's own adapter -> [M, N] bf16.
-    ``bank``: adapters.AdapterBank of this projection; ``plan``: adapters.RequestPlan whose requests make up the M rows; ``residual`` [M, N] is
-    added before the one rounding.  Differentiable in x2d, residual and a trainable bank's down / up; ``ckpt8`` keeps x2d in 8 bits for the latter."""
-    if x2d.dim() != 2 or x2d.dtype != torch.bfloat16:
-        raise ValueError(f"adapter_linear: expected bfloat16 [rows, {packed.K}], got {x2d.dtype} {tuple(x2d.shape)}")
-    M, K = x2d.shape
-    N = packed.N
-    if K != packed.K or bank.K != K or bank.N != N:
-        raise ValueError(f"adapter_linear: input of width {K}, projection [{packed.N}, {packed.K}], adapters on [{bank.N}, {bank.K}]")
-    if plan.max_id >= bank.G:
-        raise ValueError(f"adapter_linear: the plan names adapter {plan.max_id}, the bank has {bank.G}")
-    unit = plan.unit(M)
-    if residual is not None and (tuple(residual.shape) != (M, N) or residual.dtype != torch.bfloat16):
-        raise ValueError(f"adapter_linear: residual must be bfloat16 [{M}, {N}], not {residual.dtype} {tuple(residual.shape)}")
-    _here(x2d, "adapter_linear")
-    if bank.a.device != x2d.device or plan.table.device != x2d.device or packed.w.device != x2d.device or (residual is not None and residual.device != x2d.device):
-        raise ValueError("adapter_linear: input, projection, adapters, plan and residual must live on one device")
+    """Y = X.W^T + b + residual + s_g (X.A_g^T).B_g^T, g by request: ``x2d`` [M, K] bf16 through ``packed`` (PackedLinear, K and N multiples of 8) with
+    every request's own adapter -> [M, N] bf16, one fp32 accumulator and one rounding.  ``bank``: adapters.AdapterBank of this projection;
+    ``plan``: adapters.RequestPlan whose requests make up the M rows.  Differentiable in x2d, residual and a trainable bank's down / up;
+    ``ckpt8`` keeps x2d in 8 bits for the latter: T is computed again from the codes, and dA and dB see their values in the place of X."""
+    _plain(x2d, "adapter_linear")
     bank.refresh()
-    if torch.is_grad_enabled() and (x2d.requires_grad or (residual is not None and residual.requires_grad) or
-                                    (bank.trainable and (bank.down.requires_grad or bank.up.requires_grad))):
-        return AdapterLinearFn.apply(x2d, bank.down, bank.up, residual, packed, bank, plan, unit, bool(ckpt8))
-    x, ldx = _gemm_rows(x2d)
-    res, ldr = (None, 0) if residual is None else _gemm_rows(residual)
-    return _adapter_product(x, ldx, packed.w, packed.bias, res, ldr, bank.a, bank.b, bank, plan, unit, N, K)[0]
+    if x2d.requires_grad and not bank.trainable:
+        bank.lay_out_transposed()
+    return L.native().adapter_linear(x2d, packed.w, packed.wt, packed.bias, bank.handle, plan.handle, bank.down, bank.up, residual, ckpt8)
 
 
 class GegluFn(torch.autograd.Function):

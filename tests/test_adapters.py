@@ -142,6 +142,10 @@ def test_frozen_input_or_frozen_adapters():
     x = d["x"].to(DEV).requires_grad_(True)
     dx, = torch.autograd.grad(ops.adapter_linear(x, packed, bank, plan), x, dy)
     check("dx", dx, ref[1], slack[1], HALF)
+    y = ops.adapter_linear(x, packed, handles(d, lengths, ids, equal, True)[1], plan)
+    g, = torch.autograd.grad(y.float().square().sum(), x, create_graph=True)       # no second derivative: refused, not dropped
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
     with torch.no_grad():
         assert not ops.adapter_linear(x, packed, bank, plan).requires_grad
 
@@ -274,7 +278,7 @@ def test_bank_follows_its_parameters():
     half = dict(d, up=(d["up"].float() * 0.5).to(torch.bfloat16))
     ref, slack = reference(half, rows, ids, False, d["x"])
     check("y", ops.adapter_linear(x, packed, bank, plan), ref[0], slack[0], HALF)
-    with pytest.raises(_lib.AqlError):
+    with pytest.raises(RuntimeError):
         y.sum().backward()                              # the weights changed after that forward pass
     opt = torch.optim.SGD(bank.parameters(), lr=0.25)
     ops.adapter_linear(x, packed, bank, plan).backward(d["dy"].to(DEV))
@@ -282,8 +286,8 @@ def test_bank_follows_its_parameters():
     opt.step()
     assert torch.equal(bank.up.detach(), new_up)
     ops.adapter_linear(x, packed, bank, plan)
-    assert torch.equal(bank.b[:, :, :bank.rank][:-1], (new_up * d["live"].to(DEV)[:, None, :]).to(torch.bfloat16)[:-1])
-    assert torch.equal(bank.bt, bank.b.transpose(1, 2)) and torch.equal(bank.at, bank.a.transpose(1, 2))
+    assert torch.equal(bank.handle.b[:, :, :bank.rank][:-1], (new_up * d["live"].to(DEV)[:, None, :]).to(torch.bfloat16)[:-1])
+    assert torch.equal(bank.handle.bt, bank.handle.b.transpose(1, 2)) and torch.equal(bank.handle.at, bank.handle.a.transpose(1, 2))
 
 
 @gpu

@@ -132,20 +132,19 @@ class RequestPlan:
         seg = ids[first] if ids.size else ids
         self.max_id = int(seg.max()) if seg.size else -1
         size = np.diff(start)
+        unit_id = np.repeat(seg, size)
         # sorted order of the rows that have an adapter, for the weight gradients
-        order = np.argsort(seg, kind="stable")
-        order = order[seg[order] >= 0]
-        used, count_at = np.unique(seg[order], return_index=True)
-        pos = np.r_[0, np.cumsum(size[order])]
+        perm = np.argsort(unit_id, kind="stable")[int((unit_id < 0).sum()):]
+        used, count = np.unique(unit_id[perm], return_counts=True)
+        used_pos = np.r_[0, np.cumsum(count)]
         slot = np.full(max(self.max_id + 1, 1), -1, dtype=np.int64)
         slot[used] = np.arange(used.size)
-        parts = dict(start=start, id=seg, seg_start=start[order] if order.size else order, seg_pos=pos,
-                     used_pos=np.r_[pos[count_at], pos[-1]] if used.size else pos, used_id=used, slot=slot)
+        parts = dict(unit_id=unit_id, perm=perm, used_pos=used_pos, slot=slot)
         flat = np.concatenate([p.astype(np.int32) for p in parts.values()])
         h = self.handle = L.native().Plan()  # what the kernels' binding reads
         self.table = h.table = torch.from_numpy(flat).to(dev)
         h.at = np.r_[0, np.cumsum([p.size for p in parts.values()])[:-1]].tolist()
         h.start = start.tolist()
-        h.units, h.requests, h.live_units, h.equal, h.max_id = self.units, self.requests, int(pos[-1]), self.equal, self.max_id
+        h.units, h.requests, h.live_units, h.equal, h.max_id = self.units, self.requests, int(perm.size), self.equal, self.max_id
         h.nseg = int(seg.size) if self.max_id >= 0 else 0              # no adapters at all: no segments
-        h.nsorted, h.nused, h.nslot = int(order.size), int(used.size), int(slot.size)
+        h.nused, h.nslot = int(used.size), int(slot.size)

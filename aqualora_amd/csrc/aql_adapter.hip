@@ -7,12 +7,13 @@
 //     P_g = sum over the rows of g of  U[m] V[m]^T     (aql_adapter_wgrad: dA from (dT, X), dB from (T, dY))
 // are the weight gradients.
 //
-// Rows are described by segments: rows [start[s] unit, start[s + 1] unit) have adapter id[s], -1 for none.  A tile of rows finds its segments by
-// binary search, so tiles stay dense whatever the requests' lengths; where several segments meet in a tile, the low-rank term runs once
-// per segment with the other segments' T rows taken as zeros (a select: what they hold cannot reach the sum).
+// Row m has adapter id[m / unit], -1 for none: one load, whatever the requests' lengths (a binary search over their starts cost a chain of
+// scalar loads: 15 us against 6 us where 16 requests meet in a tile of 16 rows).  Tiles of rows stay dense; the low-rank term runs once for each
+// adapter that a tile meets, with the other adapters' T rows taken as zeros (a select: what they hold cannot reach the sum).
 //
-// T is kept in fp32: the gradients dA and dB are fp32 sums of its products and would lose half their digits to a bf16 T.  Their matrix products
-// split T into three bf16 parts (24 bits); the second launch of the linear rounds T to bf16 once, where it multiplies B.
+// T is written as bf16 parts: T = hi + mid + lo, hi = T rounded to bf16, mid = the rest rounded, lo = the rest of that.  The second launch reads
+// hi alone (the one rounding of T in the linear, as in the single-adapter kernels).  The gradients dA and dB are fp32 sums of T's products
+// and would lose two thirds of their digits to a bf16 T: they read all three parts (24 bits), which only a training pass writes.
 #include "aql_act8.cuh"
 
 namespace {
@@ -20,86 +21,111 @@ namespace {
 constexpr int BK = 64;
 constexpr uint32_t OOB = 0x80000000u;
 
-struct Segs {
-  const int* start;   // [n + 1], in units
-  const int* id;      // [n]
-  int n, unit;
+struct Rows {
+  const int* id;   // adapter of each unit of rows; null: no adapters at all
+  int unit;
 };
-
-// the segment that holds `row` (0 <= row < rows of the plan); uniform arguments, scalar loads
-__device__ __forceinline__ int seg_of(const Segs& s, long row) {
-  int lo = 0, hi = s.n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if ((long)s.start[mid] * s.unit <= row) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
+__device__ __forceinline__ int id_of(const Rows& r, long row) { return r.id[r.unit == 1 ? (uint32_t)row : (uint32_t)row / (uint32_t)r.unit]; }
 
 __device__ __forceinline__ bf16x8_t zero8() { return bf16x8_t{0, 0, 0, 0, 0, 0, 0, 0}; }
 __device__ __forceinline__ bf16x8_t load8(const bf16_t* p) { return *reinterpret_cast<const bf16x8_t*>(p); }
+// loads that may be dead go to a clamped address and are selected afterwards: a load under a branch costs the branch, and the compiler, which no
+// longer knows how many loads are in flight behind it, waits for all of them
+__device__ __forceinline__ bf16x8_t keep(bf16x8_t v, bool on) {
+  union { bf16x8_t f; uint32_t w[4]; } u;
+  u.f = v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) u.w[i] = on ? u.w[i] : 0u;
+  return u.f;
+}
+__device__ __forceinline__ uint4 keep(uint4 v, bool on) { return make_uint4(on ? v.x : 0u, on ? v.y : 0u, on ? v.z : 0u, on ? v.w : 0u); }
 __device__ __forceinline__ bf16x8_t pack8(const float* v) {
   union { uint32_t w[4]; bf16x8_t f; } u;
 #pragma unroll
   for (int i = 0; i < 4; ++i) u.w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
   return u.f;
 }
-// eight fp32 T values as an operand fragment (rounded to bf16: the one rounding of T in the linear), zeros where `on` is false
-__device__ __forceinline__ bf16x8_t t_frag(const float* p, bool on) {
-  if (!on) return zero8();
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-  return pack8(v);
+// T's parts of row m: hi at T + m P R, mid and lo R and 2 R further on (P = 1: hi alone, P = 3)
+__device__ __forceinline__ void store_t4(bf16_t* t, int R, int P, const float (&v)[4]) {   // four consecutive columns
+  float r[4] = {v[0], v[1], v[2], v[3]};
+  for (int p = 0; p < P; ++p) {
+    const uint2 w = make_uint2(pack_bf16x2(r[0], r[1]), pack_bf16x2(r[2], r[3]));
+    *reinterpret_cast<uint2*>(t + p * R) = w;
+    r[0] -= bf16lo(w.x), r[1] -= bf16hi(w.x), r[2] -= bf16lo(w.y), r[3] -= bf16hi(w.y);   // exact
+  }
 }
 __device__ __forceinline__ f32x4_t mfma(bf16x8_t a, bf16x8_t b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
 // ---------------------------------------------------------------------------------------------------------------------- T = s A x
-// One workgroup: 16 rows x 16 RT adapter rows of ONE segment (blockIdx.y counts the segments of the row tile); its four wavefronts split the
-// contraction and join in LDS.  Fragments come straight from memory: lane (i = lane & 15, q = lane >> 4) holds row i, columns k + 8 q ..
-// k + 8 q + 7 of either operand, and gets T[m = lane & 15][r = 4 q + e] back.
-template <int RT, bool CODES>
-__global__ __launch_bounds__(256) void down_kernel(const bf16_t* __restrict__ X, long ldx, const uint8_t* __restrict__ codes,
-                                                   const uint8_t* __restrict__ exps, long M, int K, const bf16_t* __restrict__ A,
-                                                   const int* __restrict__ ranks, const float* __restrict__ scales, int R, Segs sg,
-                                                   float* __restrict__ T) {
-  __shared__ float red[3][RT][64][4];
+struct DownArgs {
+  const bf16_t* X;
+  const uint8_t *codes, *exps;
+  const bf16_t* A;
+  const int* ranks;
+  const float* scales;
+  bf16_t* T;
+  long ldx, M;
+  int K, R, P;
+  Rows rows;
+};
+
+// Few rows, short requests or 8-bit codes.  One workgroup: 16 rows x 16 RT adapter rows of ONE adapter (blockIdx.y counts the adapters that the row
+// tile meets); its NW wavefronts split the contraction and join in LDS.  Fragments come straight from memory, four steps of 32 columns at a time
+// (all their loads in flight together): lane (i = lane & 15, q = lane >> 4) holds row i, columns k + 8 q .. k + 8 q + 7 of either operand, and
+// gets T[m = lane & 15][r = 4 q + e] back.
+template <int RT, int NW, bool CODES>
+__global__ __launch_bounds__(NW * 64) void down_kernel(const DownArgs a) {
+  constexpr int UN = 4;
+  __shared__ float red[NW - 1][RT][64][4];
   const long m0 = (long)blockIdx.x * 16;
-  const int s = seg_of(sg, m0) + blockIdx.y;
-  if (s >= sg.n) return;
-  const long lo = max(m0, (long)sg.start[s] * sg.unit), hi = min(m0 + 16, (long)sg.start[s + 1] * sg.unit);
-  const int g = sg.id[s];
-  if (lo >= hi || g < 0) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, q = lane >> 4;
+  const int gi = m0 + i < a.M ? id_of(a.rows, m0 + i) : -1;
+  uint32_t left = (uint32_t)__ballot(gi >= 0) & 0xffffu;   // rows whose adapter has not been met yet
+  int g = -1;
+  for (int k = blockIdx.y; left; --k) {                    // the blockIdx.y-th adapter of the tile, in order of its first row
+    g = __builtin_amdgcn_readlane(gi, __builtin_ctz(left));
+    if (k == 0) break;
+    left &= ~(uint32_t)__ballot(gi == g);
+    g = -1;
+  }
+  if (g < 0) return;
   const int r0 = blockIdx.z * 16 * RT;
-  const int ksteps = (K + 31) / 32, kb = ksteps * wave / 4, ke = ksteps * (wave + 1) / 4;
-  const long m = min(m0 + i, M - 1);
-  const bf16_t* Ag = A + (long)g * R * K;
+  const int ksteps = (a.K + 31) / 32;
+  const long m = min(m0 + i, a.M - 1);
+  const bf16_t* Ag = a.A + (long)g * a.R * a.K;
   f32x4_t acc[RT];
 #pragma unroll
   for (int t = 0; t < RT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int ks = kb; ks < ke; ++ks) {
-    const int k = ks * 32 + q * 8;
-    const bool in = k < K;
-    bf16x8_t xf = zero8();
-    if constexpr (CODES) {
-      if (in) {
-        const uint2 c = *reinterpret_cast<const uint2*>(codes + m * (long)(ksteps * 32) + k);
-        const float st = act8::step(exps[m * (long)ksteps + ks]);
-        float v[8];
-        act8::values4(c.x, st, v);
-        act8::values4(c.y, st, v + 4);
-        xf = pack8(v);
+  for (int kb = wave * UN; kb < ksteps; kb += NW * UN) {
+    bf16x8_t xf[UN], af[UN][RT];
+    uint2 cd[UN];
+    uint32_t ex[UN];
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const int k = (kb + u) * 32 + q * 8;
+      const bool in = k < a.K;
+      const int kc = in ? k : 0;
+      if constexpr (CODES) {
+        cd[u] = *reinterpret_cast<const uint2*>(a.codes + m * (long)(ksteps * 32) + kc);
+        ex[u] = a.exps[m * (long)ksteps + (kc >> 5)];
+      } else {
+        xf[u] = load8(a.X + m * a.ldx + kc);
       }
-    } else {
-      if (in) xf = load8(X + m * ldx + k);
+#pragma unroll
+      for (int t = 0; t < RT; ++t) af[u][t] = load8(Ag + (long)min(r0 + t * 16 + i, a.R - 1) * a.K + kc);   // (rows past R are never stored)
     }
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const int r = r0 + t * 16 + i;
-      const bf16x8_t af = in && r < R ? load8(Ag + (long)r * K + k) : zero8();
-      acc[t] = mfma(af, xf, acc[t]);
+    for (int u = 0; u < UN; ++u) {
+      if constexpr (CODES) {
+        float v[8];
+        act8::values4(cd[u].x, act8::step(ex[u]), v);
+        act8::values4(cd[u].y, act8::step(ex[u]), v + 4);
+        xf[u] = pack8(v);
+      }
+      const bool in = (kb + u) * 32 + q * 8 < a.K;
+      xf[u] = keep(xf[u], in);
+#pragma unroll
+      for (int t = 0; t < RT; ++t) acc[t] = mfma(keep(af[u][t], in), xf[u], acc[t]);
     }
   }
   if (wave) {
@@ -108,77 +134,83 @@ __global__ __launch_bounds__(256) void down_kernel(const bf16_t* __restrict__ X,
   }
   __syncthreads();
   if (wave) return;
-  const float sc = scales[g];
-  const int rank = ranks[g];
-  const long mr = m0 + i;
+  const float sc = a.scales[g];
+  const int rank = a.ranks[g];
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     const int r = r0 + t * 16 + q * 4;
-    float4 o;
-    float* ov = &o.x;
+    float o[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float v = ((acc[t][e] + red[0][t][lane][e]) + red[1][t][lane][e]) + red[2][t][lane][e];
-      ov[e] = r + e < rank ? sc * v : 0.f;   // columns past the adapter's rank are 0 whatever x holds
+      float v = acc[t][e];
+#pragma unroll
+      for (int w = 0; w < NW - 1; ++w) v += red[w][t][lane][e];
+      o[e] = r + e < rank ? sc * v : 0.f;   // columns past the adapter's rank are 0 whatever x holds
     }
-    if (mr >= lo && mr < hi && r < R) *reinterpret_cast<float4*>(T + mr * R + r) = o;
+    if (gi == g && r < a.R) store_t4(a.T + m * a.P * a.R + r, a.R, a.P, o);
   }
 }
 
 struct LinArgs {
   const bf16_t *X, *W, *bias, *res, *B;
   bf16_t* Y;
-  const float* T;
+  const bf16_t* T;
   long ldx, ldw, ldr, ldy, M;
-  int N, K, R;
-  Segs sg;   // n = 0: no low-rank term
+  int N, K, R, P;
+  Rows rows;   // id null: no low-rank term
 };
 
 // ------------------------------------------------------------------------------------------- few rows: 16 x 16 NF tiles, split contraction
-// Eight wavefronts split the contraction of one tile (and the tile's (segment, rank step) pairs) and join in LDS: with few rows the launch is
-// bound by the latency of the weight loads, so the loads of a tile are spread over as many wavefronts as it can feed.
+// Eight wavefronts split the contraction of one tile (and the tile's (adapter, rank step) pairs) and join in LDS: with few rows the launch is
+// bound by the latency of the weight loads, so the loads of a tile are spread over as many wavefronts as it can feed and issued UN steps at a time.
 template <int NF>
 __global__ __launch_bounds__(512) void skinny_kernel(const LinArgs a) {
+  constexpr int UN = 4;
   __shared__ float red[8][NF][64][4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, q = lane >> 4;
   const long m0 = (long)blockIdx.y * 16;
   const int n0 = blockIdx.x * 16 * NF;
-  const int ksteps = (a.K + 31) / 32, kb = ksteps * wave / 8, ke = ksteps * (wave + 1) / 8;
+  const int ksteps = (a.K + 31) / 32;
   const long m = min(m0 + i, a.M - 1);
+  const int gi = a.rows.id && m0 + i < a.M ? id_of(a.rows, m0 + i) : -1;
   f32x4_t acc[NF];
 #pragma unroll
   for (int j = 0; j < NF; ++j) acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int ks = kb; ks < ke; ++ks) {
-    const int k = ks * 32 + q * 8;
-    const bool in = k < a.K;
-    const bf16x8_t xf = in ? load8(a.X + m * a.ldx + k) : zero8();
+  for (int kb = wave * UN; kb < ksteps; kb += 8 * UN) {
+    bf16x8_t xf[UN], wf[UN][NF];
 #pragma unroll
-    for (int j = 0; j < NF; ++j) {
-      const int n = n0 + j * 16 + i;
-      const bf16x8_t wf = in && n < a.N ? load8(a.W + (long)n * a.ldw + k) : zero8();
-      acc[j] = mfma(wf, xf, acc[j]);
+    for (int u = 0; u < UN; ++u) {
+      const int k = (kb + u) * 32 + q * 8;
+      const bool in = k < a.K;
+      const int kc = in ? k : 0;
+      xf[u] = load8(a.X + m * a.ldx + kc);
+#pragma unroll
+      for (int j = 0; j < NF; ++j) wf[u][j] = load8(a.W + (long)min(n0 + j * 16 + i, a.N - 1) * a.ldw + kc);   // (rows past N are never stored)
+    }
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const bool in = (kb + u) * 32 + q * 8 < a.K;
+      xf[u] = keep(xf[u], in);
+#pragma unroll
+      for (int j = 0; j < NF; ++j) acc[j] = mfma(keep(wf[u][j], in), xf[u], acc[j]);
     }
   }
-  if (a.sg.n) {
-    const int s0 = seg_of(a.sg, m0), rsteps = (a.R + 31) / 32;
-    int turn = 0;
-    for (int s = s0; s < a.sg.n && (long)a.sg.start[s] * a.sg.unit < m0 + 16; ++s) {
-      const int g = a.sg.id[s];
-      if (g < 0) continue;
-      const bool mine = m0 + i >= (long)a.sg.start[s] * a.sg.unit && m0 + i < (long)a.sg.start[s + 1] * a.sg.unit;
-      const bf16_t* Bg = a.B + (long)g * a.N * a.R;
-      for (int rs = 0; rs < rsteps; ++rs, ++turn) {
-        if ((turn & 7) != wave) continue;
-        const int r = rs * 32 + q * 8;
-        const bool in = r < a.R;
-        const bf16x8_t tf = t_frag(a.T + m * a.R + r, in && mine);
+  uint32_t left = (uint32_t)__ballot(gi >= 0) & 0xffffu;   // rows whose adapter is still to come
+  const int rsteps = (a.R + 31) / 32;
+  for (int turn = 0; left;) {
+    const int g = __builtin_amdgcn_readlane(gi, __builtin_ctz(left));
+    left &= ~(uint32_t)__ballot(gi == g);
+    const bf16_t* Bg = a.B + (long)g * a.N * a.R;
+    for (int rs = 0; rs < rsteps; ++rs, ++turn) {
+      if ((turn & 7) != wave) continue;
+      const int r = rs * 32 + q * 8;
+      const bool in = r < a.R;
+      const bf16x8_t tf = in && gi == g ? load8(a.T + m * a.P * a.R + r) : zero8();
 #pragma unroll
-        for (int j = 0; j < NF; ++j) {
-          const int n = n0 + j * 16 + i;
-          const bf16x8_t bf = in && n < a.N ? load8(Bg + (long)n * a.R + r) : zero8();
-          acc[j] = mfma(bf, tf, acc[j]);
-        }
+      for (int j = 0; j < NF; ++j) {
+        const int n = n0 + j * 16 + i;
+        const bf16x8_t bf = in && n < a.N ? load8(Bg + (long)n * a.R + r) : zero8();
+        acc[j] = mfma(bf, tf, acc[j]);
       }
     }
   }
@@ -216,20 +248,23 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, char* dst, uint
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)dst, 16, voff, soff, 0, 0);
 }
 
-// rows x 64 columns of one operand, global -> LDS; lane (row = tid >> 3, slot = tid & 7) fetches source chunk slot ^ ((row >> 1) & 7)
-template <int ROWS>
+// rows x 64 columns of one operand, global -> LDS, by NW wavefronts; lane (row = tid >> 3, slot = tid & 7) fetches source chunk slot ^ ((row >> 1) & 7)
+template <int ROWS, int NW>
 struct Stage {
-  static constexpr int NL = ROWS / 32;
+  static constexpr int RPI = 8 * NW, NL = ROWS / RPI;
+  static_assert(ROWS % RPI == 0 && RPI % 16 == 0, "whole copies");
   __amdgpu_buffer_rsrc_t rs;
   uint32_t voff[NL], soff;
   int krem, kc;
-  __device__ __forceinline__ void init(const bf16_t* base, long ld, int live, int K, int tid) {   // base: first row of the tile
+  // base: first row of the tile; live(r): whether row r of the tile is read (others are zeros)
+  template <class L>
+  __device__ __forceinline__ void begin(const bf16_t* base, long ld, int K, int tid, L live) {
     rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t*>(base), 0, 0x40000000, 0x00020000);
     kc = ((tid & 7) ^ ((tid >> 4) & 7)) * 8;
 #pragma unroll
     for (int l = 0; l < NL; ++l) {
-      const int r = (tid >> 3) + 32 * l;
-      voff[l] = r < live ? (uint32_t)r * (uint32_t)(ld * 2) + kc * 2 : OOB;
+      const int r = (tid >> 3) + RPI * l;
+      voff[l] = live(r) ? (uint32_t)r * (uint32_t)(ld * 2) + kc * 2 : OOB;
     }
     soff = 0;
     krem = K;
@@ -237,78 +272,23 @@ struct Stage {
   __device__ __forceinline__ void fetch(char* dst, int wave) {
     const bool bad = kc >= krem;
 #pragma unroll
-    for (int l = 0; l < NL; ++l) dma16(rs, dst + (32 * l + 8 * wave) * 128, bad ? OOB : voff[l], soff);
+    for (int l = 0; l < NL; ++l) dma16(rs, dst + (RPI * l + 8 * wave) * 128, bad ? OOB : voff[l], soff);
     soff += BK * 2;
     krem -= BK;
   }
 };
 
-// 256 threads, 2 x 2 wavefronts, BM x BN outputs; NSTG LDS stages with NSTG - 1 tiles of the contraction in flight.  The weight-side
-// fragment is MFMA operand A, so a lane ends with four consecutive columns of one row.  The low-rank term runs on fragments loaded straight
-// from memory, under the first tiles' DMA.
-template <int BM, int BN, int NSTG>
-__global__ __launch_bounds__(256) void tile_kernel(const LinArgs a) {
-  constexpr int WM = BM / 2, WN = BN / 2, FM = WM / 16, FN = WN / 16;
-  constexpr int STAGE = (BM + BN) * 128, PITCH = (BN + 4) * 4;
-  constexpr int LDS = NSTG * STAGE > BM * PITCH ? NSTG * STAGE : BM * PITCH;
-  constexpr int NLD = BM / 32 + BN / 32;
-  __shared__ __attribute__((aligned(16))) char lds[LDS];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = lane & 15, q = lane >> 4;
-  const int tiles_n = (a.N + BN - 1) / BN;
-  const long m0 = (long)(blockIdx.x / tiles_n) * BM;
-  const int n0 = (blockIdx.x % tiles_n) * BN;
-  const int wm0 = (wave >> 1) * WM, wn0 = (wave & 1) * WN;
-  Stage<BM> sx;
-  Stage<BN> sw;
-  sx.init(a.X + m0 * a.ldx, a.ldx, (int)min((long)BM, a.M - m0), a.K, tid);
-  sw.init(a.W + (long)n0 * a.ldw, a.ldw, min(BN, a.N - n0), a.K, tid);
-  f32x4_t acc[FM][FN];
-#pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  auto issue = [&](int st) {
-    sx.fetch(lds + st * STAGE, wave);
-    sw.fetch(lds + st * STAGE + BM * 128, wave);
-  };
-#pragma unroll
-  for (int u = 0; u < NSTG - 1; ++u) issue(u);
-
-  if (a.sg.n) {
-    const long w0 = m0 + wm0;   // this wavefront's rows
-    const int rsteps = (a.R + 31) / 32;
-    if (w0 < a.M)
-      for (int s = seg_of(a.sg, w0); s < a.sg.n && (long)a.sg.start[s] * a.sg.unit < w0 + WM; ++s) {
-        const int g = a.sg.id[s];
-        if (g < 0) continue;
-        const long lo = (long)a.sg.start[s] * a.sg.unit, hi = (long)a.sg.start[s + 1] * a.sg.unit;
-        const bf16_t* Bg = a.B + (long)g * a.N * a.R;
-        for (int rs = 0; rs < rsteps; ++rs) {
-          const int r = rs * 32 + q * 8;
-          const bool in = r < a.R;
-          bf16x8_t tf[FM], bf[FN];
-#pragma unroll
-          for (int i = 0; i < FM; ++i) {
-            const long m = w0 + i * 16 + i16;
-            tf[i] = t_frag(a.T + m * a.R + r, in && m >= lo && m < hi);
-          }
-#pragma unroll
-          for (int j = 0; j < FN; ++j) {
-            const int n = n0 + wn0 + j * 16 + i16;
-            bf[j] = in && n < a.N ? load8(Bg + (long)n * a.R + r) : zero8();
-          }
-#pragma unroll
-          for (int i = 0; i < FM; ++i)
-#pragma unroll
-            for (int j = 0; j < FN; ++j) acc[i][j] = mfma(bf[j], tf[i], acc[i][j]);
-        }
-      }
-  }
-
-  const int kt = (a.K + BK - 1) / BK;
+// acc += the product of NK stages of 64 columns: NSTG LDS stages, NSTG - 1 in flight, one barrier per stage.  The weight-side fragment is MFMA operand A,
+// so a lane ends with four consecutive columns (4 q + e) of one row (lane & 15).  issue(st) starts the next stage's copies (NLD per wavefront,
+// always: past the end they are out of range and fill zeros, so the count of copies still allowed in flight is a constant).
+template <int BM, int BN, int WGM, int WGN, int NSTG, class I>
+__device__ __forceinline__ void ring(char* lds, int nk, int tid, f32x4_t (&acc)[BM / WGM / 16][BN / WGN / 16], I issue) {
+  constexpr int NW = WGM * WGN, WM = BM / WGM, WN = BN / WGN, FM = WM / 16, FN = WN / 16;
+  constexpr int STAGE = (BM + BN) * 128, NLD = (BM + BN) / (8 * NW);
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = lane & 15, q = lane >> 4;
+  const int wm0 = (wave / WGN) * WM, wn0 = (wave % WGN) * WN;
   int rd = 0, wr = NSTG - 1;
-  for (int t = 0; t < kt; ++t) {
-    // every step issues NLD copies (past the end: out of range, zero fill), so the count of those still allowed in flight is a constant
+  for (int t = 0; t < nk; ++t) {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NSTG - 2) * NLD) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -319,9 +299,9 @@ __global__ __launch_bounds__(256) void tile_kernel(const LinArgs a) {
       bf16x8_t fa[FM], fb[FN];
       const int chunk = ks * 4 + q;
 #pragma unroll
-      for (int i = 0; i < FM; ++i) fa[i] = *reinterpret_cast<const bf16x8_t*>(pa + lds_off(wm0 + i * 16 + i16, chunk));
-#pragma unroll
       for (int j = 0; j < FN; ++j) fb[j] = *reinterpret_cast<const bf16x8_t*>(pb + lds_off(wn0 + j * 16 + i16, chunk));
+#pragma unroll
+      for (int i = 0; i < FM; ++i) fa[i] = *reinterpret_cast<const bf16x8_t*>(pa + lds_off(wm0 + i * 16 + i16, chunk));
 #pragma unroll
       for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -331,48 +311,162 @@ __global__ __launch_bounds__(256) void tile_kernel(const LinArgs a) {
     wr = wr + 1 == NSTG ? 0 : wr + 1;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the zero-filling copies still write LDS
-  __syncthreads();
-  // the fp32 tile through LDS: rows leave as 16-byte stores, bias and residual are added before the one rounding
+}
+
+// consecutive workgroups go to the eight XCDs in turn: XCD x takes the x-th eighth of the tiles, so that tiles that share operands share an L2
+__device__ __forceinline__ uint32_t xcd_tile(uint32_t b, uint32_t n) {
+  const uint32_t x = b & 7, i = b >> 3, q = n >> 3, r = n & 7;
+  return x * q + min(x, r) + i;
+}
+
+// the smallest adapter above `after` among the BM rows of a tile (ids in LDS), or -1; the same in every lane of every wavefront
+template <int BM>
+__device__ __forceinline__ int next_adapter(const int* ids, int after, int lane) {
+  uint32_t best = 0x7fffffffu;
+#pragma unroll
+  for (int k = 0; k < BM / 64; ++k) {
+    const int g = ids[k * 64 + lane];
+    best = min(best, g > after ? (uint32_t)g : 0x7fffffffu);
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) best = min(best, (uint32_t)__shfl_xor((int)best, d));
+  const int g = __builtin_amdgcn_readfirstlane((int)best);
+  return g == 0x7fffffff ? -1 : g;
+}
+
+// WGM x WGN wavefronts, BM x BN outputs.  The low-rank term of each adapter that the tile meets goes through the same ring, behind the projection's
+// own columns: R further columns of the contraction, the adapter's rows of T (others read as zeros) against its B.  (Fragments of T and B
+// straight from memory instead cost a load latency per 32 columns of rank: 28 against 18 us at 4096 x 640 x 640, rank 320.)
+template <int BM, int BN, int WGM, int WGN, int NSTG>
+__global__ __launch_bounds__(WGM * WGN * 64) void tile_kernel(const LinArgs a) {
+  constexpr int NW = WGM * WGN, WM = BM / WGM, WN = BN / WGN, FM = WM / 16, FN = WN / 16, STAGE = (BM + BN) * 128;
+  // ONE shared array: with a second one the compiler tells the two apart, takes the fragment reads for readers of the copies in flight, and waits
+  // for all of them (s_waitcnt vmcnt(0)) in every step
+  __shared__ __attribute__((aligned(16))) char lds[NSTG * STAGE + BM * 4];
+  int* ids = reinterpret_cast<int*>(lds + NSTG * STAGE);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = lane & 15, q = lane >> 4;
+  const uint32_t tiles_n = (a.N + BN - 1) / BN, tile = xcd_tile(blockIdx.x, gridDim.x);
+  const long m0 = (long)(tile / tiles_n) * BM;
+  const int n0 = (int)(tile % tiles_n) * BN;
+  const int mlive = (int)min((long)BM, a.M - m0), nlive = min(BN, a.N - n0);
+  f32x4_t acc[FM][FN];
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
-    for (int j = 0; j < FN; ++j)
-      *reinterpret_cast<f32x4_t*>(lds + (wm0 + i * 16 + i16) * PITCH + (wn0 + j * 16 + q * 4) * 4) = acc[i][j];
+    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  Stage<BM, NW> sx;
+  Stage<BN, NW> sw;
+  sx.begin(a.X + m0 * a.ldx, a.ldx, a.K, tid, [&](int r) { return r < mlive; });
+  sw.begin(a.W + (long)n0 * a.ldw, a.ldw, a.K, tid, [&](int r) { return r < nlive; });
+  int nk = (a.K + BK - 1) / BK, left = nk, g = -1;   // stages in all; stages left of the current part; its adapter
+  const int rk = (a.R + BK - 1) / BK;
+  auto issue = [&](int st) {
+    if (left == 0 && a.rows.id != nullptr) {   // (uniform)
+      g = next_adapter<BM>(ids, g, lane);
+      left = g < 0 ? 1 << 30 : rk;
+      if (g >= 0) {
+        sx.begin(a.T + m0 * a.P * a.R, (long)a.P * a.R, a.R, tid, [&](int r) { return ids[r] == g; });
+        sw.begin(a.B + ((long)g * a.N + n0) * a.R, a.R, a.R, tid, [&](int r) { return r < nlive; });
+      }
+    }
+    --left;
+    sx.fetch(lds + st * STAGE, wave);
+    sw.fetch(lds + st * STAGE + BM * 128, wave);
+  };
+  if (a.rows.id != nullptr) {
+    for (int r = tid; r < BM; r += NW * 64) ids[r] = r < mlive ? id_of(a.rows, m0 + r) : -1;
+    __syncthreads();
+  }
+#pragma unroll
+  for (int u = 0; u < NSTG - 1; ++u) issue(u);
+  if (a.rows.id != nullptr)
+    for (int h = next_adapter<BM>(ids, -1, lane); h >= 0; h = next_adapter<BM>(ids, h, lane)) nk += rk;
+  ring<BM, BN, WGM, WGN, NSTG>(lds, nk, tid, acc, issue);
+  // bias and residual are added to the fp32 sums before the one rounding
+  const long w0 = m0 + (wave / WGN) * WM;          // this wavefront's rows and columns
+  const int v0 = n0 + (wave % WGN) * WN;
+#pragma unroll
+  for (int j = 0; j < FN; ++j) {
+    const int n = v0 + j * 16 + q * 4;
+    if (n >= a.N) continue;
+    const uint2 b = a.bias ? *reinterpret_cast<const uint2*>(a.bias + n) : make_uint2(0u, 0u);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const long m = w0 + i * 16 + i16;
+      if (m >= a.M) continue;
+      const uint2 r = a.res ? *reinterpret_cast<const uint2*>(a.res + m * a.ldr + n) : make_uint2(0u, 0u);
+      const f32x4_t v = acc[i][j];
+      *reinterpret_cast<uint2*>(a.Y + m * a.ldy + n) = make_uint2(pack_bf16x2(v[0] + bf16lo(b.x) + bf16lo(r.x), v[1] + bf16hi(b.x) + bf16hi(r.x)),
+                                                                  pack_bf16x2(v[2] + bf16lo(b.y) + bf16lo(r.y), v[3] + bf16hi(b.y) + bf16hi(r.y)));
+    }
+  }
+}
+
+// T = s A x for many rows of long requests: 64 rows x BN adapter rows per workgroup, once for each adapter that the rows meet (mostly one)
+template <int BN, int NSTG>
+__global__ __launch_bounds__(256) void down_tile_kernel(const DownArgs a) {
+  constexpr int BM = 64, FM = 2, FN = BN / 32, STAGE = (BM + BN) * 128;
+  __shared__ __attribute__((aligned(16))) char lds[NSTG * STAGE + BM * 4];   // (one array: see tile_kernel)
+  int* ids = reinterpret_cast<int*>(lds + NSTG * STAGE);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = lane & 15, q = lane >> 4;
+  const uint32_t tiles_r = (a.R + BN - 1) / BN, tile = xcd_tile(blockIdx.x, gridDim.x);
+  const long m0 = (long)(tile / tiles_r) * BM;
+  const int r0 = (int)(tile % tiles_r) * BN;
+  const int mlive = (int)min((long)BM, a.M - m0), rlive = min(BN, a.R - r0);
+  if (tid < BM) ids[tid] = tid < mlive ? id_of(a.rows, m0 + tid) : -1;
   __syncthreads();
-  for (int id = tid; id < BM * (BN / 8); id += 256) {
-    const int row = id / (BN / 8), c = id % (BN / 8);
-    const long m = m0 + row;
-    const int n = n0 + c * 8;
-    if (m >= a.M || n >= a.N) continue;
-    const float4 u = *reinterpret_cast<const float4*>(lds + row * PITCH + c * 32), w = *reinterpret_cast<const float4*>(lds + row * PITCH + c * 32 + 16);
-    float v[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
-    auto add = [&](const bf16_t* p) {
-      const uint4 b = *reinterpret_cast<const uint4*>(p);
-      v[0] += bf16lo(b.x), v[1] += bf16hi(b.x), v[2] += bf16lo(b.y), v[3] += bf16hi(b.y);
-      v[4] += bf16lo(b.z), v[5] += bf16hi(b.z), v[6] += bf16lo(b.w), v[7] += bf16hi(b.w);
+  int turn = 0;   // where the rows meet several adapters, blockIdx.y = 0 and 1 take them in turn
+  for (int g = next_adapter<BM>(ids, -1, lane); g >= 0; g = next_adapter<BM>(ids, g, lane), ++turn) {
+    if ((turn & 1) != (int)blockIdx.y) continue;
+    f32x4_t acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    Stage<BM, 4> sx;
+    Stage<BN, 4> sa;
+    sx.begin(a.X + m0 * a.ldx, a.ldx, a.K, tid, [&](int r) { return r < mlive; });
+    sa.begin(a.A + ((long)g * a.R + r0) * a.K, a.K, a.K, tid, [&](int r) { return r < rlive; });
+    auto issue = [&](int st) {
+      sx.fetch(lds + st * STAGE, wave);
+      sa.fetch(lds + st * STAGE + BM * 128, wave);
     };
-    if (a.bias) add(a.bias + n);
-    if (a.res) add(a.res + m * a.ldr + n);
-    *reinterpret_cast<uint4*>(a.Y + m * a.ldy + n) =
-        make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+#pragma unroll
+    for (int u = 0; u < NSTG - 1; ++u) issue(u);
+    ring<BM, BN, 2, 2, NSTG>(lds, (a.K + BK - 1) / BK, tid, acc, issue);
+    const float sc = a.scales[g];
+    const int rank = a.ranks[g];
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const int mr = (wave >> 1) * 32 + i * 16 + i16;
+      const long m = m0 + mr;
+      const int gm = ids[mr];
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const int r = r0 + (wave & 1) * (BN / 2) + j * 16 + q * 4;
+        float o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = r + e < rank ? sc * acc[i][j][e] : 0.f;
+        if (gm == g && r < a.R) store_t4(a.T + m * a.P * a.R + r, a.R, a.P, o);
+      }
+    }
+    __syncthreads();   // the stages are free for the next adapter
   }
 }
 
 // ------------------------------------------------------------------------------------------------------------------ weight gradients
-// The rows of all adapters in sorted order (adapter by adapter, segment by segment) are one axis of `rows` positions, cut into chunks of `chunk`
-// positions.  A workgroup takes one chunk x 128 columns of V x RB columns of U; where adapters change inside its chunk it finishes one and
-// begins the next.  Piece (chunk b, j-th used adapter) is partial sum b + j: along the axis every new piece raises b or j.  A second launch adds
-// an adapter's partial sums in their order: no atomics, the same bits every time.
+// The rows of all adapters in sorted order (adapter by adapter) are one axis of `rows` positions, cut into chunks of `chunk` positions.  A workgroup
+// takes one chunk x 128 columns of V x RB columns of U; where adapters change inside its chunk it finishes one and begins the next.  Piece
+// (chunk b, j-th used adapter) is partial sum b + j: along the axis every new piece raises b or j.  A second launch adds an adapter's partial
+// sums in their order: no atomics, the same bits every time.
 struct Order {
-  const int* seg_start;   // [n] first row of the k-th segment in sorted order, in units
-  const int* seg_pos;     // [n + 1] its first position, in units
-  const int* used_pos;    // [nused + 1] first position of the j-th used adapter, in units
-  const int* used_id;     // [nused]
-  const int* slot;        // [nslot] j of adapter g, or -1
-  int n, nused, nslot, unit;
+  const int* perm;       // [rows / unit] the unit of rows at each position of the axis, in units
+  const int* used_pos;   // [nused + 1] first position of the j-th used adapter, in units
+  const int* slot;       // [nslot] j of adapter g, or -1
+  int nused, nslot, unit;
+  uint32_t magic, shift; // p / unit = (p magic) >> 32 >> shift for p < 2^31 (unit > 1)
   long rows;
 };
-
 typedef short v4s_t __attribute__((ext_vector_type(4)));
 template <int PB>
 __device__ __forceinline__ int tr_off(int row, int chunk) { return row * PB + ((chunk ^ ((row & 7) << 1)) << 4); }   // PB >= 256: the XOR moves a chunk by up to 14
@@ -387,16 +481,25 @@ __device__ __forceinline__ bf16x8_t tr_frag(const char* tile, int r32, int col0,
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+struct Grad {            // one gradient: dA (U = dT, V = X or its codes) or dB (U = T, V = dY)
+  const bf16_t *U, *V;
+  const uint8_t *codes, *exps;
+  long ldv;
+  int C, chunk, blocks;  // columns of V, positions per chunk, workgroups
+  float *part, *out;     // partial sums, result
+};
+
+// One workgroup's share of one gradient.  The next tile is on its way from memory (registers) while a tile is multiplied; the rest
+// of the latency is hidden by the other workgroups of the CU (three: the registers allow no more; with two tiles on their way one fits, 41 against 25 us).
 template <int RB, bool CODES, bool TRANS>   // TRANS: partial sums as [C][R] (dB), else [R][C] (dA)
-__global__ __launch_bounds__(256) void wgrad_kernel(const float* __restrict__ U, int R, const bf16_t* __restrict__ V, long ldv,
-                                                    const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exps, int C, Order o,
-                                                    int chunk, float* __restrict__ part) {
+__device__ __forceinline__ void wgrad_body(const Grad& G, int R, const Order& o, uint32_t id, char* vt, char* ut) {
   constexpr int TK = 64, CB = 128, PV = 256, PU = RB == 32 ? 256 : 512, FU = RB / 16;
-  __shared__ __attribute__((aligned(16))) char vt[TK * PV], ut[TK * PU];
-  __shared__ int rowof[TK];
+  constexpr int NV = TK * CB / 8 / 256, NU = TK * RB / 8 / 256;   // 16-byte chunks of V, and of each part of U, per thread
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int c0 = blockIdx.y * CB, r0 = blockIdx.z * RB;
-  const long p_begin = (long)blockIdx.x * chunk, p_end = min(p_begin + chunk, o.rows);
+  const int C = G.C, tc = (C + CB - 1) / CB, tr = (R + RB - 1) / RB;
+  const uint32_t ck = id / (tc * tr), rest = id - ck * (tc * tr);   // neighbours share rows
+  const int c0 = (int)(rest % tc) * CB, r0 = (int)(rest / tc) * RB;
+  const long p_begin = (long)ck * G.chunk, p_end = min(p_begin + G.chunk, o.rows);
   int j = 0;   // the used adapter that holds p_begin
   for (int hi = o.nused; hi - j > 1;) {
     const int mid = (j + hi) >> 1;
@@ -404,6 +507,44 @@ __global__ __launch_bounds__(256) void wgrad_kernel(const float* __restrict__ U,
     else hi = mid;
   }
   const int cp = (C + 31) / 32 * 32;
+  const int vrow = tid >> 4, vch = tid & 15, vc = c0 + vch * 8;
+  const int urow = tid / (RB / 8), uch = tid % (RB / 8), ur = r0 + uch * 8;
+  struct Tile {
+    uint4 v[NV], u[NU][3];
+    uint2 c[NV];
+    uint32_t e[NV];
+  } next;
+  int mv[NV], mu[NU], qv[NV], qu[NU];   // the tile to fetch next: unit of each row, and the row in it (nothing uses a load before the fetch)
+  auto unit_of = [&](long p, int& m, int& q) {
+    const uint32_t u = o.unit == 1 ? (uint32_t)p : __umulhi((uint32_t)p, o.magic) >> o.shift;
+    m = o.perm[u];
+    q = (int)((uint32_t)p - u * (uint32_t)o.unit);
+  };
+  auto rows_of = [&](long p, long end) {
+#pragma unroll
+    for (int l = 0; l < NV; ++l) unit_of(min(p + vrow + 16 * l, end - 1), mv[l], qv[l]);   // (dead rows: the piece's last)
+#pragma unroll
+    for (int l = 0; l < NU; ++l) unit_of(min(p + urow + (2048 / RB) * l, end - 1), mu[l], qu[l]);
+  };
+  const int vcl = vc < C ? vc : 0, url = ur < R ? ur : 0;   // (columns past the end: loaded from column 0, never stored)
+  auto fetch = [&](Tile& t) {
+#pragma unroll
+    for (int l = 0; l < NV; ++l) {
+      const uint32_t row = mv[l] * o.unit + qv[l];
+      if constexpr (CODES) {
+        t.c[l] = *reinterpret_cast<const uint2*>(G.codes + (uint64_t)row * (uint32_t)cp + vcl);
+        t.e[l] = G.exps[(uint64_t)row * (uint32_t)(cp >> 5) + (vcl >> 5)];
+      } else {
+        t.v[l] = *reinterpret_cast<const uint4*>(G.V + (uint64_t)row * (uint32_t)G.ldv + vcl);
+      }
+    }
+#pragma unroll
+    for (int l = 0; l < NU; ++l) {
+      const bf16_t* q = G.U + (uint64_t)(uint32_t)(mu[l] * o.unit + qu[l]) * (uint32_t)(3 * R) + url;
+#pragma unroll
+      for (int h = 0; h < 3; ++h) t.u[l][h] = *reinterpret_cast<const uint4*>(q + h * R);
+    }
+  };
   for (long p = p_begin; p < p_end; ++j) {
     const long piece_end = min(p_end, (long)o.used_pos[j + 1] * o.unit);
     f32x4_t acc[2][FU];   // 32 columns of V per wavefront
@@ -411,83 +552,50 @@ __global__ __launch_bounds__(256) void wgrad_kernel(const float* __restrict__ U,
     for (int v = 0; v < 2; ++v)
 #pragma unroll
       for (int u = 0; u < FU; ++u) acc[v][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    rows_of(p, piece_end);
+    fetch(next);
+    rows_of(p + TK, piece_end);
     for (; p < piece_end; p += TK) {
-      const int nrow = (int)min((long)TK, piece_end - p);
+      const Tile& t = next;
       __syncthreads();   // the last tile's fragments have been read
-      if (tid < TK) {
-        int row = -1;
-        if (tid < nrow) {
-          const long pos = p + tid;
-          int lo = 0, hi = o.n;
-          while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if ((long)o.seg_pos[mid] * o.unit <= pos) lo = mid;
-            else hi = mid;
-          }
-          row = (int)((long)o.seg_start[lo] * o.unit + (pos - (long)o.seg_pos[lo] * o.unit));
+#pragma unroll
+      for (int l = 0; l < NV; ++l) {
+        uint4 w;
+        if constexpr (CODES) {
+          float v[8];
+          act8::values4(t.c[l].x, act8::step(t.e[l]), v);
+          act8::values4(t.c[l].y, act8::step(t.e[l]), v + 4);
+          w = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+        } else {
+          w = t.v[l];
         }
-        rowof[tid] = row;
+        *reinterpret_cast<uint4*>(vt + tr_off<PV>(vrow + 16 * l, vch)) = keep(w, p + vrow + 16 * l < piece_end);
       }
+#pragma unroll
+      for (int l = 0; l < NU; ++l)
+#pragma unroll
+        for (int h = 0; h < 3; ++h)
+          *reinterpret_cast<uint4*>(ut + tr_off<PU>(urow + (2048 / RB) * l, h * (RB / 8) + uch)) = keep(t.u[l][h], p + urow + (2048 / RB) * l < piece_end);
       __syncthreads();
-#pragma unroll
-      for (int l = 0; l < TK * CB / 8 / 256; ++l) {
-        const int row = (tid >> 4) + 16 * l, ch = tid & 15, c = c0 + ch * 8;
-        const long m = rowof[row];
-        uint4 w = make_uint4(0u, 0u, 0u, 0u);
-        if (m >= 0 && c < C) {
-          if constexpr (CODES) {
-            const uint2 k = *reinterpret_cast<const uint2*>(codes + m * cp + c);
-            const float st = act8::step(exps[m * (cp >> 5) + (c >> 5)]);
-            float v[8];
-            act8::values4(k.x, st, v);
-            act8::values4(k.y, st, v + 4);
-            w = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-          } else {
-            w = *reinterpret_cast<const uint4*>(V + m * ldv + c);
-          }
-        }
-        *reinterpret_cast<uint4*>(vt + tr_off<PV>(row, ch)) = w;
-      }
-#pragma unroll
-      for (int l = 0; l < TK * RB / 8 / 256; ++l) {
-        const int id = tid + 256 * l, row = id / (RB / 8), ch = id % (RB / 8), r = r0 + ch * 8;
-        const long m = rowof[row];
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (m >= 0 && r < R) {
-          const float4 x = *reinterpret_cast<const float4*>(U + m * R + r), y = *reinterpret_cast<const float4*>(U + m * R + r + 4);
-          v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
-        }
-        // v = h + m + l, three bf16 parts that hold 24 bits (each difference is exact)
-#pragma unroll
-        for (int part3 = 0; part3 < 3; ++part3) {
-          const uint4 w = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-          *reinterpret_cast<uint4*>(ut + tr_off<PU>(row, part3 * (RB / 8) + ch)) = w;
-          const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            v[2 * e] -= bf16lo(ww[e]);
-            v[2 * e + 1] -= bf16hi(ww[e]);
-          }
-        }
-      }
-      __syncthreads();
+      fetch(next);   // the next tile's loads run under this tile's products (past the piece: its last row again)
+      rows_of(p + 2 * TK, piece_end);
 #pragma unroll
       for (int s = 0; s < TK / 32; ++s) {
         bf16x8_t fv[2];
 #pragma unroll
         for (int v = 0; v < 2; ++v) fv[v] = tr_frag<PV>(vt, s, wave * 32 + v * 16, lane);
 #pragma unroll
-        for (int part3 = 2; part3 >= 0; --part3)
+        for (int h = 2; h >= 0; --h)
 #pragma unroll
           for (int u = 0; u < FU; ++u) {
-            const bf16x8_t fu = tr_frag<PU>(ut, s, part3 * RB + u * 16, lane);
+            const bf16x8_t fu = tr_frag<PU>(ut, s, h * RB + u * 16, lane);
 #pragma unroll
             for (int v = 0; v < 2; ++v) acc[v][u] = TRANS ? mfma(fu, fv[v], acc[v][u]) : mfma(fv[v], fu, acc[v][u]);
           }
       }
     }
     p = piece_end;
-    float* out = part + (long)(blockIdx.x + j) * R * C;
+    float* out = G.part + (long)(ck + j) * R * C;
 #pragma unroll
     for (int v = 0; v < 2; ++v)
 #pragma unroll
@@ -502,80 +610,131 @@ __global__ __launch_bounds__(256) void wgrad_kernel(const float* __restrict__ U,
   }
 }
 
-// out[g] = sum of the partial sums of adapter g; zeros for an adapter without rows and past an adapter's rank
-template <bool TRANS>
-__global__ __launch_bounds__(256) void wgrad_reduce_kernel(const float* __restrict__ part, int R, int C, int r_out, const int* __restrict__ ranks, Order o,
-                                                           int chunk, float* __restrict__ out) {
-  const int g = blockIdx.y;
-  const long id = (long)blockIdx.x * 256 + threadIdx.x, n = (long)r_out * C;
-  if (id >= n) return;
-  const int r = (int)(TRANS ? id % r_out : id / C);
-  const long at = TRANS ? id / r_out * R + r : id;
-  const int j = g < o.nslot ? o.slot[g] : -1;
-  float s = 0.f;
-  if (j >= 0 && r < ranks[g]) {
-    const long first = (long)o.used_pos[j] * o.unit, last = (long)o.used_pos[j + 1] * o.unit - 1;
-    const long b1 = last / chunk + j;
-    for (long b = first / chunk + j; b <= b1; ++b) s += part[b * R * C + at];
-  }
-  out[g * n + id] = s;
+// dA and dB in one launch: the first da.blocks workgroups work on dA, the others on dB
+template <int RB, bool CODES>
+__global__ __launch_bounds__(256, 3) void wgrad_kernel(const Grad da, const Grad db, int R, const Order o) {
+  __shared__ __attribute__((aligned(16))) char vt[64 * 256], ut[64 * (RB == 32 ? 256 : 512)];
+  const uint32_t id = xcd_tile(blockIdx.x, gridDim.x);
+  if (id < (uint32_t)da.blocks) wgrad_body<RB, CODES, false>(da, R, o, id, vt, ut);
+  else wgrad_body<RB, false, true>(db, R, o, id - da.blocks, vt, ut);
 }
 
+// out[g] = sum of the partial sums of adapter g; zeros for an adapter without rows and past an adapter's rank.  VEC outputs per thread
+template <bool TRANS, int VEC>
+__device__ __forceinline__ void wgrad_sum(const Grad& G, int R, int r_out, const int* ranks, const Order& o, uint32_t block) {
+  typedef float vec_t __attribute__((ext_vector_type(VEC)));
+  const int g = blockIdx.y, C = G.C;
+  const uint32_t id = (block * 256u + threadIdx.x) * VEC, n = (uint32_t)r_out * (uint32_t)C;
+  if (id >= n) return;
+  const int w = TRANS ? r_out : C;                       // VEC divides a row of the output
+  const uint32_t row = id / w, col = id - row * w;
+  const int r = (int)(TRANS ? col : row);
+  const uint32_t at = TRANS ? row * R + col : id;
+  const int j = g < o.nslot ? o.slot[g] : -1;
+  vec_t s = 0.f;
+  if (j >= 0) {
+    const long first = (long)o.used_pos[j] * o.unit, last = (long)o.used_pos[j + 1] * o.unit - 1;
+    const float* q = G.part + (first / G.chunk + j) * R * C + at;
+    const int nb = (int)(last / G.chunk - first / G.chunk) + 1;
+#pragma unroll 8
+    for (int b = 0; b < nb; ++b) s += *reinterpret_cast<const vec_t*>(q + (long)b * R * C);
+    const int rank = ranks[g];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      if (r + (TRANS ? e : 0) >= rank) s[e] = 0.f;
+  }
+  *reinterpret_cast<vec_t*>(G.out + (long)g * n + id) = s;
+}
+
+template <int VEC>   // of dB; dA's rows are a multiple of 8 long
+__global__ __launch_bounds__(256) void wgrad_reduce_kernel(const Grad da, const Grad db, int R, int r_out, const int* __restrict__ ranks, const Order o, int blocks_a) {
+  if ((int)blockIdx.x < blocks_a) wgrad_sum<false, 4>(da, R, r_out, ranks, o, blockIdx.x);
+  else wgrad_sum<true, VEC>(db, R, r_out, ranks, o, blockIdx.x - blocks_a);
+}
+
+// positions per chunk: whole tiles of 64
 int wgrad_chunk(long rows, int C, int R) {
   const long tiles = (long)((C + 127) / 128) * (R <= 32 ? 1 : (R + 63) / 64);
-  long want = 1024 / tiles;   // workgroups: four per CU
+  long want = 288 / tiles;   // workgroups of one gradient; dA and dB run together, three workgroups fit on a CU
   if (want < 1) want = 1;
   long ch = (rows + want - 1) / want;
   ch = (ch + 63) / 64 * 64;
   return (int)(ch < 64 ? 64 : ch > (1 << 20) ? (1 << 20) : ch);
 }
 
-void launch_down(const bf16_t* X, long ldx, const uint8_t* codes, const uint8_t* exps, long M, int K, const bf16_t* A, const int* ranks, const float* scales, int R,
-                 const Segs& sg, int slots, float* T, hipStream_t st) {
-  const int t16 = (R + 15) / 16, rt = t16 == 1 ? 1 : 2;
-  const dim3 grid((unsigned)((M + 15) / 16), slots, (t16 + rt - 1) / rt);
-#define AQL_DOWN(RT, CODES) hipLaunchKernelGGL((down_kernel<RT, CODES>), grid, dim3(256), 0, st, X, ldx, codes, exps, M, K, A, ranks, scales, R, sg, T)
-  if (codes) {
-    if (rt == 1) AQL_DOWN(1, true);
-    else AQL_DOWN(2, true);
-  } else {
-    if (rt == 1) AQL_DOWN(1, false);
-    else AQL_DOWN(2, false);
+// partial sums of one gradient, in floats
+double wgrad_floats(long rows, int nused, int C, int R) {
+  if (rows <= 0 || nused <= 0 || C <= 0 || R <= 0) return 0;
+  const int ch = wgrad_chunk(rows, C, R);
+  return (double)((rows + ch - 1) / ch + nused - 1) * R * C;
+}
+
+// T by 64-row tiles where a tile rarely meets a second adapter (each costs another pass over its rows) and the tiles fill the chip, by 16-row tiles
+// otherwise.  Measured (us, 64-row / 16-row tiles): 32768 x 320, rank 32: 5.3 / 9.8; 9001 x 1280, rank 64: 10.0 / 19.9; 4096 x 640, rank 320:
+// 7.6 / 17.6; 4096 x 1280, rank 32 (64 tiles): 6.9 / 6.0; 1001 x 768, rank 64 (16 tiles): 6.7 / 6.3; 1000 x 2560, rank 32 (16 tiles): 10.7 / 9.0.
+void launch_down(const DownArgs& a, int runs, int slots, hipStream_t st) {
+  const long tiles = (a.M + 63) / 64 * (a.R <= 32 ? 1 : (a.R + 63) / 64);
+  if (!a.codes && a.M / runs >= 64 && tiles >= 96) {
+    if (a.R <= 32) hipLaunchKernelGGL((down_tile_kernel<32, 4>), dim3((unsigned)tiles, 2), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((down_tile_kernel<64, 4>), dim3((unsigned)tiles, 2), dim3(256), 0, st, a);
+    return;
   }
+  const int t16 = (a.R + 15) / 16;
+  // few workgroups: fewer adapter rows each, so that more CUs share the loads (8 x 1280, rank 32: 3.8 us with 16 rows, 5.0 with 32; 64 x 1280, rank 64:
+  // 4.3 / 5.5 / 8.0 with 16 / 32 / 64); many: more, so that X is read less often (9001 x 1280 codes, rank 64: 30 / 23 / 20)
+  const long b16 = (a.M + 15) / 16 * t16;
+  const int rt = t16 == 1 || b16 <= 256 ? 1 : t16 == 2 || b16 <= 512 ? 2 : 4;
+  const dim3 grid((unsigned)((a.M + 15) / 16), slots, (t16 + rt - 1) / rt);
+#define AQL_DOWN(RT)                                                                          \
+  do {                                                                                        \
+    if (a.codes) hipLaunchKernelGGL((down_kernel<RT, 4, true>), grid, dim3(256), 0, st, a);   \
+    else hipLaunchKernelGGL((down_kernel<RT, 4, false>), grid, dim3(256), 0, st, a);          \
+  } while (0)
+  if (rt == 1) AQL_DOWN(1);
+  else if (rt == 2) AQL_DOWN(2);
+  else AQL_DOWN(4);
 #undef AQL_DOWN
 }
 
-bool seg_ok(const void* start, const void* id, int n, int unit) { return n >= 0 && (n == 0 || (start && id && unit >= 1)); }
+bool rows_ok(const void* id, int runs, int unit) { return runs >= 0 && (runs == 0 || (id && unit >= 1)); }
 
 }  // namespace
 
-// Y = X W^T + bias + residual + the low-rank term; T: [M][R] fp32, written for the rows that have an adapter.  slots: the most segments that meet in one tile
-// of 16 rows (16-aligned tiles of rows).
+// Y = X W^T + bias + residual + the low-rank term; T: [M][parts][R] bf16, written for the rows that have an adapter.  slots: at least the number of adapters that
+// any 16 rows [16 i, 16 i + 16) meet; runs: stretches of neighbouring rows with one adapter (how long they are decides between the forms of the first launch).
 extern "C" int aql_adapter_linear(const bf16_t* X, long ldx, const bf16_t* W, long ldw, const bf16_t* bias, const bf16_t* residual, long ldr, bf16_t* Y,
                                   long ldy, long M, int N, int K, const bf16_t* A, const bf16_t* B, const int* ranks, const float* scales, int R,
-                                  const int* seg_start, const int* seg_id, int nseg, int unit, int slots, float* T, hipStream_t stream) {
+                                  const int* unit_id, int unit, int runs, int slots, bf16_t* T, int parts, hipStream_t stream) {
   AQL_CHECK_ARG(M >= 0 && M < (1L << 31) - 256 && N > 0 && K > 0 && N % 8 == 0 && K % 8 == 0, "aql_adapter_linear: bad shape M=%ld N=%d K=%d (N, K: multiples of 8)", M, N, K);
   if (M == 0) return AQL_OK;
   AQL_CHECK_ARG(X && W && Y, "aql_adapter_linear: null operand");
   AQL_CHECK_ARG(ldx >= K && ldw >= K && ldy >= N && (!residual || ldr >= N) && ldx % 8 == 0 && ldw % 8 == 0 && ldy % 8 == 0 && ldr % 8 == 0 && ldx < (1L << 21) &&
                     ldw < (1L << 21), "aql_adapter_linear: leading dimensions (multiples of 8, at least the width, below 2^21)");
   AQL_CHECK_ARG((((uintptr_t)X | (uintptr_t)W | (uintptr_t)bias | (uintptr_t)residual | (uintptr_t)Y) & 15) == 0, "aql_adapter_linear: operands must be 16-byte aligned");
-  AQL_CHECK_ARG(seg_ok(seg_start, seg_id, nseg, unit) && (nseg == 0 || (A && B && ranks && scales && T && R > 0 && R % 8 == 0 && slots >= 1 && slots <= 16)),
-                "aql_adapter_linear: bad adapters (R=%d: a multiple of 8) or segments", R);
-  const Segs sg{seg_start, seg_id, nseg, unit};
-  if (nseg) {
-    launch_down(X, ldx, nullptr, nullptr, M, K, A, ranks, scales, R, sg, slots, T, stream);
+  AQL_CHECK_ARG(rows_ok(unit_id, runs, unit) && (runs == 0 || (A && B && ranks && scales && T && R > 0 && R % 8 == 0 && slots >= 1 && slots <= 16 && (parts == 1 || parts == 3))),
+                "aql_adapter_linear: bad adapters (R=%d: a multiple of 8) or rows", R);
+  const Rows rows{runs ? unit_id : nullptr, unit};
+  if (runs) {
+    launch_down(DownArgs{X, nullptr, nullptr, A, ranks, scales, T, ldx, M, K, R, parts, rows}, runs, slots, stream);
     AQL_CHECK_LAUNCH("aql_adapter_linear (down)");
   }
-  const LinArgs a{X, W, bias, residual, B, Y, T, ldx, ldw, ldr, ldy, M, N, K, R, sg};
+  const LinArgs a{X, W, bias, residual, B, Y, T, ldx, ldw, ldr, ldy, M, N, K, R, parts, rows};
   if (M <= 256) {
     hipLaunchKernelGGL((skinny_kernel<1>), dim3((N + 15) / 16, (unsigned)((M + 15) / 16)), dim3(512), 0, stream, a);
   } else {
-    const long big = ((M + 127) / 128) * ((N + 127) / 128);
-    if (big >= 256)
-      hipLaunchKernelGGL((tile_kernel<128, 128, 2>), dim3((unsigned)big), dim3(256), 0, stream, a);
-    else
-      hipLaunchKernelGGL((tile_kernel<64, 64, 3>), dim3((unsigned)(((M + 63) / 64) * ((N + 63) / 64))), dim3(256), 0, stream, a);
+#define AQL_TILE(BM, BN, WGM, WGN, NSTG) \
+  hipLaunchKernelGGL((tile_kernel<BM, BN, WGM, WGN, NSTG>), dim3((unsigned)(((M + BM - 1) / BM) * ((N + BN - 1) / BN))), dim3(WGM * WGN * 64), 0, stream, a)
+    // Which tile (all measured at every one of these sizes; us, best first): 256 x 320 where the width allows it and every CU gets one (4096 x 10240 x 1280:
+    // 115.8 / 154 with 128 x 160); else 128 rows by 160 or 128 columns, whichever needs less time for its rounds of two tiles per CU
+    // (32768 x 320 x 320: 15.1 / 19.4; 9001 x 1280 x 1280: 41.6 with 128, 45.9 with 160); smaller ones where those leave CUs idle (2048 x 1280 x
+    // 1280: 14.9 with 64 x 128, 18.2 with 128 x 128; 1001 x 640 x 768: 6.3 with 64 x 64, 8.4 with 64 x 128)
+    const auto tiles = [&](long bm, long bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
+    if (N % 320 == 0 && tiles(256, 320) >= 256) AQL_TILE(256, 320, 2, 4, 2);
+    else if (tiles(128, 128) >= 256 && (tiles(128, 160) + 511) / 512 * 160 <= (tiles(128, 128) + 511) / 512 * 128) AQL_TILE(128, 160, 2, 2, 2);
+    else if (tiles(128, 128) >= 256) AQL_TILE(128, 128, 2, 2, 2);
+    else if (tiles(64, 128) >= 256) AQL_TILE(64, 128, 2, 2, 3);
+    else AQL_TILE(64, 64, 2, 2, 3);
+#undef AQL_TILE
   }
   AQL_CHECK_LAUNCH("aql_adapter_linear");
   return AQL_OK;
@@ -583,59 +742,70 @@ extern "C" int aql_adapter_linear(const bf16_t* X, long ldx, const bf16_t* W, lo
 
 // T = s A x alone, from X or from its 8-bit codes
 extern "C" int aql_adapter_down(const bf16_t* X, long ldx, const uint8_t* codes, const uint8_t* exps, long M, int K, const bf16_t* A, const int* ranks,
-                                const float* scales, int R, const int* seg_start, const int* seg_id, int nseg, int unit, int slots, float* T,
+                                const float* scales, int R, const int* unit_id, int unit, int runs, int slots, bf16_t* T, int parts,
                                 hipStream_t stream) {
   AQL_CHECK_ARG(M >= 0 && M < (1L << 31) - 256 && K > 0 && K % 8 == 0 && R > 0 && R % 8 == 0, "aql_adapter_down: bad shape M=%ld K=%d R=%d", M, K, R);
-  AQL_CHECK_ARG(seg_ok(seg_start, seg_id, nseg, unit), "aql_adapter_down: bad segments");
-  if (M == 0 || nseg == 0) return AQL_OK;
-  AQL_CHECK_ARG(!codes == !exps && !X != !codes && (!X || (ldx >= K && ldx % 8 == 0 && ((uintptr_t)X & 15) == 0)) && A && ranks && scales && T && slots >= 1 && slots <= 16,
+  AQL_CHECK_ARG(rows_ok(unit_id, runs, unit), "aql_adapter_down: bad rows");
+  if (M == 0 || runs == 0) return AQL_OK;
+  AQL_CHECK_ARG(!codes == !exps && !X != !codes && (!X || (ldx >= K && ldx % 8 == 0 && ((uintptr_t)X & 15) == 0)) && A && ranks && scales && T && slots >= 1 && slots <= 16 && (parts == 1 || parts == 3),
                 "aql_adapter_down: bad operands (exactly one of X and its codes)");
-  launch_down(X, ldx, codes, exps, M, K, A, ranks, scales, R, Segs{seg_start, seg_id, nseg, unit}, slots, T, stream);
+  launch_down(DownArgs{X, codes, exps, A, ranks, scales, T, ldx, M, K, R, parts, Rows{unit_id, unit}}, runs, slots, stream);
   AQL_CHECK_LAUNCH("aql_adapter_down");
   return AQL_OK;
 }
 
-// fp32 elements of the workspace of aql_adapter_wgrad (rows: those that have an adapter; nused: adapters that have rows), or -1: more than 2^31 - 1
-extern "C" int aql_adapter_wgrad_scratch_floats(long rows, int nused, int C, int R) {
-  if (rows <= 0 || nused <= 0 || C <= 0 || R <= 0) return 0;
-  const int ch = wgrad_chunk(rows, C, R);
-  const double n = (double)((rows + ch - 1) / ch + nused - 1) * R * C;
+// fp32 elements of the workspace of aql_adapter_wgrad (rows: those that have an adapter; nused: adapters that have rows; K, N: 0 for a gradient that is
+// not asked for), or -1: more than 2^31 - 1
+extern "C" int aql_adapter_wgrad_scratch_floats(long rows, int nused, int K, int N, int R) {
+  const double n = wgrad_floats(rows, nused, K, R) + wgrad_floats(rows, nused, N, R);
   return n < 2147483647.0 ? (int)n : -1;
 }
 
-extern "C" int aql_adapter_wgrad(const float* U, int R, const bf16_t* V, long ldv, const uint8_t* codes, const uint8_t* exps, long M, int C, int G, int r_out,
-                                 const int* ranks, const int* seg_start, const int* seg_pos, const int* used_pos, const int* used_id, const int* slot, int nseg,
-                                 int nused, int nslot, int unit, long rows, int trans, float* out, float* scratch, long scratch_floats, hipStream_t stream) {
-  AQL_CHECK_ARG(M >= 0 && M < (1L << 31) - 256 && C > 0 && C % 8 == 0 && R > 0 && R % 8 == 0 && G > 0 && G <= 65535 && r_out > 0 && r_out <= R && rows >= 0 && rows <= M,
-                "aql_adapter_wgrad: bad shape M=%ld C=%d R=%d G=%d", M, C, R, G);
-  AQL_CHECK_ARG(out && ranks && !codes == !exps && !V != !codes && (V == nullptr || (ldv >= C && ldv % 8 == 0 && ((uintptr_t)V & 15) == 0)), "aql_adapter_wgrad: bad operands");
-  AQL_CHECK_ARG(rows == 0 || (U && seg_start && seg_pos && used_pos && used_id && slot && nseg > 0 && nused > 0 && nslot > 0 && unit >= 1), "aql_adapter_wgrad: bad segments");
-  const int need = aql_adapter_wgrad_scratch_floats(rows, nused, C, R);
+extern "C" int aql_adapter_wgrad(const bf16_t* dT, const bf16_t* X, long ldx, const uint8_t* codes, const uint8_t* exps, int K, float* dA, const bf16_t* T,
+                                 const bf16_t* dY, long lddy, int N, float* dB, long M, int G, int R, int r_out, const int* ranks, const int* perm,
+                                 const int* used_pos, const int* slot, int nused, int nslot, int unit, long rows, float* scratch, long scratch_floats,
+                                 hipStream_t stream) {
+  AQL_CHECK_ARG(M >= 0 && M < (1L << 31) - 256 && R > 0 && R % 8 == 0 && G > 0 && G <= 65535 && r_out > 0 && r_out <= R && rows >= 0 && rows <= M,
+                "aql_adapter_wgrad: bad shape M=%ld R=%d G=%d", M, R, G);
+  AQL_CHECK_ARG((dA || dB) && ranks, "aql_adapter_wgrad: null operand");
+  AQL_CHECK_ARG(!dA || (K > 0 && K % 8 == 0 && (long)R * K < (1L << 31) && !codes == !exps && !X != !codes && (!X || (ldx >= K && ldx % 8 == 0 && ldx < (1L << 31) && ((uintptr_t)X & 15) == 0))),
+                "aql_adapter_wgrad: bad operands of dA (exactly one of X and its codes)");
+  AQL_CHECK_ARG(!dB || (N > 0 && N % 8 == 0 && (long)R * N < (1L << 31) && dY && lddy >= N && lddy % 8 == 0 && lddy < (1L << 31) && ((uintptr_t)dY & 15) == 0), "aql_adapter_wgrad: bad operands of dB");
+  AQL_CHECK_ARG(rows == 0 || ((!dA || dT) && (!dB || T) && perm && used_pos && slot && nused > 0 && nslot > 0 && unit >= 1 && rows % unit == 0), "aql_adapter_wgrad: bad rows");
+  if (!dA) K = 0;
+  if (!dB) N = 0;
+  const int need = aql_adapter_wgrad_scratch_floats(rows, nused, K, N, R);
   AQL_CHECK_ARG(need >= 0 && scratch_floats >= need && (need == 0 || scratch), "aql_adapter_wgrad: workspace of %ld floats, %d needed", scratch_floats, need);
-  Order o{seg_start, seg_pos, used_pos, used_id, slot, nseg, nused, rows ? nslot : 0, unit, rows};
-  const int ch = rows ? wgrad_chunk(rows, C, R) : 64;
-  if (rows) {
-    const dim3 grid((unsigned)((rows + ch - 1) / ch), (C + 127) / 128, R <= 32 ? 1 : (R + 63) / 64);
-#define AQL_WG(RB, CODES, TRANS) hipLaunchKernelGGL((wgrad_kernel<RB, CODES, TRANS>), grid, dim3(256), 0, stream, U, R, V, ldv, codes, exps, C, o, ch, scratch)
-    if (R <= 32) {
-      if (codes && trans) AQL_WG(32, true, true);
-      else if (codes) AQL_WG(32, true, false);
-      else if (trans) AQL_WG(32, false, true);
-      else AQL_WG(32, false, false);
-    } else {
-      if (codes && trans) AQL_WG(64, true, true);
-      else if (codes) AQL_WG(64, true, false);
-      else if (trans) AQL_WG(64, false, true);
-      else AQL_WG(64, false, false);
+  uint32_t L = 1;
+  while (rows && (1L << L) < unit) ++L;
+  const Order o{perm, used_pos, slot, nused, rows ? nslot : 0, unit, rows && unit > 1 ? (uint32_t)((1UL << (31 + L)) / (uint32_t)unit + 1) : 0u, L - 1, rows};
+  const int rb = R <= 32 ? 32 : 64, tr = (R + rb - 1) / rb;
+  const auto job = [&](const bf16_t* U, const bf16_t* V, long ldv, int C, float* part, float* out) {
+    Grad g{U, V, nullptr, nullptr, ldv, C, 64, 0, part, out};
+    if (C && rows) {
+      g.chunk = wgrad_chunk(rows, C, R);
+      g.blocks = (int)((rows + g.chunk - 1) / g.chunk) * ((C + 127) / 128) * tr;
     }
-#undef AQL_WG
+    return g;
+  };
+  Grad a = job(dT, X, ldx, K, scratch, dA);
+  a.codes = codes, a.exps = exps;
+  const Grad b = job(T, dY, lddy, N, scratch + (long)wgrad_floats(rows, nused, K, R), dB);
+  if (rows) {
+    const dim3 grid(a.blocks + b.blocks);
+    if (R <= 32) {
+      if (codes) hipLaunchKernelGGL((wgrad_kernel<32, true>), grid, dim3(256), 0, stream, a, b, R, o);
+      else hipLaunchKernelGGL((wgrad_kernel<32, false>), grid, dim3(256), 0, stream, a, b, R, o);
+    } else {
+      if (codes) hipLaunchKernelGGL((wgrad_kernel<64, true>), grid, dim3(256), 0, stream, a, b, R, o);
+      else hipLaunchKernelGGL((wgrad_kernel<64, false>), grid, dim3(256), 0, stream, a, b, R, o);
+    }
     AQL_CHECK_LAUNCH("aql_adapter_wgrad");
   }
-  const dim3 rgrid((unsigned)(((long)r_out * C + 255) / 256), G);
-  if (trans)
-    hipLaunchKernelGGL(wgrad_reduce_kernel<true>, rgrid, dim3(256), 0, stream, scratch, R, C, r_out, ranks, o, ch, out);
-  else
-    hipLaunchKernelGGL(wgrad_reduce_kernel<false>, rgrid, dim3(256), 0, stream, scratch, R, C, r_out, ranks, o, ch, out);
+  const bool vec = r_out % 4 == 0;
+  const int ba = (int)(((long)r_out * K / 4 + 255) / 256), bb = (int)(((long)r_out * N / (vec ? 4 : 1) + 255) / 256);
+  if (vec) hipLaunchKernelGGL(wgrad_reduce_kernel<4>, dim3(ba + bb, G), dim3(256), 0, stream, a, b, R, r_out, ranks, o, ba);
+  else hipLaunchKernelGGL(wgrad_reduce_kernel<1>, dim3(ba + bb, G), dim3(256), 0, stream, a, b, R, r_out, ranks, o, ba);
   AQL_CHECK_LAUNCH("aql_adapter_wgrad (sum)");
   return AQL_OK;
 }

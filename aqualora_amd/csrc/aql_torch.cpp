@@ -214,9 +214,9 @@ struct Plan {   // the device side of adapters.RequestPlan
   Tensor table;
   std::vector<long> start;   // host copy, in units
   long units = 0, requests = 0, live_units = 0;
-  int nseg = 0, nsorted = 0, nused = 0, nslot = 0, max_id = -1;
+  int nseg = 0, nused = 0, nslot = 0, max_id = -1;
   bool equal = false;
-  std::vector<long> at;      // offsets of start, id, seg_start, seg_pos, used_pos, used_id, slot in the table
+  std::vector<long> at;      // offsets of unit_id, perm, used_pos, slot in the table
   std::unordered_map<long, int> slots_by_unit;
 
   const int* part(int k) const { return (const int*)table.data_ptr() + at[k]; }
@@ -232,7 +232,7 @@ struct Plan {   // the device side of adapters.RequestPlan
     if (rows % requests) bad_value("RequestPlan: " + std::to_string(rows) + " rows do not divide among " + std::to_string(requests) + " equal requests");
     return std::max(1L, rows / requests);
   }
-  int slots(long unit) {   // the most segments that meet in 16 rows [16 i, 16 i + 16)
+  int slots(long unit) {   // the most segments, and so adapters, that meet in 16 rows [16 i, 16 i + 16)
     auto it = slots_by_unit.find(unit);
     if (it != slots_by_unit.end()) return it->second;
     int most = 0, count = 0;
@@ -256,40 +256,42 @@ struct Call : torch::CustomClassHolder {   // what a backward pass of adapter_li
   bool train = false, residual = false;
 };
 
-// one pass of aql_adapter_linear -> (y [M, N], T [M, R] or undefined)
+// one pass of aql_adapter_linear -> (y [M, N], T [M, parts, R] or undefined)
 std::pair<Tensor, Tensor> product(const Rows& x, const Tensor& w, const Tensor& bias, const Rows& res, const Tensor& a, const Tensor& b, const Bank& bank,
-                                  Plan& plan, long unit, long N, long K) {
+                                  Plan& plan, long unit, long N, long K, int parts) {
   const long M = x.t.size(0);
   Tensor y = at::empty({M, N}, x.t.options().requires_grad(false)), T;
-  if (plan.nseg) T = at::empty({M, bank.R}, x.t.options().dtype(at::kFloat).requires_grad(false));
+  if (plan.nseg) T = at::empty({M, parts, bank.R}, y.options());
   const auto st = stream_of(y);
   ran(aql_adapter_linear(ptr<bf16_t>(x.t), x.ld, ptr<bf16_t>(w), K, ptr<bf16_t>(bias), ptr<bf16_t>(res.t), res.ld, ptr<bf16_t>(y), N, M, (int)N, (int)K,
-                         ptr<bf16_t>(a), ptr<bf16_t>(b), ptr<int>(bank.ranks), ptr<float>(bank.scales), (int)bank.R, plan.part(0), plan.part(1), plan.nseg,
-                         (int)unit, plan.slots(unit), ptr<float>(T), st), "aql_adapter_linear", st);
+                         ptr<bf16_t>(a), ptr<bf16_t>(b), ptr<int>(bank.ranks), ptr<float>(bank.scales), (int)bank.R, plan.part(0), (int)unit, plan.nseg,
+                         plan.slots(unit), ptr<bf16_t>(T), parts, st), "aql_adapter_linear", st);
   return {y, T};
 }
 
 Tensor down(const Rows& x, const Tensor& codes, const Tensor& exps, long M, long K, const Tensor& a, const Bank& bank, Plan& plan, long unit) {
-  Tensor T = at::empty({M, bank.R}, a.options().dtype(at::kFloat));
+  Tensor T = at::empty({M, 3, bank.R}, a.options());
   const auto st = stream_of(T);
   ran(aql_adapter_down(ptr<bf16_t>(x.t), x.ld, ptr<uint8_t>(codes), ptr<uint8_t>(exps), M, (int)K, ptr<bf16_t>(a), ptr<int>(bank.ranks), ptr<float>(bank.scales),
-                       (int)bank.R, plan.part(0), plan.part(1), plan.nseg, (int)unit, plan.slots(unit), ptr<float>(T), st), "aql_adapter_down", st);
+                       (int)bank.R, plan.part(0), (int)unit, plan.nseg, plan.slots(unit), ptr<bf16_t>(T), 3, st), "aql_adapter_down", st);
   return T;
 }
 
-// fp32 gradient of a stack: [G, r, C], or [G, C, r] with `trans`
-Tensor wgrad(const Tensor& u, const Rows& v, const Tensor& codes, const Tensor& exps, long M, long C, bool trans, const Bank& bank, const Plan& plan, long unit) {
+// fp32 gradients of the stacks: dA [G, r, K] where want_a, dB [G, N, r] where want_b
+void wgrad(const Tensor& dT, const Rows& x, const Tensor& codes, const Tensor& exps, bool want_a, const Tensor& T, const Rows& dy, bool want_b, long M,
+           const Bank& bank, const Plan& plan, long unit, Tensor& dA, Tensor& dB) {
   const auto f32 = bank.scales.options();
-  Tensor out = trans ? at::empty({bank.G, C, bank.r}, f32) : at::empty({bank.G, bank.r, C}, f32);
+  if (want_a) dA = at::empty({bank.G, bank.r, bank.K}, f32);
+  if (want_b) dB = at::empty({bank.G, bank.N, bank.r}, f32);
   const long rows = plan.live_units * unit;
-  const int n = aql_adapter_wgrad_scratch_floats(rows, plan.nused, (int)C, (int)bank.R);
+  const int n = aql_adapter_wgrad_scratch_floats(rows, plan.nused, want_a ? (int)bank.K : 0, want_b ? (int)bank.N : 0, (int)bank.R);
   if (n < 0) throw AqlErr("adapter_linear: the weight gradients' workspace passes 2^31 elements; train fewer rows or adapters per call");
-  const Tensor scratch = at::empty({n}, f32);
-  const auto st = stream_of(out);
-  ran(aql_adapter_wgrad(ptr<float>(u), (int)bank.R, ptr<bf16_t>(v.t), v.ld, ptr<uint8_t>(codes), ptr<uint8_t>(exps), M, (int)C, (int)bank.G, (int)bank.r,
-                        ptr<int>(bank.ranks), plan.part(2), plan.part(3), plan.part(4), plan.part(5), plan.part(6), plan.nsorted, plan.nused, plan.nslot, (int)unit,
-                        rows, trans, ptr<float>(out), n ? ptr<float>(scratch) : nullptr, n, st), "aql_adapter_wgrad", st);
-  return out;
+  Tensor scratch;
+  if (n) scratch = at::empty({n}, f32);
+  const auto st = stream_of(bank.scales);
+  ran(aql_adapter_wgrad(ptr<bf16_t>(dT), ptr<bf16_t>(x.t), x.ld, ptr<uint8_t>(codes), ptr<uint8_t>(exps), (int)bank.K, ptr<float>(dA), ptr<bf16_t>(T),
+                        ptr<bf16_t>(dy.t), dy.ld, (int)bank.N, ptr<float>(dB), M, (int)bank.G, (int)bank.R, (int)bank.r, ptr<int>(bank.ranks), plan.part(1),
+                        plan.part(2), plan.part(3), plan.nused, plan.nslot, (int)unit, rows, ptr<float>(scratch), n, st), "aql_adapter_wgrad", st);
 }
 
 struct AdapterLinear : torch::autograd::Function<AdapterLinear> {
@@ -298,7 +300,7 @@ struct AdapterLinear : torch::autograd::Function<AdapterLinear> {
                         c10::intrusive_ptr<Call> c, bool ckpt8, bool train) {
     Rows x = gemm_rows(x2d), res;
     if ((c->residual = residual.has_value())) res = gemm_rows(*residual);
-    auto [y, T] = product(x, c->w, c->bias, res, c->bank->a, c->bank->b, *c->bank, *c->plan, c->unit, c->N, c->K);
+    auto [y, T] = product(x, c->w, c->bias, res, c->bank->a, c->bank->b, *c->bank, *c->plan, c->unit, c->N, c->K, train && !ckpt8 ? 3 : 1);
     Tensor codes, exps, keep = x.t;
     c->train = train;
     if (!train) {
@@ -333,16 +335,11 @@ struct AdapterLinear : torch::autograd::Function<AdapterLinear> {
         Tensor dT, T = s[1];
         Rows x;
         if (s[0].defined()) x = {s[0], c->M > 1 ? s[0].stride(0) : c->K};
-        if (want_x) std::tie(out[0], dT) = product(dy, c->wt, Tensor(), Rows(), bank.bt, bank.at, bank, *c->plan, c->unit, c->K, c->N);
-        if (c->train) {
-          if (want_a) {
-            if (!dT.defined() && c->plan->nseg) dT = down(dy, Tensor(), Tensor(), c->M, c->N, bank.bt, bank, *c->plan, c->unit);
-            out[1] = wgrad(dT, x, s[2], s[3], c->M, c->K, false, bank, *c->plan, c->unit);
-          }
-          if (want_b) {
-            if (!T.defined() && c->plan->nseg) T = down(Rows(), s[2], s[3], c->M, c->K, bank.a, bank, *c->plan, c->unit);
-            out[2] = wgrad(T, dy, Tensor(), Tensor(), c->M, c->N, true, bank, *c->plan, c->unit);
-          }
+        if (want_x) std::tie(out[0], dT) = product(dy, c->wt, Tensor(), Rows(), bank.bt, bank.at, bank, *c->plan, c->unit, c->K, c->N, c->train && want_a ? 3 : 1);
+        if (c->train && (want_a || want_b)) {
+          if (want_a && !dT.defined() && c->plan->nseg) dT = down(dy, Tensor(), Tensor(), c->M, c->N, bank.bt, bank, *c->plan, c->unit);
+          if (want_b && !T.defined() && c->plan->nseg) T = down(Rows(), s[2], s[3], c->M, c->K, bank.a, bank, *c->plan, c->unit);
+          wgrad(dT, x, s[2], s[3], want_a, T, dy, want_b, c->M, bank, *c->plan, c->unit, out[1], out[2]);
         }
       }
       if (want_r) out[3] = g[0];
@@ -378,7 +375,7 @@ Tensor adapter_linear(const Tensor& x, const Tensor& w, const Tensor& wt, const 
   }
   Rows r;
   if (res.defined()) r = gemm_rows(res);
-  return product(gemm_rows(x), w, bias, r, bank->a, bank->b, *bank, *plan, unit, N, K).first;
+  return product(gemm_rows(x), w, bias, r, bank->a, bank->b, *bank, *plan, unit, N, K, 1).first;
 }
 
 }  // namespace
@@ -407,7 +404,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def(py::init<>())
       .def_readwrite("table", &Plan::table).def_readwrite("start", &Plan::start).def_readwrite("at", &Plan::at)
       .def_readwrite("units", &Plan::units).def_readwrite("requests", &Plan::requests).def_readwrite("live_units", &Plan::live_units)
-      .def_readwrite("nseg", &Plan::nseg).def_readwrite("nsorted", &Plan::nsorted).def_readwrite("nused", &Plan::nused).def_readwrite("nslot", &Plan::nslot)
+      .def_readwrite("nseg", &Plan::nseg).def_readwrite("nused", &Plan::nused).def_readwrite("nslot", &Plan::nslot)
       .def_readwrite("max_id", &Plan::max_id).def_readwrite("equal", &Plan::equal)
       .def("unit", &Plan::unit).def("slots", &Plan::slots);
 }

@@ -223,27 +223,28 @@ int aql_groupnorm_silu_bwd(const bf16_t* x, const bf16_t* dy, int B, int HW, int
 /* ---- low-rank adapters of many requests beside one projection (csrc/aql_adapter.hip) --------------------------------------------------
  *   T[m] = scales[g] A[g] x_m,   Y[m] = W x_m + bias + B[g] T[m] + residual[m],   g = the adapter of row m (none: Y = W x + bias + residual)
  * A: [G][R][K], B: [G][N][R] bf16, stacked at one rank R (a multiple of 8); rows of A / columns of B past ranks[g] are taken as zeros.
- * Segments: rows [seg_start[s] unit, seg_start[s + 1] unit) have adapter seg_id[s] (-1: none), s < nseg, none empty, together all M rows;
- * nseg = 0: no adapters at all.  slots: the most segments that meet in 16 rows [16 i, 16 i + 16).  All tables are device memory; ids are not
- * checked against G here (the binding does).  T: [M][R] fp32, out; rows without an adapter are left as they are.
+ * Row m has adapter unit_id[m / unit] (-1: none); the M / unit (rounded up) ids are device memory and not checked against G here (the binding does).
+ * runs: stretches of neighbouring rows with one adapter, 0: no adapters at all; slots (1..16): at least the adapters that any 16 rows
+ * [16 i, 16 i + 16) meet.  T: [M][parts][R] bf16, out: T rounded (parts = 1), or T = hi + mid + lo in three parts for a
+ * later aql_adapter_wgrad (parts = 3); rows without an adapter are left as they are.
  * Backward data: the same entry with X = dY, W = W^T [K][N], A = B^T [G][R][N], B = A^T [G][K][R]: T is dT, Y is dX.
  * N, K, leading dimensions: multiples of 8; pointers 16-byte aligned.  One fp32 accumulator per output, rounded to bf16 once.          */
 int aql_adapter_linear(const bf16_t* X, long ldx, const bf16_t* W, long ldw, const bf16_t* bias, const bf16_t* residual, long ldr, bf16_t* Y,
                        long ldy, long M, int N, int K, const bf16_t* A, const bf16_t* B, const int* ranks, const float* scales, int R,
-                       const int* seg_start, const int* seg_id, int nseg, int unit, int slots, float* T, aql_stream_t stream);
+                       const int* unit_id, int unit, int runs, int slots, bf16_t* T, int parts, aql_stream_t stream);
 /* T alone, from X or from its 8-bit checkpoint (exactly one of the two) */
 int aql_adapter_down(const bf16_t* X, long ldx, const uint8_t* codes, const uint8_t* exps, long M, int K, const bf16_t* A, const int* ranks,
-                     const float* scales, int R, const int* seg_start, const int* seg_id, int nseg, int unit, int slots, float* T,
-                     aql_stream_t stream);
-/* Weight gradients: out[g] = sum over the rows m of adapter g of U[m] V[m]^T ([r_out][C]; trans: [C][r_out]), zeros for an adapter without rows
- * and past ranks[g].  dA: U = dT, V = X (or its checkpoint), C = K.  dB: U = T, V = dY, C = N, trans = 1.  Rows in sorted order: the k-th
- * segment (adapter by adapter) begins at row seg_start[k] and at position seg_pos[k]; the j-th used adapter used_id[j] holds the positions
- * [used_pos[j], used_pos[j + 1]); slot[g] = j or -1, g < nslot; all in units.  rows: positions in all, in rows.  The same bits every time.
- * scratch: aql_adapter_wgrad_scratch_floats(rows, nused, C, R) fp32 elements (-1: too large).                                          */
-int aql_adapter_wgrad_scratch_floats(long rows, int nused, int C, int R);
-int aql_adapter_wgrad(const float* U, int R, const bf16_t* V, long ldv, const uint8_t* codes, const uint8_t* exps, long M, int C, int G, int r_out,
-                      const int* ranks, const int* seg_start, const int* seg_pos, const int* used_pos, const int* used_id, const int* slot,
-                      int nseg, int nused, int nslot, int unit, long rows, int trans, float* out, float* scratch, long scratch_floats,
+                     const float* scales, int R, const int* unit_id, int unit, int runs, int slots, bf16_t* T, int parts, aql_stream_t stream);
+/* Weight gradients, both or one (the other's result null):
+ *   dA[g] = sum over the rows m of adapter g of dT[m] x_m^T  ([r_out][K], x_m from X or its checkpoint),  dB[g] = sum of dY[m] T[m]^T  ([N][r_out])
+ * in fp32, overwritten, G of each; zeros for an adapter without rows and past ranks[g].  dT, T: three parts as above.  Rows in sorted order (adapter
+ * by adapter): perm[p] is the unit of rows at position p, the j-th used adapter holds the positions [used_pos[j], used_pos[j + 1]), slot[g] = j
+ * or -1 for g < nslot, all in units of `unit` rows; rows: those that have an adapter.  The same bits every time.
+ * scratch: aql_adapter_wgrad_scratch_floats(rows, nused, K, N, R) fp32 elements (K or N = 0: not asked for; -1: too large).             */
+int aql_adapter_wgrad_scratch_floats(long rows, int nused, int K, int N, int R);
+int aql_adapter_wgrad(const bf16_t* dT, const bf16_t* X, long ldx, const uint8_t* codes, const uint8_t* exps, int K, float* dA, const bf16_t* T,
+                      const bf16_t* dY, long lddy, int N, float* dB, long M, int G, int R, int r_out, const int* ranks, const int* perm,
+                      const int* used_pos, const int* slot, int nused, int nslot, int unit, long rows, float* scratch, long scratch_floats,
                       aql_stream_t stream);
 /* LayerNorm that trains its own weights (csrc/aql_lnorm_train.hip): rows of any width up to 8192 and any row stride (`ldx`, elements),
  * element alignment; dtype / param_dtype 0 = bf16, 1 = fp32 (of x, y, dy, dres, dx / of gamma, beta); beta may be null.  stats: [M][2] fp32 (mean, rstd).

@@ -334,20 +334,22 @@ def test_refusals_without_a_gpu():
         adapters.AdapterBank(torch.zeros(1, 4, 8), torch.zeros(1, 8, 4), device="cpu")
     lib, p = _lib.load(), _lib.c_p(4096)               # p is never dereferenced: every call is refused on the host
 
-    def linear(M=64, N=64, K=64, R=8, ldx=64, X=p, T=p, slots=2, nseg=1, unit=1, seg=p):
-        return lib.aql_adapter_linear(X, ldx, p, K, None, None, 0, p, N, M, N, K, p, p, p, p, R, seg, seg, nseg, unit, slots, T, None)
+    def linear(M=64, N=64, K=64, R=8, ldx=64, X=p, T=p, slots=2, nseg=1, unit=1, seg=p, parts=1):
+        return lib.aql_adapter_linear(X, ldx, p, K, None, None, 0, p, N, M, N, K, p, p, p, p, R, seg, unit, nseg, slots, T, parts, None)
     for kw in (dict(N=60), dict(K=60, ldx=64), dict(ldx=56), dict(R=4), dict(R=0), dict(X=None), dict(T=None), dict(slots=0), dict(slots=17), dict(unit=0),
-               dict(seg=None), dict(nseg=-1), dict(X=_lib.c_p(4104)), dict(M=-1), dict(M=1 << 31), dict(ldx=1 << 21)):
+               dict(seg=None), dict(nseg=-1), dict(X=_lib.c_p(4104)), dict(M=-1), dict(M=1 << 31), dict(ldx=1 << 21), dict(parts=2)):
         assert linear(**kw) != 0, kw
     assert linear(M=0) == 0
-    assert lib.aql_adapter_down(p, 64, p, p, 64, 64, p, p, p, 8, p, p, 1, 1, 2, p, None) != 0       # both sources
-    assert lib.aql_adapter_down(None, 0, None, None, 64, 64, p, p, p, 8, p, p, 1, 1, 2, p, None) != 0
-    need = lib.aql_adapter_wgrad_scratch_floats(64, 2, 64, 8)
-    assert need > 0 and lib.aql_adapter_wgrad_scratch_floats(1 << 30, 60000, 1 << 14, 1024) == -1
+    assert lib.aql_adapter_down(p, 64, p, p, 64, 64, p, p, p, 8, p, 1, 1, 2, p, 3, None) != 0       # both sources
+    assert lib.aql_adapter_down(None, 0, None, None, 64, 64, p, p, p, 8, p, 1, 1, 2, p, 3, None) != 0
+    need = lib.aql_adapter_wgrad_scratch_floats(64, 2, 64, 64, 8)
+    assert need > 0 and lib.aql_adapter_wgrad_scratch_floats(1 << 30, 60000, 1 << 14, 1 << 14, 1024) == -1
+    assert 0 < lib.aql_adapter_wgrad_scratch_floats(64, 2, 64, 0, 8) < need
 
-    def wgrad(V=p, codes=None, r=8, rows=64, n=need, G=3, C=64):
-        return lib.aql_adapter_wgrad(p, 8, V, 64, codes, codes, 64, C, G, r, p, p, p, p, p, p, 2, 2, 3, 1, rows, 0, p, p, n, None)
-    for kw in (dict(codes=p), dict(V=None), dict(r=9), dict(rows=65), dict(n=need - 1), dict(G=0), dict(G=1 << 16), dict(C=60)):
+    def wgrad(X=p, codes=None, r=8, rows=64, n=need, G=3, K=64, unit=1, dA=p, dB=p, dY=p, dT=p):
+        return lib.aql_adapter_wgrad(dT, X, 64, codes, codes, K, dA, p, dY, 64, 64, dB, 64, G, 8, r, p, p, p, p, 2, 3, unit, rows, p, n, None)
+    for kw in (dict(codes=p), dict(X=None), dict(r=9), dict(rows=65), dict(n=need - 1), dict(G=0), dict(G=1 << 16), dict(K=60), dict(unit=0), dict(unit=3),
+               dict(dA=None, dB=None), dict(dY=None), dict(dT=None)):
         assert wgrad(**kw) != 0, kw
 
 

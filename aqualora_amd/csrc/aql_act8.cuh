@@ -22,14 +22,20 @@ __device__ __forceinline__ uint32_t exp_byte(uint32_t amax_bits) {   // amax_bit
 __device__ __forceinline__ float inv_step(uint32_t b) { return b == 255u ? 0.f : __uint_as_float((254u - b) << 23); }
 __device__ __forceinline__ float step(uint32_t b) { return b == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(b << 23); }
 
-// four codes in one word.  1.5 2^23 + v rounds v to the nearest even integer and leaves it, in two's complement, in the low byte
-__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float inv) {
+// four codes in one word.  The clamp to +-127 steps comes before the scaling (both are exact), then 1.5 2^23 + v / step rounds to the nearest even integer
+// and leaves it, in two's complement, in the low byte
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float inv, float lim) {
   constexpr float MAGIC = 12582912.f;
-  const uint32_t ua = __float_as_uint(__builtin_amdgcn_fmed3f(a * inv, -127.f, 127.f) + MAGIC);
-  const uint32_t ub = __float_as_uint(__builtin_amdgcn_fmed3f(b * inv, -127.f, 127.f) + MAGIC);
-  const uint32_t uc = __float_as_uint(__builtin_amdgcn_fmed3f(c * inv, -127.f, 127.f) + MAGIC);
-  const uint32_t ud = __float_as_uint(__builtin_amdgcn_fmed3f(d * inv, -127.f, 127.f) + MAGIC);
-  return (ua & 255u) | ((ub & 255u) << 8) | ((uc & 255u) << 16) | (ud << 24);
+  const uint32_t ua = __float_as_uint(fmaf(__builtin_amdgcn_fmed3f(a, -lim, lim), inv, MAGIC));
+  const uint32_t ub = __float_as_uint(fmaf(__builtin_amdgcn_fmed3f(b, -lim, lim), inv, MAGIC));
+  const uint32_t uc = __float_as_uint(fmaf(__builtin_amdgcn_fmed3f(c, -lim, lim), inv, MAGIC));
+  const uint32_t ud = __float_as_uint(fmaf(__builtin_amdgcn_fmed3f(d, -lim, lim), inv, MAGIC));
+  return __builtin_amdgcn_perm(ub, ua, 0x0c0c0400u) | __builtin_amdgcn_perm(ud, uc, 0x04000c0cu);
+}
+// the eight codes of a chunk whose block has exponent byte b
+__device__ __forceinline__ uint2 codes8(const float* v, uint32_t b) {
+  const float inv = inv_step(b), lim = 127.f * step(b);
+  return make_uint2(codes4(v[0], v[1], v[2], v[3], inv, lim), codes4(v[4], v[5], v[6], v[7], inv, lim));
 }
 // value of byte i of a word of codes: (code + 128) comes out of one v_cvt_f32_ubyte; both further steps are exact
 template <int I>
@@ -119,11 +125,22 @@ __device__ __forceinline__ uint32_t quad_umax(uint32_t v) {
   o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false);            // quad_perm [2,3,0,1]
   return max(v, o);
 }
-__device__ __forceinline__ uint32_t amax_bits8(const float* v) {
+// bits of the largest magnitude of eight elements, as fp32
+__device__ __forceinline__ uint32_t amax_bits8(const Raw8<float>& r) {
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  for (int i = 0; i < 8; ++i) m = max(m, r.w[i] & 0x7fffffffu);
   return m;
+}
+__device__ __forceinline__ uint32_t amax_bits8(const Raw8<bf16_t>& r) {   // two at a time: magnitudes compare as unsigned integers
+  typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+  u16x2_t m = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = r.w[i] & 0x7fff7fffu;
+    m = __builtin_elementwise_max(m, *reinterpret_cast<const u16x2_t*>(&w));
+  }
+  return (uint32_t)max(m.x, m.y) << 16;
 }
 
 }  // namespace act8

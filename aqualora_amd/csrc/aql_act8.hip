@@ -17,10 +17,8 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ x, long
   float v[8];
   load_raw(x + (long)row * ldx + 8 * c, C - 8 * (int)c, r);
   widen(r, v);
-  const uint32_t b = exp_byte(quad_umax(amax_bits8(v)));
-  const float inv = inv_step(b);
-  const uint2 q = make_uint2(codes4(v[0], v[1], v[2], v[3], inv), codes4(v[4], v[5], v[6], v[7], inv));
-  *reinterpret_cast<uint2*>(codes + ((long)row * nchunk + c) * 8) = q;
+  const uint32_t b = exp_byte(quad_umax(amax_bits8(r)));
+  *reinterpret_cast<uint2*>(codes + ((long)row * nchunk + c) * 8) = codes8(v, b);
   if ((c & 3) == 0) exps[(long)row * (nchunk >> 2) + (c >> 2)] = (uint8_t)b;
 }
 

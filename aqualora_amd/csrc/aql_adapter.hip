@@ -349,11 +349,29 @@ __global__ __launch_bounds__(WGM * WGN * 64) void tile_kernel(const LinArgs a) {
   const long m0 = (long)(tile / tiles_n) * BM;
   const int n0 = (int)(tile % tiles_n) * BN;
   const int mlive = (int)min((long)BM, a.M - m0), nlive = min(BN, a.N - n0);
+  const long w0 = m0 + (wave / WGN) * WM;          // this wavefront's rows and columns
+  const int v0 = n0 + (wave % WGN) * WN;
+  // the fp32 sums begin with bias and residual: their loads run under the first copies instead of behind the last product, and there is one rounding
   f32x4_t acc[FM][FN];
 #pragma unroll
-  for (int i = 0; i < FM; ++i)
+  for (int j = 0; j < FN; ++j) {
+    const int n = min(v0 + j * 16 + q * 4, a.N - 4);   // (past the end: the last, never stored)
+    const uint2 b = a.bias ? *reinterpret_cast<const uint2*>(a.bias + n) : make_uint2(0u, 0u);
+    const f32x4_t bv = {bf16lo(b.x), bf16hi(b.x), bf16lo(b.y), bf16hi(b.y)};
 #pragma unroll
-    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < FM; ++i) acc[i][j] = bv;
+  }
+  if (a.res) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const bf16_t* p = a.res + min(w0 + i * 16 + i16, a.M - 1) * a.ldr;
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const uint2 r = *reinterpret_cast<const uint2*>(p + min(v0 + j * 16 + q * 4, a.N - 4));
+        acc[i][j] += f32x4_t{bf16lo(r.x), bf16hi(r.x), bf16lo(r.y), bf16hi(r.y)};
+      }
+    }
+  }
   Stage<BM, NW> sx;
   Stage<BN, NW> sw;
   sx.begin(a.X + m0 * a.ldx, a.ldx, a.K, tid, [&](int r) { return r < mlive; });
@@ -382,22 +400,16 @@ __global__ __launch_bounds__(WGM * WGN * 64) void tile_kernel(const LinArgs a) {
   if (a.rows.id != nullptr)
     for (int h = next_adapter<BM>(ids, -1, lane); h >= 0; h = next_adapter<BM>(ids, h, lane)) nk += rk;
   ring<BM, BN, WGM, WGN, NSTG>(lds, nk, tid, acc, issue);
-  // bias and residual are added to the fp32 sums before the one rounding
-  const long w0 = m0 + (wave / WGN) * WM;          // this wavefront's rows and columns
-  const int v0 = n0 + (wave % WGN) * WN;
 #pragma unroll
-  for (int j = 0; j < FN; ++j) {
-    const int n = v0 + j * 16 + q * 4;
-    if (n >= a.N) continue;
-    const uint2 b = a.bias ? *reinterpret_cast<const uint2*>(a.bias + n) : make_uint2(0u, 0u);
+  for (int i = 0; i < FM; ++i) {
+    const long m = w0 + i * 16 + i16;
+    if (m >= a.M) continue;
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      const long m = w0 + i * 16 + i16;
-      if (m >= a.M) continue;
-      const uint2 r = a.res ? *reinterpret_cast<const uint2*>(a.res + m * a.ldr + n) : make_uint2(0u, 0u);
+    for (int j = 0; j < FN; ++j) {
+      const int n = v0 + j * 16 + q * 4;
+      if (n >= a.N) continue;
       const f32x4_t v = acc[i][j];
-      *reinterpret_cast<uint2*>(a.Y + m * a.ldy + n) = make_uint2(pack_bf16x2(v[0] + bf16lo(b.x) + bf16lo(r.x), v[1] + bf16hi(b.x) + bf16hi(r.x)),
-                                                                  pack_bf16x2(v[2] + bf16lo(b.y) + bf16lo(r.y), v[3] + bf16hi(b.y) + bf16hi(r.y)));
+      *reinterpret_cast<uint2*>(a.Y + m * a.ldy + n) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
     }
   }
 }

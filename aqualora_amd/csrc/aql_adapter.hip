@@ -738,13 +738,14 @@ extern "C" int aql_adapter_linear(const bf16_t* X, long ldx, const bf16_t* W, lo
   hipLaunchKernelGGL((tile_kernel<BM, BN, WGM, WGN, NSTG>), dim3((unsigned)(((M + BM - 1) / BM) * ((N + BN - 1) / BN))), dim3(WGM * WGN * 64), 0, stream, a)
     // Which tile (all measured at every one of these sizes; us, best first): 256 x 320 where the width allows it and every CU gets one (4096 x 10240 x 1280:
     // 115.8 / 154 with 128 x 160); else 128 rows by 160 or 128 columns, whichever needs less time for its rounds of two tiles per CU
-    // (32768 x 320 x 320: 15.1 / 19.4; 9001 x 1280 x 1280: 41.6 with 128, 45.9 with 160); smaller ones where those leave CUs idle (2048 x 1280 x
+    // (32768 x 320 x 320: 15.1 / 19.4; 9001 x 1280 x 1280: 40.8 with 128, 45.9 with 160; 128 x 128 on eight wavefronts, on four 59.8 against 55.9 with
+    // the low-rank term); smaller ones where those leave CUs idle (2048 x 1280 x
     // 1280: 14.9 with 64 x 128, 18.2 with 128 x 128; 1001 x 640 x 768: 6.3 with 64 x 64, 8.4 with 64 x 128)
     const auto tiles = [&](long bm, long bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
     if (N % 320 == 0 && tiles(256, 320) >= 256) AQL_TILE(256, 320, 2, 4, 2);
     else if (tiles(128, 128) >= 256 && (tiles(128, 160) + 511) / 512 * 160 <= (tiles(128, 128) + 511) / 512 * 128) AQL_TILE(128, 160, 2, 2, 2);
-    else if (tiles(128, 128) >= 256) AQL_TILE(128, 128, 2, 2, 2);
-    else if (tiles(64, 128) >= 256) AQL_TILE(64, 128, 2, 2, 3);
+    else if (tiles(128, 128) >= 256) AQL_TILE(128, 128, 2, 4, 2);
+    else if (tiles(64, 128) >= 256) AQL_TILE(64, 128, 2, 4, 3);
     else AQL_TILE(64, 64, 2, 2, 3);
 #undef AQL_TILE
   }

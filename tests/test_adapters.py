@@ -24,6 +24,9 @@ CASES = {
     "equal_77": ((5, 385), [0, 3, 1, 3, -1], 768, 640, 64),
     "tiles_of_128": ([1030, 1, 2000, 1169], [1, 0, 2, 1], 72, 1032, 8),
     "large_rank": ([130, 70, 200], [1, 0, 1], 200, 320, 320),
+    "whole_rows_in_one_launch": ([9000, 130, 5, 15500], [1, 0, -1, 2], 200, 264, 40),
+    "wide_tiles": ([7000, 3000, 6400], [0, 1, 0], 72, 1600, 16),
+    "columns_of_160": ([20000, 13000], [1, 0], 64, 320, 72),
     "neighbours_of_one_adapter": ([16, 16, 16, 300], [1, 1, 0, 0], 64, 64, 12),
     "no_adapters": ([3, 270], [-1, -1], 64, 72, 8),
 }

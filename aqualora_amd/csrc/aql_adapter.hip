@@ -69,7 +69,7 @@ struct DownArgs {
   Rows rows;
 };
 
-// Few rows, short requests or 8-bit codes.  One workgroup: 16 rows x 16 RT adapter rows of ONE adapter (blockIdx.y counts the adapters that the row
+// Few rows or short requests.  One workgroup: 16 rows x 16 RT adapter rows of ONE adapter (blockIdx.y counts the adapters that the row
 // tile meets); its NW wavefronts split the contraction and join in LDS.  Fragments come straight from memory, four steps of 32 columns at a time
 // (all their loads in flight together): lane (i = lane & 15, q = lane >> 4) holds row i, columns k + 8 q .. k + 8 q + 7 of either operand, and
 // gets T[m = lane & 15][r = 4 q + e] back.
@@ -466,6 +466,101 @@ __global__ __launch_bounds__(256) void down_tile_kernel(const DownArgs a) {
   }
 }
 
+// The same from 8-bit codes: a thread turns 16 codes of a row into bf16 on their way into LDS (exact), one stage ahead of the product, with the next
+// stage's codes on their way from memory; A comes by copies as above.
+template <int BN>
+__global__ __launch_bounds__(256) void down8_tile_kernel(const DownArgs a) {
+  constexpr int BM = 64, FM = 2, FN = BN / 32, NSTG = 3, STAGE = (BM + BN) * 128;
+  __shared__ __attribute__((aligned(16))) char lds[NSTG * STAGE + BM * 4];   // (one array: see tile_kernel)
+  int* ids = reinterpret_cast<int*>(lds + NSTG * STAGE);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = lane & 15, q = lane >> 4;
+  const uint32_t tiles_r = (a.R + BN - 1) / BN, tile = xcd_tile(blockIdx.x, gridDim.x);
+  const long m0 = (long)(tile / tiles_r) * BM;
+  const int r0 = (int)(tile % tiles_r) * BN;
+  const int mlive = (int)min((long)BM, a.M - m0), rlive = min(BN, a.R - r0);
+  if (tid < BM) ids[tid] = tid < mlive ? id_of(a.rows, m0 + tid) : -1;
+  __syncthreads();
+  const int nb = (a.K + 31) / 32, nk = (a.K + BK - 1) / BK;   // blocks of a row, stages
+  const int xr = tid >> 2, xc = (tid & 3) * 16;               // this thread's row, and its 16 columns of a stage
+  const uint8_t* cr = a.codes + (m0 + min(xr, mlive - 1)) * (long)nb * 32;
+  const uint8_t* er = a.exps + (m0 + min(xr, mlive - 1)) * (long)nb;
+  int turn = 0;
+  for (int g = next_adapter<BM>(ids, -1, lane); g >= 0; g = next_adapter<BM>(ids, g, lane), ++turn) {
+    if ((turn & 1) != (int)blockIdx.y) continue;
+    f32x4_t acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    Stage<BN, 4> sa;
+    sa.begin(a.A + ((long)g * a.R + r0) * a.K, a.K, a.K, tid, [&](int r) { return r < rlive; });
+    uint4 code;
+    uint32_t ex;
+    auto load = [&](int t) {   // past the row's last block: the first again, the row of A is zero there
+      const int k = t * BK + xc, kk = k < nb * 32 ? k : 0;
+      code = *reinterpret_cast<const uint4*>(cr + kk);
+      ex = er[kk >> 5];
+      ex = k < nb * 32 ? ex : 1u;
+    };
+    auto put = [&](int st) {
+      const float sp = act8::step(ex);
+      float v[8];
+      act8::values4(code.x, sp, v);
+      act8::values4(code.y, sp, v + 4);
+      *reinterpret_cast<bf16x8_t*>(lds + st * STAGE + lds_off(xr, xc >> 3)) = pack8(v);
+      act8::values4(code.z, sp, v);
+      act8::values4(code.w, sp, v + 4);
+      *reinterpret_cast<bf16x8_t*>(lds + st * STAGE + lds_off(xr, (xc >> 3) + 1)) = pack8(v);
+    };
+    load(0);
+    sa.fetch(lds + BM * 128, wave);
+    put(0);
+    sa.fetch(lds + STAGE + BM * 128, wave);
+    load(1);
+    int rd = 0;
+    for (int t = 0; t < nk; ++t) {
+      const int nx = rd + 1 == NSTG ? 0 : rd + 1, fr = nx + 1 == NSTG ? 0 : nx + 1;
+      // still in flight: the next stage's copies and the codes behind them.  Stage t's codes are in LDS when everybody's writes are done
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(BN / 32 + 2) : "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      put(nx);
+      sa.fetch(lds + fr * STAGE + BM * 128, wave);
+      load(t + 2);
+      const char *pa = lds + rd * STAGE, *pb = pa + BM * 128;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        bf16x8_t fa[FM], fb[FN];
+#pragma unroll
+        for (int j = 0; j < FN; ++j) fb[j] = *reinterpret_cast<const bf16x8_t*>(pb + lds_off((wave & 1) * (BN / 2) + j * 16 + i16, ks * 4 + q));
+#pragma unroll
+        for (int i = 0; i < FM; ++i) fa[i] = *reinterpret_cast<const bf16x8_t*>(pa + lds_off((wave >> 1) * 32 + i * 16 + i16, ks * 4 + q));
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int j = 0; j < FN; ++j) acc[i][j] = mfma(fb[j], fa[i], acc[i][j]);
+      }
+      rd = nx;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const float sc = a.scales[g];
+    const int rank = a.ranks[g];
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const int mr = (wave >> 1) * 32 + i * 16 + i16;
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const int r = r0 + (wave & 1) * (BN / 2) + j * 16 + q * 4;
+        float o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = r + e < rank ? sc * acc[i][j][e] : 0.f;
+        if (ids[mr] == g && r < a.R) store_t4(a.T + (m0 + mr) * a.P * a.R + r, a.R, a.P, o);
+      }
+    }
+    __syncthreads();   // the stages are free for the next adapter
+  }
+}
+
 // ------------------------------------------------------------------------------------------------------------------ weight gradients
 // The rows of all adapters in sorted order (adapter by adapter) are one axis of `rows` positions, cut into chunks of `chunk` positions.  A workgroup
 // takes one chunk x 128 columns of V x RB columns of U; where adapters change inside its chunk it finishes one and begins the next.  Piece
@@ -505,7 +600,8 @@ struct Grad {            // one gradient: dA (U = dT, V = X or its codes) or dB 
 // of the latency is hidden by the other workgroups of the CU (three: the registers allow no more; with two tiles on their way one fits, 41 against 25 us).
 template <int RB, bool CODES, bool TRANS>   // TRANS: partial sums as [C][R] (dB), else [R][C] (dA)
 __device__ __forceinline__ void wgrad_body(const Grad& G, int R, const Order& o, uint32_t id, char* vt, char* ut) {
-  constexpr int TK = 64, CB = 128, PV = 256, PU = RB == 32 ? 256 : 512, FU = RB / 16;
+  constexpr int TK = 64, CB = 128, PV = 256, PU = RB == 32 ? 256 : 512;
+  constexpr int WU = RB / 32, WV = 4 / WU, FV = CB / WV / 16, FU = 2;   // wavefronts WV x WU, FV x FU fragments each (fewer LDS reads than 4 x 1)
   constexpr int NV = TK * CB / 8 / 256, NU = TK * RB / 8 / 256;   // 16-byte chunks of V, and of each part of U, per thread
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int C = G.C, tc = (C + CB - 1) / CB, tr = (R + RB - 1) / RB;
@@ -518,6 +614,7 @@ __device__ __forceinline__ void wgrad_body(const Grad& G, int R, const Order& o,
     if ((long)o.used_pos[mid] * o.unit <= p_begin) j = mid;
     else hi = mid;
   }
+  const int wv0 = wave / WU * (CB / WV), wu0 = wave % WU * 32;
   const int cp = (C + 31) / 32 * 32;
   const int vrow = tid >> 4, vch = tid & 15, vc = c0 + vch * 8;
   const int urow = tid / (RB / 8), uch = tid % (RB / 8), ur = r0 + uch * 8;
@@ -559,9 +656,9 @@ __device__ __forceinline__ void wgrad_body(const Grad& G, int R, const Order& o,
   };
   for (long p = p_begin; p < p_end; ++j) {
     const long piece_end = min(p_end, (long)o.used_pos[j + 1] * o.unit);
-    f32x4_t acc[2][FU];   // 32 columns of V per wavefront
+    f32x4_t acc[FV][FU];
 #pragma unroll
-    for (int v = 0; v < 2; ++v)
+    for (int v = 0; v < FV; ++v)
 #pragma unroll
       for (int u = 0; u < FU; ++u) acc[v][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     rows_of(p, piece_end);
@@ -593,26 +690,26 @@ __device__ __forceinline__ void wgrad_body(const Grad& G, int R, const Order& o,
       rows_of(p + 2 * TK, piece_end);
 #pragma unroll
       for (int s = 0; s < TK / 32; ++s) {
-        bf16x8_t fv[2];
+        bf16x8_t fv[FV];
 #pragma unroll
-        for (int v = 0; v < 2; ++v) fv[v] = tr_frag<PV>(vt, s, wave * 32 + v * 16, lane);
+        for (int v = 0; v < FV; ++v) fv[v] = tr_frag<PV>(vt, s, wv0 + v * 16, lane);
 #pragma unroll
         for (int h = 2; h >= 0; --h)
 #pragma unroll
           for (int u = 0; u < FU; ++u) {
-            const bf16x8_t fu = tr_frag<PU>(ut, s, h * RB + u * 16, lane);
+            const bf16x8_t fu = tr_frag<PU>(ut, s, h * RB + wu0 + u * 16, lane);
 #pragma unroll
-            for (int v = 0; v < 2; ++v) acc[v][u] = TRANS ? mfma(fu, fv[v], acc[v][u]) : mfma(fv[v], fu, acc[v][u]);
+            for (int v = 0; v < FV; ++v) acc[v][u] = TRANS ? mfma(fu, fv[v], acc[v][u]) : mfma(fv[v], fu, acc[v][u]);
           }
       }
     }
     p = piece_end;
     float* out = G.part + (long)(ck + j) * R * C;
 #pragma unroll
-    for (int v = 0; v < 2; ++v)
+    for (int v = 0; v < FV; ++v)
 #pragma unroll
       for (int u = 0; u < FU; ++u) {
-        const int cb = c0 + wave * 32 + v * 16, rb = r0 + u * 16, a = (lane >> 4) * 4, b = lane & 15;
+        const int cb = c0 + wv0 + v * 16, rb = r0 + wu0 + u * 16, a = (lane >> 4) * 4, b = lane & 15;
         if (TRANS) {   // lane: column b of V, columns a .. a + 3 of U
           if (cb + b < C && rb + a < R) *reinterpret_cast<f32x4_t*>(out + (long)(cb + b) * R + rb + a) = acc[v][u];
         } else {       // lane: column b of U, columns a .. a + 3 of V
@@ -686,8 +783,10 @@ double wgrad_floats(long rows, int nused, int C, int R) {
 // 7.6 / 17.6; 4096 x 1280, rank 32 (64 tiles): 6.9 / 6.0; 1001 x 768, rank 64 (16 tiles): 6.7 / 6.3; 1000 x 2560, rank 32 (16 tiles): 10.7 / 9.0.
 void launch_down(const DownArgs& a, int runs, int slots, hipStream_t st) {
   const long tiles = (a.M + 63) / 64 * (a.R <= 32 ? 1 : (a.R + 63) / 64);
-  if (!a.codes && a.M / runs >= 64 && tiles >= 96) {
-    if (a.R <= 32) hipLaunchKernelGGL((down_tile_kernel<32, 4>), dim3((unsigned)tiles, 2), dim3(256), 0, st, a);
+  if (a.M / runs >= 64 && tiles >= 96) {
+    if (a.codes && a.R <= 32) hipLaunchKernelGGL((down8_tile_kernel<32>), dim3((unsigned)tiles, 2), dim3(256), 0, st, a);
+    else if (a.codes) hipLaunchKernelGGL((down8_tile_kernel<64>), dim3((unsigned)tiles, 2), dim3(256), 0, st, a);
+    else if (a.R <= 32) hipLaunchKernelGGL((down_tile_kernel<32, 4>), dim3((unsigned)tiles, 2), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((down_tile_kernel<64, 4>), dim3((unsigned)tiles, 2), dim3(256), 0, st, a);
     return;
   }

@@ -118,6 +118,7 @@ class RequestPlan:
         if ids.size and ids.min() < -1:
             raise ValueError("RequestPlan: adapters are numbered from 0; -1 is none")
         self.equal = lengths is None
+        self.adapters, self.device = [int(a) for a in ids], dev
         self.requests = int(ids.size)
         n = np.ones(ids.size, dtype=np.int64) if self.equal else np.asarray([int(x) for x in lengths], dtype=np.int64)
         if n.size != ids.size or (n.size and n.min() < 0):

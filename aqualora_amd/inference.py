@@ -3,6 +3,7 @@ sample latents with DDIM + classifier-free guidance.
 
   create_watermark_lora  scripts/create_wm_lora.py:9-51   down' = diag(S(m)) . down . scale   (conv: down * S[:,None,None,None])
   fuse_lora              pipe.fuse_lora(lora_scale) as used at evaluation/utils_eval.py:81-82: W += lora_scale . up @ down
+  attach_adapters        several owners' baked LoRAs beside one set of weights: every image of a batch through its own (adapters.RequestPlan)
   ddim_sample            StableDiffusionPipeline + DDIMScheduler (utils_eval.py:83-126): 50 steps, leading spacing,
                          steps_offset 1, eta 0, guidance 7.5 (recalled semantics; unpinned)
 The VAE decode that turns latents into pixels is outside this path.
@@ -11,6 +12,7 @@ import torch
 
 from . import _lib as L
 from . import ops
+from .adapters import AdapterBank, RequestPlan
 from .checkpoint import site_to_ckpt_key
 from .lora import _walk, load_unet_keys
 from .watermark import sd15_alphas_cumprod
@@ -62,6 +64,35 @@ def fuse_lora(unet, lora_state_dict, lora_scale=1.0, keys=None):
         host.set_lora_layer(None)
 
 
+@torch.no_grad()
+def attach_adapters(unet, lora_state_dicts, lora_scales=None, keys=None, trainable=False):
+    """Put one AdapterBank on every LoRA site of the U-Net, adapter i from ``lora_state_dicts[i]`` (the keys of `create_watermark_lora` /
+    ``pytorch_lora_weights.safetensors``, or ``<site>.{down,up}.weight`` as `checkpoint.load_lora_state` gives them; ranks may differ),
+    multiplied by ``lora_scales[i]``.  The weights stay as they are: `fuse_lora` serves one owner per model copy, this serves all of them from
+    one -- ``unet(..., cross_attention_kwargs={"scale": RequestPlan([owner of each image])})``, or ``scale=`` of the samplers.  Returns the
+    banks by site (``trainable``: their parameters learn)."""
+    if not lora_state_dicts:
+        raise ValueError("attach_adapters: no adapters")
+    keys = keys if keys is not None else load_unet_keys(unet)
+    scales = [1.0] * len(lora_state_dicts) if lora_scales is None else list(lora_scales)
+    banks = {}
+    for key in keys:
+        host = _walk(unet, key)
+        ck = site_to_ckpt_key(key)
+        pairs = []
+        for sd in lora_state_dicts:
+            name = ck if ck + ".down.weight" in sd else key
+            d, u = sd[name + ".down.weight"].float(), sd[name + ".up.weight"].float()
+            pairs.append((d.reshape(d.shape[0], -1), u.reshape(u.shape[0], -1)))
+        ranks = [d.shape[0] for d, _ in pairs]
+        r = max(ranks)
+        pad = torch.nn.functional.pad
+        down = torch.stack([pad(d, (0, 0, 0, r - d.shape[0])) for d, _ in pairs])
+        up = torch.stack([pad(u, (0, r - u.shape[1])) for _, u in pairs])
+        host.adapter_bank = banks[key] = AdapterBank(down, up, ranks=ranks, scales=scales, trainable=trainable, device=host.weight.device)
+    return banks
+
+
 def ddim_timesteps(num_inference_steps, num_train_timesteps=1000, steps_offset=1):
     ratio = num_train_timesteps // num_inference_steps
     return [(i * ratio) + steps_offset for i in range(num_inference_steps)][::-1]
@@ -69,9 +100,14 @@ def ddim_timesteps(num_inference_steps, num_train_timesteps=1000, steps_offset=1
 
 @torch.no_grad()
 def _cfg_scale(scale, B):
-    """Per-sample LoRA scale of a guided (2B) U-Net call.  ``scale`` is None (LoRA-free / fused U-Net), a float, or the
+    """Per-sample LoRA scale of a guided (2B) U-Net call.  ``scale`` is None (LoRA-free / fused U-Net), a float, a RequestPlan (the owner
+    of each image: `attach_adapters`), or the
     [B, r] (or [1, r]) per-message diagonal of the un-fused watermark LoRA; rob_enhance_finetune.py:1002 concatenates it
     for the unconditional and conditional halves: ``cat([mapper(m)] * 2) * 1.03``."""
+    if isinstance(scale, RequestPlan):
+        if not scale.equal or scale.requests != B:
+            raise ValueError(f"sampling {B} images needs a RequestPlan of {B} requests without lengths")
+        return RequestPlan(scale.adapters * 2, device=scale.device)
     if scale is None or not torch.is_tensor(scale):
         return scale
     s = scale if scale.shape[0] == B else scale.expand(B, scale.shape[1])

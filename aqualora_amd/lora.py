@@ -15,6 +15,8 @@ image) and the injection / patch loops of train/ppft_train.py:620-689 (``inject_
 ``scale`` follows the reference: a float multiplies the LoRA branch, a ``[B, r]`` tensor is the per-message
 diagonal S (``B.diag(S).A``).  ``scale=None`` is an extension: skip the LoRA branch (bit-identical to the
 reference's all-zero scale of the "clean" pass, ppft_train.py:1026-1029, without spending the FLOPs).
+``scale=adapters.RequestPlan(...)`` is another: every sample of the batch runs through its own owner's adapter (the banks that
+``inference.attach_adapters`` put on the hosts) beside the shared projection.
 The fused host forwards also accept ``residual=`` (added in the GEMM epilogue).
 """
 import types
@@ -23,6 +25,7 @@ import torch
 import torch.nn as nn
 
 from . import ops
+from .adapters import RequestPlan
 
 
 # ----------------------------------------------------------------------------- diffusers-compatible classes
@@ -191,6 +194,19 @@ def _run_linear(x2d, packed, lora_layer, scale, nb, rps, residual, geglu=False):
     return ops.lora_linear(x2d, packed, site, S, S16, rps, residual, geglu)
 
 
+def _run_adapters(host, x2d, plan, nb, residual, geglu=False):
+    """A host's forward under a RequestPlan: its bank (inference.attach_adapters), or the plain projection where it has none."""
+    bank = getattr(host, "adapter_bank", None)
+    if bank is None:
+        if host.lora_layer is not None:
+            raise ValueError("a RequestPlan needs adapter banks (inference.attach_adapters), but this module carries a LoRA layer and no bank")
+        return ops.lora_linear(x2d, _packed_linear(host), None, None, None, 1, residual, geglu)
+    if plan.equal and plan.requests != nb:
+        raise ValueError(f"RequestPlan of {plan.requests} requests for a batch of {nb}")
+    y = ops.adapter_linear(x2d, _packed_linear(host), bank, plan, residual=residual)
+    return ops.geglu(y) if geglu else y
+
+
 # ------------------------------------------------------------------------------------ the four forwards
 def CustomLoRACompatibleLinearforward(self, hidden_states, scale=1.0, residual=None, geglu=False):
     """nn.Linear.forward(x) [+ lora_layer(x, scale)]  -- one fused MFMA GEMM (reference lora_modules.py:56-62).
@@ -204,7 +220,10 @@ def CustomLoRACompatibleLinearforward(self, hidden_states, scale=1.0, residual=N
     nb = shp[0] if hidden_states.dim() >= 2 else 1
     rps = x2d.shape[0] // nb
     res2d = None if residual is None else residual.reshape(-1, self.out_features).contiguous()
-    y = _run_linear(x2d, _packed_linear(self), self.lora_layer, scale, nb, rps, res2d, geglu)
+    if isinstance(scale, RequestPlan):
+        y = _run_adapters(self, x2d, scale, nb, res2d, geglu)
+    else:
+        y = _run_linear(x2d, _packed_linear(self), self.lora_layer, scale, nb, rps, res2d, geglu)
     return y.reshape(*shp[:-1], y.shape[-1])
 
 
@@ -217,7 +236,10 @@ def CustomLoRACompatibleConvforward(self, hidden_states, scale=1.0, residual=Non
         B, C, H, W = x.shape
         x2d = ops.nhwc_view(x).reshape(B * H * W, C)
         res2d = None if residual is None else ops.nhwc_view(ops.as_cl(residual)).reshape(B * H * W, self.out_channels)
-        y = _run_linear(x2d, _packed_linear(self), self.lora_layer, scale, B, H * W, res2d)
+        if isinstance(scale, RequestPlan):
+            y = _run_adapters(self, x2d, scale, B, res2d)
+        else:
+            y = _run_linear(x2d, _packed_linear(self), self.lora_layer, scale, B, H * W, res2d)
         return y.view(B, H, W, self.out_channels).permute(0, 3, 1, 2)
     if k == (3, 3) and self.padding in ((1, 1), 1) and self.stride in ((1, 1), (2, 2)) and self.lora_layer is None:
         x = hidden_states if hidden_states.dtype == torch.bfloat16 else hidden_states.to(torch.bfloat16)

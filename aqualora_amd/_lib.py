@@ -231,6 +231,8 @@ def native():
         loader.exec_module(mod)
         if mod.abi_version() != ABI_VERSION:
             raise AqlError(f"{TORCH_LIB_PATH} calls a kernel library of AQL_ABI_VERSION {mod.abi_version()}, this binding expects {ABI_VERSION}: rebuild")
+        if mod.abi_address() != ctypes.cast(load().aql_abi_version, c_p).value:
+            raise AqlError(f"{TORCH_LIB_PATH} is not bound to {LIB_PATH}: link that with -Wl,-soname,libaqualora_hip.so, as the Makefile does")
         mod.set_error_class(AqlError)
         _native = mod
     return _native

@@ -4,6 +4,8 @@ rows belong to whom (`RequestPlan`), the two handles of `ops.adapter_linear`.
 A watermark LoRA that has been baked for an owner (`inference.create_watermark_lora`) is an ordinary LoRA with matrices of its own.  Fusing it
 into the weights serves one owner per model copy; `ops.lora_linear` shares one pair of matrices between all samples.  Here every request of a
 batch names its adapter, and the batch still runs the shared projection as one product."""
+import threading
+
 import numpy as np
 import torch
 import torch.nn as nn
@@ -49,7 +51,7 @@ class AdapterBank:
         self._live = torch.arange(self.rank, device=dev)[None] < h.ranks[:, None]      # [G, r]
         h.a = torch.zeros(self.G, self.R, self.K, dtype=torch.bfloat16, device=dev)
         h.b = torch.zeros(self.G, self.N, self.R, dtype=torch.bfloat16, device=dev)
-        self._transposed = False
+        self._transposed, self._lock = False, threading.Lock()
         self._ver = None
         if trainable:
             self.down = nn.Parameter(down.detach().to(device=dev, dtype=torch.float32, copy=True))
@@ -99,10 +101,13 @@ class AdapterBank:
             return
         if torch.cuda.is_current_stream_capturing():
             raise L.AqlError("AdapterBank: call lay_out_transposed() before capturing a pass that differentiates a frozen bank's input")
-        h = self.handle
-        h.at, h.bt = h.a.transpose(1, 2).contiguous(), h.b.transpose(1, 2).contiguous()
-        torch.cuda.current_stream(self.device).synchronize()      # once: later calls may come on other streams
-        self._transposed = True
+        with self._lock:                     # two threads may come here together: the first lays out
+            if self._transposed:
+                return
+            h = self.handle
+            h.at, h.bt = h.a.transpose(1, 2).contiguous(), h.b.transpose(1, 2).contiguous()
+            torch.cuda.current_stream(self.device).synchronize()      # once: later calls may come on other streams
+            self._transposed = True
 
 
 class RequestPlan:

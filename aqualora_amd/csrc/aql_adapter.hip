@@ -856,10 +856,10 @@ extern "C" int aql_adapter_linear(const bf16_t* X, long ldx, const bf16_t* W, lo
 extern "C" int aql_adapter_down(const bf16_t* X, long ldx, const uint8_t* codes, const uint8_t* exps, long M, int K, const bf16_t* A, const int* ranks,
                                 const float* scales, int R, const int* unit_id, int unit, int runs, int slots, bf16_t* T, int parts,
                                 hipStream_t stream) {
-  AQL_CHECK_ARG(M >= 0 && M < (1L << 31) - 256 && K > 0 && K % 8 == 0 && R > 0 && R % 8 == 0, "aql_adapter_down: bad shape M=%ld K=%d R=%d", M, K, R);
+  AQL_CHECK_ARG(M >= 0 && M < (1L << 31) - 256 && K > 0 && K % 8 == 0 && K < (1 << 21) && R > 0 && R % 8 == 0, "aql_adapter_down: bad shape M=%ld K=%d R=%d", M, K, R);
   AQL_CHECK_ARG(rows_ok(unit_id, runs, unit), "aql_adapter_down: bad rows");
   if (M == 0 || runs == 0) return AQL_OK;
-  AQL_CHECK_ARG(!codes == !exps && !X != !codes && (!X || (ldx >= K && ldx % 8 == 0 && ((uintptr_t)X & 15) == 0)) && A && ranks && scales && T && slots >= 1 && slots <= 16 && (parts == 1 || parts == 3),
+  AQL_CHECK_ARG(!codes == !exps && !X != !codes && (!X || (ldx >= K && ldx % 8 == 0 && ldx < (1L << 21) && ((uintptr_t)X & 15) == 0)) && A && ranks && scales && T && slots >= 1 && slots <= 16 && (parts == 1 || parts == 3),
                 "aql_adapter_down: bad operands (exactly one of X and its codes)");
   launch_down(DownArgs{X, codes, exps, A, ranks, scales, T, ldx, M, K, R, parts, Rows{unit_id, unit}}, runs, slots, stream);
   AQL_CHECK_LAUNCH("aql_adapter_down");

@@ -13,6 +13,7 @@
 
 #include <cstdlib>
 #include <memory>
+#include <mutex>
 #include <optional>
 #include <string>
 #include <unordered_map>
@@ -84,6 +85,23 @@ Rows gemm_rows(const Tensor& t) {
   return r;
 }
 
+Tensor leaf(const Tensor& t) { return t.defined() && t.is_leaf() && t.requires_grad() ? t : Tensor(); }
+
+// A leaf's accumulation node runs on the stream on which it was made.  A captured backward pass that reaches one made on another stream (an eager graph of
+// the same leaf still lives) would draw that stream into the capture, which ends the process: refused instead.
+void leaves_ok(const std::vector<Tensor>& leaves, const Tensor& g, const char* name) {
+  const auto here = c10::hip::getCurrentHIPStream(g.get_device());
+  hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(here.stream(), &cs) != hipSuccess || cs == hipStreamCaptureStatusNone) return;
+  for (const Tensor& t : leaves) {
+    if (!t.defined()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (node && node->stream() && node->stream()->id() != here.id())   // (of one device: here() has seen to that)
+      throw AqlErr(std::string(name) + ": this backward pass is being captured, but a graph of the same parameters that was made on another stream still lives; drop it "
+                   "(its outputs and losses) before the capture");
+  }
+}
+
 // gradients of a backward pass under create_graph: they carry a node that refuses a second backward pass
 variable_list once(variable_list grads, const char* name) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -121,8 +139,14 @@ std::pair<Tensor, Tensor> act8_pack(const Tensor& x) {
 }
 
 Tensor act8_unpack(const Tensor& codes, const Tensor& exps, std::vector<int64_t> shape, bool bf16) {
+  const long C = shape.empty() ? 0 : shape.back(), Cp = (C + 31) / 32 * 32;
+  int64_t M = 1;
+  for (size_t i = 0; i + 1 < shape.size(); ++i) M *= shape[i];
+  const auto fits = [&](const Tensor& t, long w) { return t.scalar_type() == at::kByte && t.dim() == 2 && t.size(0) == M && t.size(1) == w && t.is_contiguous(); };
+  if (C < 1 || !fits(codes, Cp) || !fits(exps, Cp / 32) || codes.device() != exps.device())
+    bad_value("Act8.unpack: codes uint8 [" + std::to_string(M) + ", " + std::to_string(Cp) + "] and exps uint8 [" + std::to_string(M) + ", " +
+              std::to_string(Cp / 32) + "], contiguous on one device, not " + shape_of(codes) + " and " + shape_of(exps));
   here(codes, "Act8.unpack");
-  const long C = shape.back();
   Tensor out = at::empty(shape, codes.options().dtype(bf16 ? at::kBFloat16 : at::kFloat));
   const auto st = stream_of(codes);
   ran(aql_act8_unpack(ptr<uint8_t>(codes), ptr<uint8_t>(exps), codes.size(0), (int)C, out.data_ptr(), bf16 ? 0 : 1, C, st), "aql_act8_unpack", st);
@@ -142,6 +166,7 @@ struct LayerNormTrain : torch::autograd::Function<LayerNormTrain> {
                                 ptr<float>(stats), ptr<uint8_t>(codes), ptr<uint8_t>(exps), st), "aql_layernorm_train_fwd", st);
     ctx->save_for_backward({ckpt8 ? Tensor() : r.t, codes, exps, gamma, stats});
     ctx->saved_data["beta"] = beta.defined();
+    ctx->saved_data["leaves"] = std::vector<Tensor>{leaf(x), leaf(gamma), leaf(beta)};
     if (passthrough) return {y, x.view_as(x)};
     return {y};
   }
@@ -155,6 +180,7 @@ struct LayerNormTrain : torch::autograd::Function<LayerNormTrain> {
       return {g.size() > 1 ? g[1] : z, z, z, z, z, z};
     }
     here(g[0], "layernorm_train backward");
+    leaves_ok(ctx->saved_data["leaves"].toTensorVector(), g[0], "layernorm_train");
     Tensor dx, dg, db;
     {
       at::AutoGradMode off(false);
@@ -218,6 +244,7 @@ struct Plan {   // the device side of adapters.RequestPlan
   bool equal = false;
   std::vector<long> at;      // offsets of unit_id, perm, used_pos, slot in the table
   std::unordered_map<long, int> slots_by_unit;
+  std::mutex guard;          // of slots_by_unit: backward passes ask from the engine's threads
 
   const int* part(int k) const { return (const int*)table.data_ptr() + at[k]; }
   long unit(long rows) const {   // rows per table unit for a call on `rows` rows
@@ -233,6 +260,7 @@ struct Plan {   // the device side of adapters.RequestPlan
     return std::max(1L, rows / requests);
   }
   int slots(long unit) {   // the most segments, and so adapters, that meet in 16 rows [16 i, 16 i + 16)
+    const std::lock_guard<std::mutex> lock(guard);
     auto it = slots_by_unit.find(unit);
     if (it != slots_by_unit.end()) return it->second;
     int most = 0, count = 0;
@@ -252,6 +280,7 @@ struct Call : torch::CustomClassHolder {   // what a backward pass of adapter_li
   std::shared_ptr<Bank> bank;
   std::shared_ptr<Plan> plan;
   Tensor w, wt, bias;
+  std::vector<Tensor> leaves;
   long unit = 1, serial = 0, M = 0, N = 0, K = 0;
   bool train = false, residual = false;
 };
@@ -296,13 +325,14 @@ void wgrad(const Tensor& dT, const Rows& x, const Tensor& codes, const Tensor& e
 
 struct AdapterLinear : torch::autograd::Function<AdapterLinear> {
   // ckpt8: the backward pass keeps X in 8 bits -- T is computed again from the codes, and dA and dB see their values in the place of X
-  static Tensor forward(AutogradContext* ctx, const Tensor& x2d, const Tensor& /*down*/, const Tensor& /*up*/, const std::optional<Tensor>& residual,
+  static Tensor forward(AutogradContext* ctx, const Tensor& x2d, const Tensor& down, const Tensor& up, const std::optional<Tensor>& residual,
                         c10::intrusive_ptr<Call> c, bool ckpt8, bool train) {
     Rows x = gemm_rows(x2d), res;
     if ((c->residual = residual.has_value())) res = gemm_rows(*residual);
     auto [y, T] = product(x, c->w, c->bias, res, c->bank->a, c->bank->b, *c->bank, *c->plan, c->unit, c->N, c->K, train && !ckpt8 ? 3 : 1);
     Tensor codes, exps, keep = x.t;
     c->train = train;
+    c->leaves = {leaf(x2d), leaf(down), leaf(up), residual ? leaf(*residual) : Tensor()};
     if (!train) {
       keep = T = Tensor();
     } else if (ckpt8) {
@@ -323,6 +353,7 @@ struct AdapterLinear : torch::autograd::Function<AdapterLinear> {
     variable_list out(7);
     if (!g[0].defined()) return out;
     here(g[0], "adapter_linear backward");
+    leaves_ok(c->leaves, g[0], "adapter_linear");
     if (bank.serial != c->serial) throw AqlErr("adapter_linear: the bank's weights changed between the forward pass and its backward pass");
     {
       at::AutoGradMode off(false);
@@ -390,6 +421,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     }
   });
   m.def("abi_version", [] { return aql_abi_version(); });
+  m.def("abi_address", [] { return (uintptr_t)&aql_abi_version; });   // which kernel library this is bound to
   m.def("act8_pack", &act8_pack);
   m.def("act8_unpack", &act8_unpack);
   m.def("layernorm_train", &layernorm_train);

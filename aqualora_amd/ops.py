@@ -2071,8 +2071,10 @@ def adapter_linear(x2d, packed, bank, plan, residual=None, ckpt8=False):
     ``plan``: adapters.RequestPlan whose requests make up the M rows.  Differentiable in x2d, residual and a trainable bank's down / up;
     ``ckpt8`` keeps x2d in 8 bits for the latter: T is computed again from the codes, and dA and dB see their values in the place of X."""
     _plain(x2d, "adapter_linear")
+    if residual is not None:
+        _plain(residual, "adapter_linear")
     bank.refresh()
-    if x2d.requires_grad and not bank.trainable:
+    if x2d.requires_grad and not bank.trainable and torch.is_grad_enabled():
         bank.lay_out_transposed()
     return L.native().adapter_linear(x2d, packed.w, packed.wt, packed.bias, bank.handle, plan.handle, bank.down, bank.up, residual, ckpt8)
 

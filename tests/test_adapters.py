@@ -3,6 +3,12 @@
 Tolerances.  u = 2^-24.  A dot product of n terms in fp32, in whatever order, is off by at most n u sum|terms|.  T (and dT) enters the product with
 B (A) as bf16: half a step, 2^-8 relative.  The output is rounded to bf16 once: 2^-8 of its value.  dA and dB are fp32 sums of products with
 T (dT) split into three bf16 parts that hold 24 bits (u relative)."""
+import os
+import shutil
+import subprocess
+import sys
+import threading
+
 import pytest
 import torch
 
@@ -330,6 +336,95 @@ def test_gradient_formula_against_differences():
         assert abs(num - (grad * v).sum()) <= 1e-10 * (grad.abs() * v.abs()).sum()
 
 
+@gpu
+def test_two_threads_with_one_bank_and_one_plan():
+    """Calls with different row counts on threads and streams of their own, against the same calls one after the other."""
+    d, lengths, rows, ids, equal = make("equal_77", 6)
+    packed, bank, plan = handles(d, lengths, ids, equal, True)
+    n = plan.requests
+    xs = [torch.randn(n * k, d["x"].shape[1], generator=torch.Generator().manual_seed(k)).to(DEV, torch.bfloat16) for k in (1, 3, 7, 20)]
+
+    def step(x):
+        x = x.detach().requires_grad_(True)
+        y = ops.adapter_linear(x, packed, bank, plan)
+        return (y.detach(),) + torch.autograd.grad(y, (x, bank.down, bank.up), torch.ones_like(y))
+    fresh = adapters.RequestPlan(plan.adapters)
+    want = [step(x) for x in xs]
+    plan = fresh
+    got, errors = [None] * len(xs), []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    got[i] = step(xs[i])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(xs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for a, b in zip(want, got):
+        assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+@gpu
+def test_frozen_bank_captures_without_gradients():
+    """An input that asks for a gradient is no reason to lay out the transposed stacks where gradients are off."""
+    d, lengths, rows, ids, equal = make("ragged", 7)
+    packed, bank, plan = handles(d, lengths, ids, equal, False)
+    x = d["x"].to(DEV).requires_grad_(True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad():
+        want = ops.adapter_linear(x, packed, bank, plan)
+        with torch.cuda.graph(graph):
+            y = ops.adapter_linear(x, packed, bank, plan)
+    for _ in range(2):
+        y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+
+
+@gpu
+def test_captured_backward_next_to_a_live_eager_graph_is_refused():
+    d, lengths, rows, ids, equal = make("ragged", 8)
+    packed, bank, plan = handles(d, lengths, ids, equal, True)
+    x, dy = d["x"].to(DEV), d["dy"].to(DEV)
+    step = lambda: torch.autograd.grad(ops.adapter_linear(x, packed, bank, plan), (bank.down, bank.up), dy)  # noqa: E731
+    want = step()
+    alive = ops.adapter_linear(x, packed, bank, plan)
+    with pytest.raises(RuntimeError, match="still lives"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            step()
+    torch.cuda.synchronize()
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_the_binding_uses_the_library_that_is_loaded(tmp_path):
+    """AQL_LIB selects the kernel library for the operators bound in C++ as well."""
+    other = tmp_path / "other.so"
+    shutil.copy(_lib.LIB_PATH, other)
+    code = ("import torch\nfrom aqualora_amd import _lib\n_lib.native()\n"
+            "maps = {l.split()[-1] for l in open('/proc/self/maps') if l.strip().endswith('.so')}\n"
+            "print(sorted(m for m in maps if m.endswith('other.so') or m.endswith('libaqualora_hip.so')))")
+    out = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, AQL_LIB=str(other)), cwd=os.path.dirname(os.path.dirname(_lib.__file__)),
+                         capture_output=True, text=True)
+    assert out.returncode == 0, out.stderr
+    assert out.stdout.strip() == str([str(other)])
+
+
 def test_refusals_without_a_gpu():
     with pytest.raises(_lib.AqlError):
         adapters.RequestPlan([0], device="cpu")
@@ -345,6 +440,8 @@ def test_refusals_without_a_gpu():
     assert linear(M=0) == 0
     assert lib.aql_adapter_down(p, 64, p, p, 64, 64, p, p, p, 8, p, 1, 1, 2, p, 3, None) != 0       # both sources
     assert lib.aql_adapter_down(None, 0, None, None, 64, 64, p, p, p, 8, p, 1, 1, 2, p, 3, None) != 0
+    assert lib.aql_adapter_down(p, 1 << 21, None, None, 64, 64, p, p, p, 8, p, 1, 1, 2, p, 3, None) != 0     # past the copies' 32-bit offsets
+    assert lib.aql_adapter_down(None, 0, p, p, 64, 1 << 21, p, p, p, 8, p, 1, 1, 2, p, 3, None) != 0
     need = lib.aql_adapter_wgrad_scratch_floats(64, 2, 64, 64, 8)
     assert need > 0 and lib.aql_adapter_wgrad_scratch_floats(1 << 30, 60000, 1 << 14, 1 << 14, 1024) == -1
     assert 0 < lib.aql_adapter_wgrad_scratch_floats(64, 2, 64, 0, 8) < need

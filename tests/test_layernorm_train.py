@@ -266,6 +266,38 @@ def test_refusals():
             ops.act8_pack(x)
 
 
+def test_act8_of_parts_that_do_not_fit_is_refused():
+    codes, exps, f = torch.zeros(6, 64, dtype=torch.uint8), torch.zeros(6, 2, dtype=torch.uint8), torch.float32
+    for c, e, shape in ((codes[:5], exps, (6, 64)), (codes, exps[:, :1], (6, 64)), (codes, exps, (6, 65)), (codes, exps, (7, 64)), (codes, exps, (2, 4, 64)),
+                        (codes.float(), exps, (6, 64)), (codes.t().contiguous().t(), exps, (6, 64)), (codes[0], exps[0], (64,)), (codes, exps, ()), (codes, exps, (6, 0))):
+        with pytest.raises(ValueError):
+            ops.Act8(c, e, shape, f).unpack()
+    with pytest.raises(_lib.AqlError):
+        ops.Act8(codes, exps, (2, 3, 40), f).unpack()      # all fits: only the GPU is missing
+
+
+@gpu
+def test_captured_backward_next_to_a_live_eager_graph_is_refused():
+    gen = torch.Generator().manual_seed(21)
+    x, dy = torch.randn(40, 320, generator=gen).to("cuda"), torch.randn(40, 320, generator=gen).to("cuda")
+    gamma = torch.ones(320, device="cuda", requires_grad=True)
+    step = lambda: torch.autograd.grad(ops.layernorm_train(x, gamma, None), (gamma,), dy)  # noqa: E731
+    want = step()
+    alive = ops.layernorm_train(x, gamma, None)
+    with pytest.raises(RuntimeError, match="still lives"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            step()
+    torch.cuda.synchronize()
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(want[0], got[0])
+
+
 def test_c_entries_refuse_bad_arguments():
     lib = _lib.load()
     p = _lib.c_p(4096)     # never dereferenced: every call below is refused on the host

@@ -9,5 +9,5 @@ name=$1; src=$2; shift 2
 mkdir -p ../../altlib
 hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function $contract -munsafe-fp-atomics -Xclang -target-feature -Xclang -packed-fp32-ops "$@" -c $src -o ../../altlib/${name}_${src%.hip}.o
 objs=$(ls aql_*.o | grep -v "^${src%.hip}.o$")
-hipcc --offload-arch=gfx950 -shared -fPIC $objs ../../altlib/${name}_${src%.hip}.o -ldl -o ../../altlib/${name}.so
+hipcc --offload-arch=gfx950 -shared -fPIC -Wl,-soname,libaqualora_hip.so $objs ../../altlib/${name}_${src%.hip}.o -ldl -o ../../altlib/${name}.so
 echo built altlib/${name}.so

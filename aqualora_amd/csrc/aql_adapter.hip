@@ -242,17 +242,26 @@ __global__ __launch_bounds__(512) void skinny_kernel(const LinArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------------------- many rows: LDS tiles
-__device__ __forceinline__ int lds_off(int row, int chunk) { return row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4); }   // conflict-free fragment reads
+// Rows of 128 bytes; the chunks of a row are exchanged by a number made of its bits so that the 16 rows of a fragment, neighbours or as pair_row takes
+// them, fall on different banks
+__device__ __forceinline__ int lds_mix(int row) { return ((row >> 1) & 1) | ((row >> 2) & 2) | (((row >> 2) ^ (row >> 4)) & 1) << 2; }
+__device__ __forceinline__ int lds_off(int row, int chunk) { return row * 128 + ((chunk ^ lds_mix(row)) << 4); }
+// the row of W that fragment j, lane row i, of FN fragments reads: two neighbouring fragments together cover 32 columns such that a lane ends with eight
+// consecutive ones of its row (4 of each) and moves them 16 bytes at a time; the last of an odd number is read as it is
+template <int FN>
+__device__ __forceinline__ int pair_row(int j, int i) {
+  return j + 1 == FN && FN % 2 ? j * 16 + i : (j >> 1) * 32 + (i >> 2) * 8 + (j & 1) * 4 + (i & 3);
+}
 
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, char* dst, uint32_t voff, uint32_t soff) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)dst, 16, voff, soff, 0, 0);
 }
 
-// rows x 64 columns of one operand, global -> LDS, by NW wavefronts; lane (row = tid >> 3, slot = tid & 7) fetches source chunk slot ^ ((row >> 1) & 7)
+// rows x 64 columns of one operand, global -> LDS, by NW wavefronts; lane (row = tid >> 3, slot = tid & 7) fetches source chunk slot ^ lds_mix(row)
 template <int ROWS, int NW>
 struct Stage {
   static constexpr int RPI = 8 * NW, NL = ROWS / RPI;
-  static_assert(ROWS % RPI == 0 && RPI % 16 == 0, "whole copies");
+  static_assert(ROWS % RPI == 0 && RPI % 32 == 0, "whole copies, of rows with the same lds_mix");
   __amdgpu_buffer_rsrc_t rs;
   uint32_t voff[NL], soff;
   int krem, kc;
@@ -260,7 +269,7 @@ struct Stage {
   template <class L>
   __device__ __forceinline__ void begin(const bf16_t* base, long ld, int K, int tid, L live) {
     rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t*>(base), 0, 0x40000000, 0x00020000);
-    kc = ((tid & 7) ^ ((tid >> 4) & 7)) * 8;
+    kc = ((tid & 7) ^ lds_mix(tid >> 3)) * 8;
 #pragma unroll
     for (int l = 0; l < NL; ++l) {
       const int r = (tid >> 3) + RPI * l;
@@ -279,9 +288,9 @@ struct Stage {
 };
 
 // acc += the product of NK stages of 64 columns: NSTG LDS stages, NSTG - 1 in flight, one barrier per stage.  The weight-side fragment is MFMA operand A,
-// so a lane ends with four consecutive columns (4 q + e) of one row (lane & 15).  issue(st) starts the next stage's copies (NLD per wavefront,
+// so a lane ends with four consecutive columns (4 q + e; PAIRS: see pair_row) of one row (lane & 15).  issue(st) starts the next stage's copies (NLD per wavefront,
 // always: past the end they are out of range and fill zeros, so the count of copies still allowed in flight is a constant).
-template <int BM, int BN, int WGM, int WGN, int NSTG, class I>
+template <int BM, int BN, int WGM, int WGN, int NSTG, bool PAIRS, class I>
 __device__ __forceinline__ void ring(char* lds, int nk, int tid, f32x4_t (&acc)[BM / WGM / 16][BN / WGN / 16], I issue) {
   constexpr int NW = WGM * WGN, WM = BM / WGM, WN = BN / WGN, FM = WM / 16, FN = WN / 16;
   constexpr int STAGE = (BM + BN) * 128, NLD = (BM + BN) / (8 * NW);
@@ -299,7 +308,7 @@ __device__ __forceinline__ void ring(char* lds, int nk, int tid, f32x4_t (&acc)[
       bf16x8_t fa[FM], fb[FN];
       const int chunk = ks * 4 + q;
 #pragma unroll
-      for (int j = 0; j < FN; ++j) fb[j] = *reinterpret_cast<const bf16x8_t*>(pb + lds_off(wn0 + j * 16 + i16, chunk));
+      for (int j = 0; j < FN; ++j) fb[j] = *reinterpret_cast<const bf16x8_t*>(pb + lds_off(wn0 + (PAIRS ? pair_row<FN>(j, i16) : j * 16 + i16), chunk));
 #pragma unroll
       for (int i = 0; i < FM; ++i) fa[i] = *reinterpret_cast<const bf16x8_t*>(pa + lds_off(wm0 + i * 16 + i16, chunk));
 #pragma unroll
@@ -353,22 +362,33 @@ __global__ __launch_bounds__(WGM * WGN * 64) void tile_kernel(const LinArgs a) {
   const int v0 = n0 + (wave % WGN) * WN;
   // the fp32 sums begin with bias and residual: their loads run under the first copies instead of behind the last product, and there is one rounding
   f32x4_t acc[FM][FN];
+  constexpr int FP = FN / 2, FO = FN % 2;   // pairs of fragments, and a last one
+  const auto low = [](uint4 b) { return f32x4_t{bf16lo(b.x), bf16hi(b.x), bf16lo(b.y), bf16hi(b.y)}; };
+  const auto high = [](uint4 b) { return f32x4_t{bf16lo(b.z), bf16hi(b.z), bf16lo(b.w), bf16hi(b.w)}; };
+  // eight columns of pair p, four of the last fragment; past the end: the last columns, never stored
+  const auto load = [&](const bf16_t* row, int j) {
+    if (j < 2 * FP) return *reinterpret_cast<const uint4*>(row + min(v0 + j * 16 + q * 8, a.N - 8));
+    const uint2 v = *reinterpret_cast<const uint2*>(row + min(v0 + j * 16 + q * 4, a.N - 4));
+    return make_uint4(v.x, v.y, 0u, 0u);
+  };
 #pragma unroll
-  for (int j = 0; j < FN; ++j) {
-    const int n = min(v0 + j * 16 + q * 4, a.N - 4);   // (past the end: the last, never stored)
-    const uint2 b = a.bias ? *reinterpret_cast<const uint2*>(a.bias + n) : make_uint2(0u, 0u);
-    const f32x4_t bv = {bf16lo(b.x), bf16hi(b.x), bf16lo(b.y), bf16hi(b.y)};
+  for (int j = 0; j < FN; j += 2) {
+    const uint4 b = a.bias ? load(a.bias, j) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-    for (int i = 0; i < FM; ++i) acc[i][j] = bv;
+    for (int i = 0; i < FM; ++i) {
+      acc[i][j] = low(b);
+      if (j < 2 * FP) acc[i][j + 1 < FN ? j + 1 : j] = high(b);
+    }
   }
   if (a.res) {
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const bf16_t* p = a.res + min(w0 + i * 16 + i16, a.M - 1) * a.ldr;
 #pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        const uint2 r = *reinterpret_cast<const uint2*>(p + min(v0 + j * 16 + q * 4, a.N - 4));
-        acc[i][j] += f32x4_t{bf16lo(r.x), bf16hi(r.x), bf16lo(r.y), bf16hi(r.y)};
+      for (int j = 0; j < FN; j += 2) {
+        const uint4 r = load(p, j);
+        acc[i][j] += low(r);
+        if (j < 2 * FP) acc[i][j + 1 < FN ? j + 1 : j] += high(r);
       }
     }
   }
@@ -399,16 +419,22 @@ __global__ __launch_bounds__(WGM * WGN * 64) void tile_kernel(const LinArgs a) {
   for (int u = 0; u < NSTG - 1; ++u) issue(u);
   if (a.rows.id != nullptr)
     for (int h = next_adapter<BM>(ids, -1, lane); h >= 0; h = next_adapter<BM>(ids, h, lane)) nk += rk;
-  ring<BM, BN, WGM, WGN, NSTG>(lds, nk, tid, acc, issue);
+  ring<BM, BN, WGM, WGN, NSTG, true>(lds, nk, tid, acc, issue);
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
     const long m = w0 + i * 16 + i16;
     if (m >= a.M) continue;
 #pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const int n = v0 + j * 16 + q * 4;
+    for (int p = 0; p < FP; ++p) {
+      const int n = v0 + p * 32 + q * 8;
       if (n >= a.N) continue;
-      const f32x4_t v = acc[i][j];
+      const f32x4_t v = acc[i][2 * p], w = acc[i][2 * p + 1];
+      *reinterpret_cast<uint4*>(a.Y + m * a.ldy + n) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3]));
+    }
+    if constexpr (FO) {
+      const int n = v0 + FP * 32 + q * 4;
+      if (n >= a.N) continue;
+      const f32x4_t v = acc[i][FN - 1];
       *reinterpret_cast<uint2*>(a.Y + m * a.ldy + n) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
     }
   }
@@ -445,7 +471,7 @@ __global__ __launch_bounds__(256) void down_tile_kernel(const DownArgs a) {
     };
 #pragma unroll
     for (int u = 0; u < NSTG - 1; ++u) issue(u);
-    ring<BM, BN, 2, 2, NSTG>(lds, (a.K + BK - 1) / BK, tid, acc, issue);
+    ring<BM, BN, 2, 2, NSTG, false>(lds, (a.K + BK - 1) / BK, tid, acc, issue);
     const float sc = a.scales[g];
     const int rank = a.ranks[g];
 #pragma unroll

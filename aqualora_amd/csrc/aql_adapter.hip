@@ -54,6 +54,20 @@ __device__ __forceinline__ void store_t4(bf16_t* t, int R, int P, const float (&
     r[0] -= bf16lo(w.x), r[1] -= bf16hi(w.x), r[2] -= bf16lo(w.y), r[3] -= bf16hi(w.y);   // exact
   }
 }
+__device__ __forceinline__ void store_t8(bf16_t* t, int R, int P, const float (&v)[8]) {   // eight
+  float r[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = v[e];
+  for (int p = 0; p < P; ++p) {
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      w[k] = pack_bf16x2(r[2 * k], r[2 * k + 1]);
+      r[2 * k] -= bf16lo(w[k]), r[2 * k + 1] -= bf16hi(w[k]);
+    }
+    *reinterpret_cast<uint4*>(t + p * R) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
 __device__ __forceinline__ f32x4_t mfma(bf16x8_t a, bf16x8_t b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
 // ---------------------------------------------------------------------------------------------------------------------- T = s A x
@@ -411,12 +425,22 @@ __global__ __launch_bounds__(WGM * WGN * 64) void tile_kernel(const LinArgs a) {
     sx.fetch(lds + st * STAGE, wave);
     sw.fetch(lds + st * STAGE + BM * 128, wave);
   };
+  // the first copies leave before the row -> adapter loads come back, where the projection's own columns are enough for them
+  const bool early = nk >= NSTG - 1;
+  if (early) {
+#pragma unroll
+    for (int u = 0; u < NSTG - 1; ++u) issue(u);
+  }
   if (a.rows.id != nullptr) {
     for (int r = tid; r < BM; r += NW * 64) ids[r] = r < mlive ? id_of(a.rows, m0 + r) : -1;
-    __syncthreads();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
   }
+  if (!early) {
 #pragma unroll
-  for (int u = 0; u < NSTG - 1; ++u) issue(u);
+    for (int u = 0; u < NSTG - 1; ++u) issue(u);
+  }
   if (a.rows.id != nullptr)
     for (int h = next_adapter<BM>(ids, -1, lane); h >= 0; h = next_adapter<BM>(ids, h, lane)) nk += rk;
   ring<BM, BN, WGM, WGN, NSTG, true>(lds, nk, tid, acc, issue);
@@ -440,6 +464,34 @@ __global__ __launch_bounds__(WGM * WGN * 64) void tile_kernel(const LinArgs a) {
   }
 }
 
+// a tile's sums -> T, the rows of adapter g.  mr0, r0: the wavefront's first row in the tile, its first column
+template <int FM, int FN>
+__device__ __forceinline__ void store_tile(const DownArgs& a, const f32x4_t (&acc)[FM][FN], const int* ids, int g, float sc, int rank, long m0, int mr0, int r0, int lane) {
+  const int i16 = lane & 15, q = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int mr = mr0 + i * 16 + i16;
+    bf16_t* row = a.T + (m0 + mr) * a.P * a.R;
+    if (ids[mr] != g) continue;
+    if constexpr (FN == 1) {
+      const int r = r0 + q * 4;
+      float o[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = r + e < rank ? sc * acc[i][0][e] : 0.f;
+      if (r < a.R) store_t4(row + r, a.R, a.P, o);
+    } else {
+#pragma unroll
+      for (int j = 0; j < FN; j += 2) {
+        const int r = r0 + j * 16 + q * 8;
+        float o[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = r + e < rank ? sc * acc[i][j + e / 4][e % 4] : 0.f;
+        if (r < a.R) store_t8(row + r, a.R, a.P, o);
+      }
+    }
+  }
+}
+
 // T = s A x for many rows of long requests: 64 rows x BN adapter rows per workgroup, once for each adapter that the rows meet (mostly one)
 template <int BN, int NSTG>
 __global__ __launch_bounds__(256) void down_tile_kernel(const DownArgs a) {
@@ -456,6 +508,8 @@ __global__ __launch_bounds__(256) void down_tile_kernel(const DownArgs a) {
   int turn = 0;   // where the rows meet several adapters, blockIdx.y = 0 and 1 take them in turn
   for (int g = next_adapter<BM>(ids, -1, lane); g >= 0; g = next_adapter<BM>(ids, g, lane), ++turn) {
     if ((turn & 1) != (int)blockIdx.y) continue;
+    const float sc = a.scales[g];   // (here: behind the product their latency would show)
+    const int rank = a.ranks[g];
     f32x4_t acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
@@ -471,23 +525,8 @@ __global__ __launch_bounds__(256) void down_tile_kernel(const DownArgs a) {
     };
 #pragma unroll
     for (int u = 0; u < NSTG - 1; ++u) issue(u);
-    ring<BM, BN, 2, 2, NSTG, false>(lds, (a.K + BK - 1) / BK, tid, acc, issue);
-    const float sc = a.scales[g];
-    const int rank = a.ranks[g];
-#pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      const int mr = (wave >> 1) * 32 + i * 16 + i16;
-      const long m = m0 + mr;
-      const int gm = ids[mr];
-#pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        const int r = r0 + (wave & 1) * (BN / 2) + j * 16 + q * 4;
-        float o[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = r + e < rank ? sc * acc[i][j][e] : 0.f;
-        if (gm == g && r < a.R) store_t4(a.T + m * a.P * a.R + r, a.R, a.P, o);
-      }
-    }
+    ring<BM, BN, 2, 2, NSTG, FN % 2 == 0>(lds, (a.K + BK - 1) / BK, tid, acc, issue);
+    store_tile(a, acc, ids, g, sc, rank, m0, (wave >> 1) * 32, r0 + (wave & 1) * (BN / 2), lane);
     __syncthreads();   // the stages are free for the next adapter
   }
 }
@@ -513,6 +552,8 @@ __global__ __launch_bounds__(256) void down8_tile_kernel(const DownArgs a) {
   int turn = 0;
   for (int g = next_adapter<BM>(ids, -1, lane); g >= 0; g = next_adapter<BM>(ids, g, lane), ++turn) {
     if ((turn & 1) != (int)blockIdx.y) continue;
+    const float sc = a.scales[g];   // (here: behind the product their latency would show)
+    const int rank = a.ranks[g];
     f32x4_t acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
@@ -558,7 +599,7 @@ __global__ __launch_bounds__(256) void down8_tile_kernel(const DownArgs a) {
       for (int ks = 0; ks < 2; ++ks) {
         bf16x8_t fa[FM], fb[FN];
 #pragma unroll
-        for (int j = 0; j < FN; ++j) fb[j] = *reinterpret_cast<const bf16x8_t*>(pb + lds_off((wave & 1) * (BN / 2) + j * 16 + i16, ks * 4 + q));
+        for (int j = 0; j < FN; ++j) fb[j] = *reinterpret_cast<const bf16x8_t*>(pb + lds_off((wave & 1) * (BN / 2) + pair_row<FN>(j, i16), ks * 4 + q));
 #pragma unroll
         for (int i = 0; i < FM; ++i) fa[i] = *reinterpret_cast<const bf16x8_t*>(pa + lds_off((wave >> 1) * 32 + i * 16 + i16, ks * 4 + q));
 #pragma unroll
@@ -569,20 +610,7 @@ __global__ __launch_bounds__(256) void down8_tile_kernel(const DownArgs a) {
       rd = nx;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    const float sc = a.scales[g];
-    const int rank = a.ranks[g];
-#pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      const int mr = (wave >> 1) * 32 + i * 16 + i16;
-#pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        const int r = r0 + (wave & 1) * (BN / 2) + j * 16 + q * 4;
-        float o[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = r + e < rank ? sc * acc[i][j][e] : 0.f;
-        if (ids[mr] == g && r < a.R) store_t4(a.T + (m0 + mr) * a.P * a.R + r, a.R, a.P, o);
-      }
-    }
+    store_tile(a, acc, ids, g, sc, rank, m0, (wave >> 1) * 32, r0 + (wave & 1) * (BN / 2), lane);
     __syncthreads();   // the stages are free for the next adapter
   }
 }

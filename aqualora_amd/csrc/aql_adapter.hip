@@ -531,11 +531,11 @@ __global__ __launch_bounds__(256) void down_tile_kernel(const DownArgs a) {
   }
 }
 
-// The same from 8-bit codes: a thread turns 16 codes of a row into bf16 on their way into LDS (exact), one stage ahead of the product, with the next
-// stage's codes on their way from memory; A comes by copies as above.
+// The same from 8-bit codes: a thread turns 16 codes of a row into bf16 on their way into LDS (exact), one stage ahead of the product, with the codes of
+// the three stages behind it on their way from memory (9001 x 1280, rank 64: 12.9 us, with one stage 18.6); A comes by copies as above.
 template <int BN>
 __global__ __launch_bounds__(256) void down8_tile_kernel(const DownArgs a) {
-  constexpr int BM = 64, FM = 2, FN = BN / 32, NSTG = 3, STAGE = (BM + BN) * 128;
+  constexpr int BM = 64, FM = 2, FN = BN / 32, NSTG = 4, STAGE = (BM + BN) * 128;
   __shared__ __attribute__((aligned(16))) char lds[NSTG * STAGE + BM * 4];   // (one array: see tile_kernel)
   int* ids = reinterpret_cast<int*>(lds + NSTG * STAGE);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = lane & 15, q = lane >> 4;
@@ -561,40 +561,48 @@ __global__ __launch_bounds__(256) void down8_tile_kernel(const DownArgs a) {
       for (int j = 0; j < FN; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     Stage<BN, 4> sa;
     sa.begin(a.A + ((long)g * a.R + r0) * a.K, a.K, a.K, tid, [&](int r) { return r < rlive; });
-    uint4 code;
-    uint32_t ex;
-    auto load = [&](int t) {   // past the row's last block: the first again, the row of A is zero there
+    uint4 code[NSTG];          // of stage t at t % 4, like the LDS stages
+    uint32_t ex[NSTG];
+    // (the fences keep copies and loads in this order: the wait below counts them)
+    auto load = [&](int t, int u) {   // past the row's last block: the first again
       const int k = t * BK + xc, kk = k < nb * 32 ? k : 0;
-      code = *reinterpret_cast<const uint4*>(cr + kk);
-      ex = er[kk >> 5];
-      ex = k < nb * 32 ? ex : 1u;
+      code[u] = *reinterpret_cast<const uint4*>(cr + kk);
+      ex[u] = er[kk >> 5];
+      asm volatile("" ::: "memory");
     };
-    auto put = [&](int st) {
-      const float sp = act8::step(ex);
+    auto fetch = [&](int u) {
+      sa.fetch(lds + u * STAGE + BM * 128, wave);
+      asm volatile("" ::: "memory");
+    };
+    auto put = [&](int t, int u) {
+      // (the values are first used here, not ahead of the barriers, where the compiler would wait for all of them together)
+      asm volatile("" : "+v"(code[u].x), "+v"(code[u].y), "+v"(code[u].z), "+v"(code[u].w), "+v"(ex[u]));
+      // past the last block A is zero: any finite step (chosen here: with the load it would wait for it)
+      const float sp = act8::step(t * BK + xc < nb * 32 ? ex[u] : 1u);
       float v[8];
-      act8::values4(code.x, sp, v);
-      act8::values4(code.y, sp, v + 4);
-      *reinterpret_cast<bf16x8_t*>(lds + st * STAGE + lds_off(xr, xc >> 3)) = pack8(v);
-      act8::values4(code.z, sp, v);
-      act8::values4(code.w, sp, v + 4);
-      *reinterpret_cast<bf16x8_t*>(lds + st * STAGE + lds_off(xr, (xc >> 3) + 1)) = pack8(v);
+      act8::values4(code[u].x, sp, v);
+      act8::values4(code[u].y, sp, v + 4);
+      *reinterpret_cast<bf16x8_t*>(lds + u * STAGE + lds_off(xr, xc >> 3)) = pack8(v);
+      act8::values4(code[u].z, sp, v);
+      act8::values4(code[u].w, sp, v + 4);
+      *reinterpret_cast<bf16x8_t*>(lds + u * STAGE + lds_off(xr, (xc >> 3) + 1)) = pack8(v);
     };
-    load(0);
-    sa.fetch(lds + BM * 128, wave);
-    put(0);
-    sa.fetch(lds + STAGE + BM * 128, wave);
-    load(1);
-    int rd = 0;
-    for (int t = 0; t < nk; ++t) {
-      const int nx = rd + 1 == NSTG ? 0 : rd + 1, fr = nx + 1 == NSTG ? 0 : nx + 1;
-      // still in flight: the next stage's copies and the codes behind them.  Stage t's codes are in LDS when everybody's writes are done
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(BN / 32 + 2) : "memory");
+    load(0, 0);
+#pragma unroll
+    for (int u = 0; u < NSTG - 1; ++u) {
+      fetch(u);
+      load(u + 1, u + 1);
+    }
+    put(0, 0);
+    auto stage = [&](int t, int u) {   // u = t % 4
+      // still in flight: the copies of two stages and three stages' codes (two loads each).  Stage t's codes are in LDS when everybody's writes are done
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * (BN / 32) + 6) : "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      put(nx);
-      sa.fetch(lds + fr * STAGE + BM * 128, wave);
-      load(t + 2);
-      const char *pa = lds + rd * STAGE, *pb = pa + BM * 128;
+      put(t + 1, (u + 1) % NSTG);
+      fetch((u + 3) % NSTG);
+      load(t + 4, u);
+      const char *pa = lds + u * STAGE, *pb = pa + BM * 128;
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
         bf16x8_t fa[FM], fb[FN];
@@ -607,8 +615,15 @@ __global__ __launch_bounds__(256) void down8_tile_kernel(const DownArgs a) {
 #pragma unroll
           for (int j = 0; j < FN; ++j) acc[i][j] = mfma(fb[j], fa[i], acc[i][j]);
       }
-      rd = nx;
+    };
+    int t = 0;
+    for (; t + NSTG <= nk; t += NSTG) {   // (whole turns without a branch inside: at a branch the compiler waits for all loads)
+#pragma unroll
+      for (int u = 0; u < NSTG; ++u) stage(t + u, u);
     }
+#pragma unroll
+    for (int u = 0; u < NSTG - 1; ++u)
+      if (t + u < nk) stage(t + u, u);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     store_tile(a, acc, ids, g, sc, rank, m0, (wave >> 1) * 32, r0 + (wave & 1) * (BN / 2), lane);
     __syncthreads();   // the stages are free for the next adapter

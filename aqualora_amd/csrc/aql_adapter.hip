@@ -640,7 +640,7 @@ struct Order {
   const int* used_pos;   // [nused + 1] first position of the j-th used adapter, in units
   const int* slot;       // [nslot] j of adapter g, or -1
   int nused, nslot, unit;
-  uint32_t magic, shift; // p / unit = (p magic) >> 32 >> shift for p < 2^31 (unit > 1)
+  uint32_t magic, shift; // p / unit = (2 p magic) >> 32 >> shift for p < 2^31
   long rows;
 };
 typedef short v4s_t __attribute__((ext_vector_type(4)));
@@ -694,7 +694,7 @@ __device__ __forceinline__ void wgrad_body(const Grad& G, int R, const Order& o,
   } next;
   int mv[NV], mu[NU], qv[NV], qu[NU];   // the tile to fetch next: unit of each row, and the row in it (nothing uses a load before the fetch)
   auto unit_of = [&](long p, int& m, int& q) {
-    const uint32_t u = o.unit == 1 ? (uint32_t)p : __umulhi((uint32_t)p, o.magic) >> o.shift;
+    const uint32_t u = __umulhi((uint32_t)p << 1, o.magic) >> o.shift;
     m = o.perm[u];
     q = (int)((uint32_t)p - u * (uint32_t)o.unit);
   };
@@ -765,7 +765,7 @@ __device__ __forceinline__ void wgrad_body(const Grad& G, int R, const Order& o,
 #pragma unroll
         for (int h = 2; h >= 0; --h)
 #pragma unroll
-          for (int u = 0; u < FU; ++u) {
+          for (int u = 0; u < FU; ++u) {   // (all of U's fragments of a step read ahead spill registers: 30 against 25 us)
             const bf16x8_t fu = tr_frag<PU>(ut, s, h * RB + wu0 + u * 16, lane);
 #pragma unroll
             for (int v = 0; v < FV; ++v) acc[v][u] = TRANS ? mfma(fu, fv[v], acc[v][u]) : mfma(fv[v], fu, acc[v][u]);
@@ -957,9 +957,9 @@ extern "C" int aql_adapter_wgrad(const bf16_t* dT, const bf16_t* X, long ldx, co
   if (!dB) N = 0;
   const int need = aql_adapter_wgrad_scratch_floats(rows, nused, K, N, R);
   AQL_CHECK_ARG(need >= 0 && scratch_floats >= need && (need == 0 || scratch), "aql_adapter_wgrad: workspace of %ld floats, %d needed", scratch_floats, need);
-  uint32_t L = 1;
+  uint32_t L = 0;   // 2^L >= unit: magic = floor(2^(31 + L) / unit) + 1 < 2^32, and the quotient is exact below 2^31
   while (rows && (1L << L) < unit) ++L;
-  const Order o{perm, used_pos, slot, nused, rows ? nslot : 0, unit, rows && unit > 1 ? (uint32_t)((1UL << (31 + L)) / (uint32_t)unit + 1) : 0u, L - 1, rows};
+  const Order o{perm, used_pos, slot, nused, rows ? nslot : 0, unit, rows ? (uint32_t)((1UL << (31 + L)) / (uint32_t)unit + 1) : 0u, L, rows};
   const int rb = R <= 32 ? 32 : 64, tr = (R + rb - 1) / rb;
   const auto job = [&](const bf16_t* U, const bf16_t* V, long ldv, int C, float* part, float* out) {
     Grad g{U, V, nullptr, nullptr, ldv, C, 64, 0, part, out};

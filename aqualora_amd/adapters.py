@@ -128,10 +128,12 @@ class RequestPlan:
         n = np.ones(ids.size, dtype=np.int64) if self.equal else np.asarray([int(x) for x in lengths], dtype=np.int64)
         if n.size != ids.size or (n.size and n.min() < 0):
             raise ValueError("RequestPlan: one length of 0 or more for each request")
-        self.units = int(n.sum())
-        if self.units >= (1 << 31) - 256:
+        if int(n.sum()) >= (1 << 31) - 256:
             raise ValueError("RequestPlan: too many rows")
         ids, n = ids[n > 0], n[n > 0]
+        unit_rows = int(np.gcd.reduce(n)) if n.size else 1            # the tables count in the largest unit that divides all requests
+        n = n // unit_rows
+        self.units = int(n.sum())
         first = np.flatnonzero(np.r_[True, ids[1:] != ids[:-1]]) if ids.size else np.zeros(0, dtype=np.int64)
         begin = np.r_[0, np.cumsum(n)]
         start = np.r_[begin[first], self.units] if ids.size else np.zeros(1, dtype=np.int64)     # [n + 1], neighbours of one adapter joined
@@ -151,6 +153,7 @@ class RequestPlan:
         self.table = h.table = torch.from_numpy(flat).to(dev)
         h.at = np.r_[0, np.cumsum([p.size for p in parts.values()])[:-1]].tolist()
         h.start = start.tolist()
-        h.units, h.requests, h.live_units, h.equal, h.max_id = self.units, self.requests, int(perm.size), self.equal, self.max_id
+        h.units, h.unit_rows, h.requests, h.live_units = self.units, unit_rows, self.requests, int(perm.size)
+        h.equal, h.max_id = self.equal, self.max_id
         h.nseg = int(seg.size) if self.max_id >= 0 else 0              # no adapters at all: no segments
         h.nused, h.nslot = int(used.size), int(slot.size)

@@ -9,7 +9,8 @@
 //
 // Row m has adapter id[m / unit], -1 for none: one load, whatever the requests' lengths (a binary search over their starts cost a chain of
 // scalar loads: 15 us against 6 us where 16 requests meet in a tile of 16 rows).  Tiles of rows stay dense; the low-rank term runs once for each
-// adapter that a tile meets, with the other adapters' T rows taken as zeros (a select: what they hold cannot reach the sum).
+// adapter that a tile meets, with the other adapters' T rows taken as zeros and their sums left alone (selects: neither what those rows hold
+// nor an infinity or a NaN in this adapter's weights reaches another request).
 //
 // T is written as bf16 parts: T = hi + mid + lo, hi = T rounded to bf16, mid = the rest rounded, lo = the rest of that.  The second launch reads
 // hi alone (the one rounding of T in the linear, as in the single-adapter kernels).  The gradients dA and dB are fp32 sums of T's products
@@ -224,7 +225,9 @@ __global__ __launch_bounds__(512) void skinny_kernel(const LinArgs a) {
       for (int j = 0; j < NF; ++j) {
         const int n = n0 + j * 16 + i;
         const bf16x8_t bf = in && n < a.N ? load8(Bg + (long)n * a.R + r) : zero8();
-        acc[j] = mfma(bf, tf, acc[j]);
+        const f32x4_t v = mfma(bf, tf, acc[j]);   // the other rows keep their sums by a select: B may hold an infinity or a NaN
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[j][e] = gi == g ? v[e] : acc[j][e];
       }
     }
   }
@@ -301,45 +304,71 @@ struct Stage {
   }
 };
 
-// acc += the product of NK stages of 64 columns: NSTG LDS stages, NSTG - 1 in flight, one barrier per stage.  The weight-side fragment is MFMA operand A,
-// so a lane ends with four consecutive columns (4 q + e; PAIRS: see pair_row) of one row (lane & 15).  issue(st) starts the next stage's copies (NLD per wavefront,
+// A ring of NSTG LDS stages of 64 columns, NSTG - 1 in flight, one barrier per stage.  issue(st) starts the next stage's copies (NLD per wavefront,
 // always: past the end they are out of range and fill zeros, so the count of copies still allowed in flight is a constant).
-template <int BM, int BN, int WGM, int WGN, int NSTG, bool PAIRS, class I>
-__device__ __forceinline__ void ring(char* lds, int nk, int tid, f32x4_t (&acc)[BM / WGM / 16][BN / WGN / 16], I issue) {
-  constexpr int NW = WGM * WGN, WM = BM / WGM, WN = BN / WGN, FM = WM / 16, FN = WN / 16;
-  constexpr int STAGE = (BM + BN) * 128, NLD = (BM + BN) / (8 * NW);
-  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = lane & 15, q = lane >> 4;
-  const int wm0 = (wave / WGN) * WM, wn0 = (wave % WGN) * WN;
+template <int BM, int BN, int NW, int NSTG>
+struct Ring {
+  static constexpr int STAGE = (BM + BN) * 128, NLD = (BM + BN) / (8 * NW);
+  char* lds;
   int rd = 0, wr = NSTG - 1;
-  for (int t = 0; t < nk; ++t) {
+  template <class I>
+  __device__ __forceinline__ const char* turn(I issue) {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NSTG - 2) * NLD) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     issue(wr);
-    const char *pa = lds + rd * STAGE, *pb = pa + BM * 128;
-#pragma unroll
-    for (int ks = 0; ks < BK / 32; ++ks) {
-      bf16x8_t fa[FM], fb[FN];
-      const int chunk = ks * 4 + q;
-#pragma unroll
-      for (int j = 0; j < FN; ++j) fb[j] = *reinterpret_cast<const bf16x8_t*>(pb + lds_off(wn0 + (PAIRS ? pair_row<FN>(j, i16) : j * 16 + i16), chunk));
-#pragma unroll
-      for (int i = 0; i < FM; ++i) fa[i] = *reinterpret_cast<const bf16x8_t*>(pa + lds_off(wm0 + i * 16 + i16, chunk));
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = mfma(fb[j], fa[i], acc[i][j]);
-    }
+    const char* p = lds + rd * STAGE;
     rd = rd + 1 == NSTG ? 0 : rd + 1;
     wr = wr + 1 == NSTG ? 0 : wr + 1;
+    return p;
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the zero-filling copies still write LDS
+  __device__ __forceinline__ void drain() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }   // the zero-filling copies still write LDS
+};
+
+// acc += one stage's product.  The weight-side fragment is MFMA operand A, so a lane ends with four consecutive columns (4 q + e; PAIRS: see pair_row)
+// of one row (lane & 15).  SOME: only rows of fragments i with bit i of `own` set in their lanes take part; the others keep their sums by a select, whatever the weight
+// side holds (a zero row against an infinity or a NaN would add a NaN).
+template <int BM, int BN, int WGM, int WGN, bool PAIRS, bool SOME = false>
+__device__ __forceinline__ void products(const char* pa, int wave, int lane, f32x4_t (&acc)[BM / WGM / 16][BN / WGN / 16], uint32_t own = 0) {
+  constexpr int WM = BM / WGM, WN = BN / WGN, FM = WM / 16, FN = WN / 16;
+  if constexpr (SOME) asm volatile("" : "+v"(lane));   // (its addresses are made anew: kept beside the other loop's they would spill)
+  const int i16 = lane & 15, q = lane >> 4, wm0 = (wave / WGN) * WM, wn0 = (wave % WGN) * WN;
+  const char* pb = pa + BM * 128;
+#pragma unroll
+  for (int ks = 0; ks < BK / 32; ++ks) {
+    bf16x8_t fa[FM], fb[FN];
+    const int chunk = ks * 4 + q;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) fb[j] = *reinterpret_cast<const bf16x8_t*>(pb + lds_off(wn0 + (PAIRS ? pair_row<FN>(j, i16) : j * 16 + i16), chunk));
+#pragma unroll
+    for (int i = 0; i < FM; ++i) fa[i] = *reinterpret_cast<const bf16x8_t*>(pa + lds_off(wm0 + i * 16 + i16, chunk));
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const f32x4_t v = mfma(fb[j], fa[i], acc[i][j]);
+        if constexpr (SOME) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = own >> i & 1 ? v[e] : acc[i][j][e];
+        } else {
+          acc[i][j] = v;
+        }
+      }
+  }
 }
 
 // consecutive workgroups go to the eight XCDs in turn: XCD x takes the x-th eighth of the tiles, so that tiles that share operands share an L2
 __device__ __forceinline__ uint32_t xcd_tile(uint32_t b, uint32_t n) {
   const uint32_t x = b & 7, i = b >> 3, q = n >> 3, r = n & 7;
   return x * q + min(x, r) + i;
+}
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t row_umin(uint32_t v) { return min(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false)); }
+__device__ __forceinline__ uint32_t wave_umin(uint32_t v) {   // four rotations of 16 lanes, then the four rows: a scalar
+  v = row_umin<0x121>(row_umin<0x122>(row_umin<0x124>(row_umin<0x128>(v))));
+  const auto at = [&](int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
+  return min(min(at(0), at(16)), min(at(32), at(48)));
 }
 
 // the smallest adapter above `after` among the BM rows of a tile (ids in LDS), or -1; the same in every lane of every wavefront
@@ -351,26 +380,30 @@ __device__ __forceinline__ int next_adapter(const int* ids, int after, int lane)
     const int g = ids[k * 64 + lane];
     best = min(best, g > after ? (uint32_t)g : 0x7fffffffu);
   }
-#pragma unroll
-  for (int d = 32; d; d >>= 1) best = min(best, (uint32_t)__shfl_xor((int)best, d));
-  const int g = __builtin_amdgcn_readfirstlane((int)best);
+  best = wave_umin(best);
+  const int g = (int)best;
   return g == 0x7fffffff ? -1 : g;
 }
 
+// whether all `live` rows of a tile have adapter g
+template <int BM>
+__device__ __forceinline__ bool one_adapter(const int* ids, int g, int live, int lane) {
+  bool all = true;
+#pragma unroll
+  for (int k = 0; k < BM / 64; ++k) all = all && (ids[k * 64 + lane] == g || k * 64 + lane >= live);
+  return __ballot(all) == ~0ull;
+}
+
 // WGM x WGN wavefronts, BM x BN outputs.  The low-rank term of each adapter that the tile meets goes through the same ring, behind the projection's
-// own columns: R further columns of the contraction, the adapter's rows of T (others read as zeros) against its B.  (Fragments of T and B
+// own columns: R further columns of the contraction, the adapter's rows of T against its B.  (Fragments of T and B
 // straight from memory instead cost a load latency per 32 columns of rank: 28 against 18 us at 4096 x 640 x 640, rank 320.)
-template <int BM, int BN, int WGM, int WGN, int NSTG>
-__global__ __launch_bounds__(WGM * WGN * 64) void tile_kernel(const LinArgs a) {
+// What the tile may meet: ANY adapters; ONE or none (the caller knows); or FIND out -- where it is not one or none, false comes back and nothing is written.
+enum Meets { ANY, ONE, FIND };
+template <int BM, int BN, int WGM, int WGN, int NSTG, Meets MEETS>
+__device__ __forceinline__ bool tile_body(const LinArgs& a, char* lds, long m0, int n0) {
   constexpr int NW = WGM * WGN, WM = BM / WGM, WN = BN / WGN, FM = WM / 16, FN = WN / 16, STAGE = (BM + BN) * 128;
-  // ONE shared array: with a second one the compiler tells the two apart, takes the fragment reads for readers of the copies in flight, and waits
-  // for all of them (s_waitcnt vmcnt(0)) in every step
-  __shared__ __attribute__((aligned(16))) char lds[NSTG * STAGE + BM * 4];
   int* ids = reinterpret_cast<int*>(lds + NSTG * STAGE);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = lane & 15, q = lane >> 4;
-  const uint32_t tiles_n = (a.N + BN - 1) / BN, tile = xcd_tile(blockIdx.x, gridDim.x);
-  const long m0 = (long)(tile / tiles_n) * BM;
-  const int n0 = (int)(tile % tiles_n) * BN;
   const int mlive = (int)min((long)BM, a.M - m0), nlive = min(BN, a.N - n0);
   const long w0 = m0 + (wave / WGN) * WM;          // this wavefront's rows and columns
   const int v0 = n0 + (wave % WGN) * WN;
@@ -410,7 +443,8 @@ __global__ __launch_bounds__(WGM * WGN * 64) void tile_kernel(const LinArgs a) {
   Stage<BN, NW> sw;
   sx.begin(a.X + m0 * a.ldx, a.ldx, a.K, tid, [&](int r) { return r < mlive; });
   sw.begin(a.W + (long)n0 * a.ldw, a.ldw, a.K, tid, [&](int r) { return r < nlive; });
-  int nk = (a.K + BK - 1) / BK, left = nk, g = -1;   // stages in all; stages left of the current part; its adapter
+  const int nk = (a.K + BK - 1) / BK;
+  int left = nk, g = -1;   // stages still to be copied of the current part; its adapter
   const int rk = (a.R + BK - 1) / BK;
   auto issue = [&](int st) {
     if (left == 0 && a.rows.id != nullptr) {   // (uniform)
@@ -441,9 +475,27 @@ __global__ __launch_bounds__(WGM * WGN * 64) void tile_kernel(const LinArgs a) {
 #pragma unroll
     for (int u = 0; u < NSTG - 1; ++u) issue(u);
   }
-  if (a.rows.id != nullptr)
-    for (int h = next_adapter<BM>(ids, -1, lane); h >= 0; h = next_adapter<BM>(ids, h, lane)) nk += rk;
-  ring<BM, BN, WGM, WGN, NSTG, true>(lds, nk, tid, acc, issue);
+  Ring<BM, BN, NW, NSTG> ring{lds};
+  if constexpr (MEETS == ANY) {
+    for (int t = 0; t < nk; ++t) products<BM, BN, WGM, WGN, true>(ring.turn(issue), wave, lane, acc);
+    if (a.rows.id != nullptr) {
+      for (int h = next_adapter<BM>(ids, -1, lane); h >= 0; h = next_adapter<BM>(ids, h, lane)) {
+        uint32_t own = 0;
+#pragma unroll
+        for (int i = 0; i < FM; ++i) own |= (uint32_t)(ids[(wave / WGN) * WM + i * 16 + i16] == h) << i;
+        for (int t = 0; t < rk; ++t) products<BM, BN, WGM, WGN, true, true>(ring.turn(issue), wave, lane, acc, own);
+      }
+    }
+  } else {
+    const int h = a.rows.id != nullptr ? next_adapter<BM>(ids, -1, lane) : -1;
+    if (MEETS == FIND && h >= 0 && !one_adapter<BM>(ids, h, mlive, lane)) {
+      ring.drain();
+      return false;
+    }
+    const int n = nk + (h < 0 ? 0 : rk);
+    for (int t = 0; t < n; ++t) products<BM, BN, WGM, WGN, true>(ring.turn(issue), wave, lane, acc);
+  }
+  ring.drain();
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
     const long m = w0 + i * 16 + i16;
@@ -460,6 +512,24 @@ __global__ __launch_bounds__(WGM * WGN * 64) void tile_kernel(const LinArgs a) {
       if (n >= a.N) continue;
       const f32x4_t v = acc[i][FN - 1];
       *reinterpret_cast<uint2*>(a.Y + m * a.ldy + n) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+    }
+  }
+  return true;
+}
+
+template <int BM, int BN, int WGM, int WGN, int NSTG, Meets MEETS = ANY>
+__global__ __launch_bounds__(WGM * WGN * 64, 2) void tile_kernel(const LinArgs a) {
+  // ONE shared array: with a second one the compiler tells the two apart, takes the fragment reads for readers of the copies in flight, and waits
+  // for all of them (s_waitcnt vmcnt(0)) in every step
+  __shared__ __attribute__((aligned(16))) char lds[NSTG * (BM + BN) * 128 + BM * 4];
+  const uint32_t tiles_n = (a.N + BN - 1) / BN, tile = xcd_tile(blockIdx.x, gridDim.x);
+  const long m0 = (long)(tile / tiles_n) * BM;
+  const int n0 = (int)(tile % tiles_n) * BN;
+  const bool done = tile_body<BM, BN, WGM, WGN, NSTG, MEETS>(a, lds, m0, n0);
+  if constexpr (MEETS == FIND) {   // the selects of ANY need registers that this tile does not have: in two halves
+    for (int half = 0; half < 2 && !done; ++half) {
+      __syncthreads();
+      if (m0 + half * (BM / 2) < a.M) tile_body<BM / 2, BN, WGM, WGN, NSTG, ANY>(a, lds, m0 + half * (BM / 2), n0);
     }
   }
 }
@@ -498,7 +568,7 @@ __global__ __launch_bounds__(256) void down_tile_kernel(const DownArgs a) {
   constexpr int BM = 64, FM = 2, FN = BN / 32, STAGE = (BM + BN) * 128;
   __shared__ __attribute__((aligned(16))) char lds[NSTG * STAGE + BM * 4];   // (one array: see tile_kernel)
   int* ids = reinterpret_cast<int*>(lds + NSTG * STAGE);
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = lane & 15, q = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t tiles_r = (a.R + BN - 1) / BN, tile = xcd_tile(blockIdx.x, gridDim.x);
   const long m0 = (long)(tile / tiles_r) * BM;
   const int r0 = (int)(tile % tiles_r) * BN;
@@ -525,7 +595,9 @@ __global__ __launch_bounds__(256) void down_tile_kernel(const DownArgs a) {
     };
 #pragma unroll
     for (int u = 0; u < NSTG - 1; ++u) issue(u);
-    ring<BM, BN, 2, 2, NSTG, FN % 2 == 0>(lds, (a.K + BK - 1) / BK, tid, acc, issue);
+    Ring<BM, BN, 4, NSTG> ring{lds};
+    for (int t = 0; t < (a.K + BK - 1) / BK; ++t) products<BM, BN, 2, 2, FN % 2 == 0>(ring.turn(issue), wave, lane, acc);
+    ring.drain();
     store_tile(a, acc, ids, g, sc, rank, m0, (wave >> 1) * 32, r0 + (wave & 1) * (BN / 2), lane);
     __syncthreads();   // the stages are free for the next adapter
   }
@@ -902,15 +974,17 @@ extern "C" int aql_adapter_linear(const bf16_t* X, long ldx, const bf16_t* W, lo
   if (M <= 256) {
     hipLaunchKernelGGL((skinny_kernel<1>), dim3((N + 15) / 16, (unsigned)((M + 15) / 16)), dim3(512), 0, stream, a);
   } else {
-#define AQL_TILE(BM, BN, WGM, WGN, NSTG) \
-  hipLaunchKernelGGL((tile_kernel<BM, BN, WGM, WGN, NSTG>), dim3((unsigned)(((M + BM - 1) / BM) * ((N + BN - 1) / BN))), dim3(WGM * WGN * 64), 0, stream, a)
+#define AQL_TILE(BM, BN, WGM, WGN, ...) \
+  hipLaunchKernelGGL((tile_kernel<BM, BN, WGM, WGN, __VA_ARGS__>), dim3((unsigned)(((M + BM - 1) / BM) * ((N + BN - 1) / BN))), dim3(WGM * WGN * 64), 0, stream, a)
     // Which tile (all measured at every one of these sizes; us, best first): 256 x 320 where the width allows it and every CU gets one (4096 x 10240 x 1280:
     // 115.8 / 154 with 128 x 160); else 128 rows by 160 or 128 columns, whichever needs less time for its rounds of two tiles per CU
     // (32768 x 320 x 320: 15.1 / 19.4; 9001 x 1280 x 1280: 40.8 with 128, 45.9 with 160; 128 x 128 on eight wavefronts, on four 59.8 against 55.9 with
     // the low-rank term); smaller ones where those leave CUs idle (2048 x 1280 x
     // 1280: 14.9 with 64 x 128, 18.2 with 128 x 128; 1001 x 640 x 768: 6.3 with 64 x 64, 8.4 with 64 x 128)
     const auto tiles = [&](long bm, long bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
-    if (N % 320 == 0 && tiles(256, 320) >= 256) AQL_TILE(256, 320, 2, 4, 2);
+    // (requests of whole 256-row tiles: no tile meets two adapters; 109 us, 115 where the kernel has to find out)
+    if (N % 320 == 0 && tiles(256, 320) >= 256 && (runs == 0 || unit % 256 == 0)) AQL_TILE(256, 320, 2, 4, 2, ONE);
+    else if (N % 320 == 0 && tiles(256, 320) >= 256) AQL_TILE(256, 320, 2, 4, 2, FIND);
     else if (tiles(128, 128) >= 256 && (tiles(128, 160) + 511) / 512 * 160 <= (tiles(128, 128) + 511) / 512 * 128) AQL_TILE(128, 160, 2, 2, 2);
     else if (tiles(128, 128) >= 256) AQL_TILE(128, 128, 2, 4, 2);
     else if (tiles(64, 128) >= 256) AQL_TILE(64, 128, 2, 4, 3);

@@ -239,7 +239,7 @@ struct Bank {   // the device side of adapters.AdapterBank
 struct Plan {   // the device side of adapters.RequestPlan
   Tensor table;
   std::vector<long> start;   // host copy, in units
-  long units = 0, requests = 0, live_units = 0;
+  long units = 0, requests = 0, live_units = 0, unit_rows = 1;   // unit_rows: rows per unit where the requests have given lengths
   int nseg = 0, nused = 0, nslot = 0, max_id = -1;
   bool equal = false;
   std::vector<long> at;      // offsets of unit_id, perm, used_pos, slot in the table
@@ -249,8 +249,8 @@ struct Plan {   // the device side of adapters.RequestPlan
   const int* part(int k) const { return (const int*)table.data_ptr() + at[k]; }
   long unit(long rows) const {   // rows per table unit for a call on `rows` rows
     if (!equal) {
-      if (rows != units) bad_value("RequestPlan: the requests have " + std::to_string(units) + " rows, the call " + std::to_string(rows));
-      return 1;
+      if (rows != units * unit_rows) bad_value("RequestPlan: the requests have " + std::to_string(units * unit_rows) + " rows, the call " + std::to_string(rows));
+      return unit_rows;
     }
     if (requests == 0) {
       if (rows) bad_value("RequestPlan: no requests for " + std::to_string(rows) + " rows");
@@ -435,7 +435,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   py::class_<Plan, std::shared_ptr<Plan>>(m, "Plan")
       .def(py::init<>())
       .def_readwrite("table", &Plan::table).def_readwrite("start", &Plan::start).def_readwrite("at", &Plan::at)
-      .def_readwrite("units", &Plan::units).def_readwrite("requests", &Plan::requests).def_readwrite("live_units", &Plan::live_units)
+      .def_readwrite("units", &Plan::units).def_readwrite("requests", &Plan::requests).def_readwrite("live_units", &Plan::live_units).def_readwrite("unit_rows", &Plan::unit_rows)
       .def_readwrite("nseg", &Plan::nseg).def_readwrite("nused", &Plan::nused).def_readwrite("nslot", &Plan::nslot)
       .def_readwrite("max_id", &Plan::max_id).def_readwrite("equal", &Plan::equal)
       .def("unit", &Plan::unit).def("slots", &Plan::slots);

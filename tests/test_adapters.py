@@ -32,6 +32,7 @@ CASES = {
     "large_rank": ([130, 70, 200], [1, 0, 1], 200, 320, 320),
     "whole_rows_in_one_launch": ([9000, 130, 5, 15500], [1, 0, -1, 2], 200, 264, 40),
     "wide_tiles": ([7000, 3000, 6400], [0, 1, 0], 72, 1600, 16),
+    "whole_wide_tiles": ((8, 16384), [1, 0, -1, 2, 2, 0, 1, -1], 72, 1280, 24),
     "columns_of_160": ([20000, 13000], [1, 0], 64, 320, 72),
     "neighbours_of_one_adapter": ([16, 16, 16, 300], [1, 1, 0, 0], 64, 64, 12),
     "no_adapters": ([3, 270], [-1, -1], 64, 72, 8),
@@ -220,6 +221,37 @@ def test_requests_do_not_reach_each_other(name):
         assert not torch.isfinite(got[0][~keep]).any()
         other = [g for g in range(bank.G) if g != ids[victim]]
         assert torch.equal(got[2][other], want[2][other]) and torch.equal(got[3][other], want[3][other])
+
+
+@gpu
+@pytest.mark.parametrize("name", [n for n, c in CASES.items() if len(set(c[1]) - {-1}) > 1])
+def test_adapters_do_not_reach_each_other(name):
+    """An adapter in use whose weights hold infinities and NaN: the rows and gradients of all the others keep their bits."""
+    d, lengths, rows, ids, equal = make(name, 9)
+    packed, bank, plan = handles(d, lengths, ids, equal, True)
+    victim = next(g for n, g in zip(rows, ids) if g >= 0 and n > 0)
+    of = torch.repeat_interleave(torch.tensor(ids), torch.tensor(rows))
+    dy = d["dy"].to(DEV)
+
+    def step(bank):
+        x = d["x"].to(DEV).requires_grad_(True)
+        y = ops.adapter_linear(x, packed, bank, plan)
+        return (y.detach(),) + torch.autograd.grad(y, (x, bank.down, bank.up), dy)
+    want = step(bank)
+    keep = (of != victim).to(DEV)
+    others = [g for g in range(bank.G) if g != victim]
+    for key, value in (("down", float("nan")), ("up", float("nan")), ("up", float("inf"))):
+        bad = dict(d, **{key: d[key].clone()})
+        bad[key][victim, -1 if key == "up" else 0, 0] = value
+        _, bank2, _ = handles(bad, lengths, ids, equal, True)
+        got = step(bank2)
+        assert not torch.isfinite(got[0][~keep]).all()
+        for a, b in zip(got[:2], want[:2]):
+            assert torch.equal(a[keep], b[keep]), (key, value)
+        for a, b in zip(got[2:], want[2:]):
+            assert torch.equal(a[others], b[others]), (key, value)
+        if key == "up":      # ... and of the adapter itself the columns that it does not touch
+            assert torch.equal(got[0][:, :-1], want[0][:, :-1])
 
 
 @gpu

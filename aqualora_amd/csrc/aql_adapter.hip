@@ -976,16 +976,19 @@ extern "C" int aql_adapter_linear(const bf16_t* X, long ldx, const bf16_t* W, lo
   } else {
 #define AQL_TILE(BM, BN, WGM, WGN, ...) \
   hipLaunchKernelGGL((tile_kernel<BM, BN, WGM, WGN, __VA_ARGS__>), dim3((unsigned)(((M + BM - 1) / BM) * ((N + BN - 1) / BN))), dim3(WGM * WGN * 64), 0, stream, a)
-    // Which tile (all measured at every one of these sizes; us, best first): 256 x 320 where the width allows it and every CU gets one (4096 x 10240 x 1280:
-    // 115.8 / 154 with 128 x 160); else 128 rows by 160 or 128 columns, whichever needs less time for its rounds of two tiles per CU
-    // (32768 x 320 x 320: 15.1 / 19.4; 9001 x 1280 x 1280: 40.8 with 128, 45.9 with 160; 128 x 128 on eight wavefronts, on four 59.8 against 55.9 with
-    // the low-rank term); smaller ones where those leave CUs idle (2048 x 1280 x
-    // 1280: 14.9 with 64 x 128, 18.2 with 128 x 128; 1001 x 640 x 768: 6.3 with 64 x 64, 8.4 with 64 x 128)
+    // Which tile (us without adapters, all tiles measured at each size): 256 x 320 where the width allows it and every CU gets one (4096 x 10240 x
+    // 1280: 99, 128 x 160 141, 128 x 128 141); else 128 rows by 160 or 128 columns, whichever needs less time for its rounds of two tiles per CU
+    // (9001 x 1280 x 1280: 37.7 with 128, 40.9 with 160), the former as 128 x 320 where that divides the width (16384 x 640 x 2560: 52.3 / 54.7;
+    // 32768 x 320 x 320: 13.0 / 16.1); smaller ones where those leave CUs idle (2048 x 1280 x 1280: 13.2 with 64 x 128, 14.8 with 128 x 128;
+    // 1001 x 640 x 768: 6.0 with 64 x 64, 6.6 with 64 x 128).  256 x 320 with requests of whole 256-row tiles: no tile meets two adapters, and the
+    // kernel need not find out (109 / 115 with rank 32).
     const auto tiles = [&](long bm, long bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
-    // (requests of whole 256-row tiles: no tile meets two adapters; 109 us, 115 where the kernel has to find out)
     if (N % 320 == 0 && tiles(256, 320) >= 256 && (runs == 0 || unit % 256 == 0)) AQL_TILE(256, 320, 2, 4, 2, ONE);
     else if (N % 320 == 0 && tiles(256, 320) >= 256) AQL_TILE(256, 320, 2, 4, 2, FIND);
-    else if (tiles(128, 128) >= 256 && (tiles(128, 160) + 511) / 512 * 160 <= (tiles(128, 128) + 511) / 512 * 128) AQL_TILE(128, 160, 2, 2, 2);
+    else if (tiles(128, 128) >= 256 && (tiles(128, 160) + 511) / 512 * 160 <= (tiles(128, 128) + 511) / 512 * 128) {
+      if (N % 320 == 0) AQL_TILE(128, 320, 2, 4, 2);
+      else AQL_TILE(128, 160, 2, 2, 2);
+    }
     else if (tiles(128, 128) >= 256) AQL_TILE(128, 128, 2, 4, 2);
     else if (tiles(64, 128) >= 256) AQL_TILE(64, 128, 2, 4, 3);
     else AQL_TILE(64, 64, 2, 2, 3);

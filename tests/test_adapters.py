@@ -33,7 +33,9 @@ CASES = {
     "whole_rows_in_one_launch": ([9000, 130, 5, 15500], [1, 0, -1, 2], 200, 264, 40),
     "wide_tiles": ([7000, 3000, 6400], [0, 1, 0], 72, 1600, 16),
     "whole_wide_tiles": ((8, 16384), [1, 0, -1, 2, 2, 0, 1, -1], 72, 1280, 24),
-    "columns_of_160": ([20000, 13000], [1, 0], 64, 320, 72),
+    "columns_of_160": ([13000, 8700], [1, 0], 64, 480, 72),
+    "columns_of_320": ([20000, 12700], [1, 0], 64, 320, 72),
+    "two_rounds": ([20000, 13000], [1, 0], 64, 320, 72),
     "neighbours_of_one_adapter": ([16, 16, 16, 300], [1, 1, 0, 0], 64, 64, 12),
     "no_adapters": ([3, 270], [-1, -1], 64, 72, 8),
 }

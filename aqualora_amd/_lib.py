@@ -61,8 +61,8 @@ SIGNATURES = {
     "aql_groupnorm_silu_bwd": [c_p, c_p, c_i, c_i, c_i, c_p, c_p, c_i, c_p, c_p, c_p, c_p, c_p],
     "aql_layernorm_fwd": [c_p, c_l, c_i, c_p, c_p, c_f, c_p, c_p, c_p],
     "aql_layernorm_bwd": [c_p, c_p, c_l, c_i, c_p, c_p, c_p, c_p, c_p],
-    # X ldx W ldw bias residual ldr Y ldy M N K | A B ranks scales R | unit_id unit runs slots | T parts stream
-    "aql_adapter_linear": [c_p, c_l, c_p, c_l, c_p, c_p, c_l, c_p, c_l, c_l, c_i, c_i, c_p, c_p, c_p, c_p, c_i, c_p, c_i, c_i, c_i, c_p, c_i, c_p],
+    # X ldx W ldw bias residual ldr Y ldy M N K | A B ranks scales R | unit_id unit runs slots used | T parts stream
+    "aql_adapter_linear": [c_p, c_l, c_p, c_l, c_p, c_p, c_l, c_p, c_l, c_l, c_i, c_i, c_p, c_p, c_p, c_p, c_i, c_p, c_i, c_i, c_i, c_i, c_p, c_i, c_p],
     "aql_adapter_down": [c_p, c_l, c_p, c_p, c_l, c_i, c_p, c_p, c_p, c_i, c_p, c_i, c_i, c_i, c_p, c_i, c_p],
     "aql_adapter_wgrad_scratch_floats": [c_l, c_i, c_i, c_i, c_i],
     # dT X ldx codes exps K dA | T dY lddy N dB | M G R r_out ranks perm used_pos slot nused nslot unit rows | scratch floats stream

@@ -953,10 +953,10 @@ bool rows_ok(const void* id, int runs, int unit) { return runs >= 0 && (runs == 
 }  // namespace
 
 // Y = X W^T + bias + residual + the low-rank term; T: [M][parts][R] bf16, written for the rows that have an adapter.  slots: at least the number of adapters that
-// any 16 rows [16 i, 16 i + 16) meet; runs: stretches of neighbouring rows with one adapter (how long they are decides between the forms of the first launch).
+// any 16 rows [16 i, 16 i + 16) meet; runs: stretches of neighbouring rows with one adapter; used: adapters that have rows (these two decide between forms only).
 extern "C" int aql_adapter_linear(const bf16_t* X, long ldx, const bf16_t* W, long ldw, const bf16_t* bias, const bf16_t* residual, long ldr, bf16_t* Y,
                                   long ldy, long M, int N, int K, const bf16_t* A, const bf16_t* B, const int* ranks, const float* scales, int R,
-                                  const int* unit_id, int unit, int runs, int slots, bf16_t* T, int parts, hipStream_t stream) {
+                                  const int* unit_id, int unit, int runs, int slots, int used, bf16_t* T, int parts, hipStream_t stream) {
   AQL_CHECK_ARG(M >= 0 && M < (1L << 31) - 256 && N > 0 && K > 0 && N % 8 == 0 && K % 8 == 0, "aql_adapter_linear: bad shape M=%ld N=%d K=%d (N, K: multiples of 8)", M, N, K);
   if (M == 0) return AQL_OK;
   AQL_CHECK_ARG(X && W && Y, "aql_adapter_linear: null operand");
@@ -971,8 +971,17 @@ extern "C" int aql_adapter_linear(const bf16_t* X, long ldx, const bf16_t* W, lo
     AQL_CHECK_LAUNCH("aql_adapter_linear (down)");
   }
   const LinArgs a{X, W, bias, residual, B, Y, T, ldx, ldw, ldr, ldy, M, N, K, R, parts, rows};
-  if (M <= 256) {
-    hipLaunchKernelGGL((skinny_kernel<1>), dim3((N + 15) / 16, (unsigned)((M + 15) / 16)), dim3(512), 0, stream, a);
+  // Sixteen rows at a time, or tiles of 64 rows and more: by the number of 16 x 16 outputs, and by the adapters that 64 rows meet, each of which costs a
+  // tile another turn of its ring per 64 columns of rank.  Both launches of a call together, us, 16 rows / 64 x 64 tiles, rank 32, four requests and
+  // single rows of eight adapters: 256 x 1280 x 1280 (1280 outputs): 16.4 / 13.1 and 20.8 / 20.9; 128 x 1280 x 1280 (640): 13.2 / 13.8 and 14.9 / 18.7;
+  // 64 x 10240 x 1280 (2560): 24.6 / 16.2 and 27.0 / 20.0
+  const long outs = ((M + 15) / 16) * ((N + 15) / 16);
+  const long met = runs ? (64L * runs / M + 1 < used ? 64L * runs / M + 1 : used) : 0;
+  if (outs < 960 + 32 * met * ((R + BK - 1) / BK)) {
+    const unsigned my = (unsigned)((M + 15) / 16);
+    // two fragments of columns per wavefront where one each gives more workgroups than CUs (64 x 1280 x 1280: 9.9 us, with one 10.8; 8 x 1280 x 1280: 10.5 / 9.0)
+    if (outs > 256) hipLaunchKernelGGL((skinny_kernel<2>), dim3((N + 31) / 32, my), dim3(512), 0, stream, a);
+    else hipLaunchKernelGGL((skinny_kernel<1>), dim3((N + 15) / 16, my), dim3(512), 0, stream, a);
   } else {
 #define AQL_TILE(BM, BN, WGM, WGN, ...) \
   hipLaunchKernelGGL((tile_kernel<BM, BN, WGM, WGN, __VA_ARGS__>), dim3((unsigned)(((M + BM - 1) / BM) * ((N + BN - 1) / BN))), dim3(WGM * WGN * 64), 0, stream, a)

@@ -294,7 +294,7 @@ std::pair<Tensor, Tensor> product(const Rows& x, const Tensor& w, const Tensor& 
   const auto st = stream_of(y);
   ran(aql_adapter_linear(ptr<bf16_t>(x.t), x.ld, ptr<bf16_t>(w), K, ptr<bf16_t>(bias), ptr<bf16_t>(res.t), res.ld, ptr<bf16_t>(y), N, M, (int)N, (int)K,
                          ptr<bf16_t>(a), ptr<bf16_t>(b), ptr<int>(bank.ranks), ptr<float>(bank.scales), (int)bank.R, plan.part(0), (int)unit, plan.nseg,
-                         plan.slots(unit), ptr<bf16_t>(T), parts, st), "aql_adapter_linear", st);
+                         plan.slots(unit), plan.nused, ptr<bf16_t>(T), parts, st), "aql_adapter_linear", st);
   return {y, T};
 }
 

@@ -37,6 +37,8 @@ CASES = {
     "columns_of_320": ([20000, 12700], [1, 0], 64, 320, 72),
     "two_rounds": ([20000, 13000], [1, 0], 64, 320, 72),
     "neighbours_of_one_adapter": ([16, 16, 16, 300], [1, 1, 0, 0], 64, 64, 12),
+    "many_rows_many_adapters": ([1] * 300, [(7 * i) % 40 for i in range(300)], 320, 640, 16),
+    "wide_few_rows": ([60, 4], [1, 0], 72, 10240, 24),
     "no_adapters": ([3, 270], [-1, -1], 64, 72, 8),
 }
 
@@ -467,7 +469,7 @@ def test_refusals_without_a_gpu():
     lib, p = _lib.load(), _lib.c_p(4096)               # p is never dereferenced: every call is refused on the host
 
     def linear(M=64, N=64, K=64, R=8, ldx=64, X=p, T=p, slots=2, nseg=1, unit=1, seg=p, parts=1):
-        return lib.aql_adapter_linear(X, ldx, p, K, None, None, 0, p, N, M, N, K, p, p, p, p, R, seg, unit, nseg, slots, T, parts, None)
+        return lib.aql_adapter_linear(X, ldx, p, K, None, None, 0, p, N, M, N, K, p, p, p, p, R, seg, unit, nseg, slots, 1, T, parts, None)
     for kw in (dict(N=60), dict(K=60, ldx=64), dict(ldx=56), dict(R=4), dict(R=0), dict(X=None), dict(T=None), dict(slots=0), dict(slots=17), dict(unit=0),
                dict(seg=None), dict(nseg=-1), dict(X=_lib.c_p(4104)), dict(M=-1), dict(M=1 << 31), dict(ldx=1 << 21), dict(parts=2)):
         assert linear(**kw) != 0, kw

@@ -259,6 +259,34 @@ def test_adapters_do_not_reach_each_other(name):
 
 
 @gpu
+@pytest.mark.parametrize("ckpt8", [False, True])
+def test_rows_past_31_bit_offsets(ckpt8):
+    """More than 2^31 elements in x and dx: the last request, which alone uses its adapter, against the definition."""
+    K, N, r, last = 1280, 64, 16, 700
+    M = (1 << 31) // K + 3000
+    gen = torch.Generator(DEV).manual_seed(11)
+    cpu = torch.Generator().manual_seed(12)
+    rn = lambda *s: torch.randn(s, generator=cpu)  # noqa: E731
+    bf = lambda t: t.to(torch.bfloat16)  # noqa: E731
+    x = torch.empty(M, K, device=DEV, dtype=torch.bfloat16)
+    dy = torch.empty(M, N, device=DEV, dtype=torch.bfloat16)
+    for t in (x, dy):
+        for part in t.split(100000):
+            part.copy_(torch.randn(part.shape, generator=gen, device=DEV))
+    d = dict(x=x[-last:].cpu(), dy=dy[-last:].cpu(), w=bf(rn(N, K) / K ** 0.5), bias=bf(rn(N)), down=bf(rn(2, r, K) / r), up=bf(0.2 * rn(2, N, r)),
+             scales=[1.0, 0.5], ranks=[r, r - 3], live=torch.arange(r)[None] < torch.tensor([[r], [r - 3]]))
+    packed, bank, _ = handles(d, [1], [0], False, True)
+    x.requires_grad_(True)
+    y = ops.adapter_linear(x, packed, bank, adapters.RequestPlan([0, 1], [M - last, last]), ckpt8=ckpt8)
+    dx, dA, dB = torch.autograd.grad(y, (x, bank.down, bank.up), dy)
+    ref, slack = reference(d, [last], [1], False, codes64(d["x"]) if ckpt8 else d["x"])
+    check("y", y[-last:], ref[0], slack[0], HALF)
+    check("dx", dx[-last:], ref[1], slack[1], HALF)
+    check("dA", dA[1], ref[2][1], slack[2][1], 2.0 ** -24)
+    check("dB", dB[1], ref[3][1], slack[3][1], 2.0 ** -24)
+
+
+@gpu
 def test_empty_call():
     d, *_ = make("one_row")
     packed = ops.PackedLinear(d["w"].to(DEV), d["bias"].to(DEV))

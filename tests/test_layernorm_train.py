@@ -241,6 +241,29 @@ def test_act8_strided_and_many_dimensions():
 
 
 @gpu
+def test_rows_past_31_bit_offsets():
+    """More than 2^31 elements: the last rows of the codes, of y and of dx against the definition."""
+    C, last = 1280, 50
+    M = (1 << 31) // C + 3000
+    gen = torch.Generator("cuda").manual_seed(13)
+    x = torch.empty(M, C, device="cuda", dtype=torch.bfloat16)
+    for part in x.split(100000):
+        part.copy_(torch.randn(part.shape, generator=gen, device="cuda"))
+    packed = ops.act8_pack(x)
+    tail = x[-last:].cpu()
+    assert torch.equal(packed.unpack()[-last:].double().cpu(), codes64(tail))
+    del packed
+    gamma, beta = torch.randn(C, generator=gen, device="cuda"), torch.randn(C, generator=gen, device="cuda")
+    for ckpt8 in (False, True):
+        xg = x.detach().requires_grad_(True)
+        y = ops.layernorm_train(xg, gamma, beta, ckpt8=ckpt8)
+        dx, = torch.autograd.grad(y, (xg,), x)
+        ref, slack = reference(tail, codes64(tail) if ckpt8 else tail, gamma.cpu(), beta.cpu(), tail, None, 1e-5)
+        for name, got, k in (("y", y[-last:], 0), ("dx", dx[-last:], 1)):
+            check(name, got, ref[k], slack[k], torch.bfloat16)
+
+
+@gpu
 def test_double_backward_is_refused():
     x = torch.randn(4, 32, device=DEV, requires_grad=True)
     g = torch.ones(32, device=DEV, requires_grad=True)

@@ -104,6 +104,8 @@ __global__ __launch_bounds__(NW * 64) void down_kernel(const DownArgs a) {
     g = -1;
   }
   if (g < 0) return;
+  const float sc = a.scales[g];   // (here, and bias and residual in the next kernel likewise: behind the join their latency would show)
+  const int rank = a.ranks[g];
   const int r0 = blockIdx.z * 16 * RT;
   const int ksteps = (a.K + 31) / 32;
   const long m = min(m0 + i, a.M - 1);
@@ -149,8 +151,6 @@ __global__ __launch_bounds__(NW * 64) void down_kernel(const DownArgs a) {
   }
   __syncthreads();
   if (wave) return;
-  const float sc = a.scales[g];
-  const int rank = a.ranks[g];
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     const int r = r0 + t * 16 + q * 4;
@@ -188,6 +188,13 @@ __global__ __launch_bounds__(512) void skinny_kernel(const LinArgs a) {
   const int ksteps = (a.K + 31) / 32;
   const long m = min(m0 + i, a.M - 1);
   const int gi = a.rows.id && m0 + i < a.M ? id_of(a.rows, m0 + i) : -1;
+  // wavefront j < NF writes fragment j at the end: row m0 + i, columns n0 + 16 j + 4 q ..
+  const long mw = m0 + i;
+  const int nw = n0 + wave * 16 + q * 4;
+  const bool writes = wave < NF && mw < a.M && nw < a.N;
+  uint2 add[2] = {make_uint2(0u, 0u), make_uint2(0u, 0u)};
+  if (writes && a.bias) add[0] = *reinterpret_cast<const uint2*>(a.bias + nw);
+  if (writes && a.res) add[1] = *reinterpret_cast<const uint2*>(a.res + mw * a.ldr + nw);
   f32x4_t acc[NF];
 #pragma unroll
   for (int j = 0; j < NF; ++j) acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -234,28 +241,16 @@ __global__ __launch_bounds__(512) void skinny_kernel(const LinArgs a) {
 #pragma unroll
   for (int j = 0; j < NF; ++j) *reinterpret_cast<f32x4_t*>(red[wave][j][lane]) = acc[j];
   __syncthreads();
-  for (int id = threadIdx.x; id < NF * 64; id += 512) {
-    const int j = id >> 6, l = id & 63;
-    const long mr = m0 + (l & 15);
-    const int n = n0 + j * 16 + (l >> 4) * 4;
-    if (mr >= a.M || n >= a.N) continue;
-    float v[4];
+  if (!writes) return;
+  float v[4] = {bf16lo(add[0].x) + bf16lo(add[1].x), bf16hi(add[0].x) + bf16hi(add[1].x), bf16lo(add[0].y) + bf16lo(add[1].y), bf16hi(add[0].y) + bf16hi(add[1].y)};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[e] = 0.f;
+  for (int e = 0; e < 4; ++e) {
+    float t = 0.f;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) v[e] += red[w][j][l][e];
-    }
-    if (a.bias) {
-      const uint2 b = *reinterpret_cast<const uint2*>(a.bias + n);
-      v[0] += bf16lo(b.x), v[1] += bf16hi(b.x), v[2] += bf16lo(b.y), v[3] += bf16hi(b.y);
-    }
-    if (a.res) {
-      const uint2 b = *reinterpret_cast<const uint2*>(a.res + mr * a.ldr + n);
-      v[0] += bf16lo(b.x), v[1] += bf16hi(b.x), v[2] += bf16lo(b.y), v[3] += bf16hi(b.y);
-    }
-    *reinterpret_cast<uint2*>(a.Y + mr * a.ldy + n) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+    for (int w = 0; w < 8; ++w) t += red[w][wave][lane][e];
+    v[e] += t;
   }
+  *reinterpret_cast<uint2*>(a.Y + mw * a.ldy + nw) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
 }
 
 // ------------------------------------------------------------------------------------------------------------- many rows: LDS tiles

@@ -8,7 +8,9 @@
 #include <torch/extension.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cstdlib>
@@ -61,6 +63,24 @@ void here(const Tensor& t, const char* name) {
                  std::to_string(c10::hip::current_device()) + "; wrap the call in torch.cuda.device(...)");
 }
 aql_stream_t stream_of(const Tensor& t) { return (aql_stream_t)c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+
+// at::empty without the dispatcher's way to it: a backward pass allocates up to seven tensors
+Tensor fresh(at::IntArrayRef size, at::ScalarType type, const Tensor& like) { return at::detail::empty_cuda(size, type, like.device(), std::nullopt); }
+// two fp32 tensors in one allocation (a pair of gradients: they live and end together); an unwanted one stays undefined
+std::pair<Tensor, Tensor> fresh_pair(bool one, at::IntArrayRef a, bool two, at::IntArrayRef b, const Tensor& like) {
+  if (!one || !two) return {one ? fresh(a, at::kFloat, like) : Tensor(), two ? fresh(b, at::kFloat, like) : Tensor()};
+  const int64_t na = (c10::multiply_integers(a) + 3) / 4 * 4;   // (both 16-byte aligned)
+  const Tensor buf = fresh({na + c10::multiply_integers(b)}, at::kFloat, like);
+  const auto view = [&](at::IntArrayRef size, int64_t offset) {
+    Tensor t = at::detail::make_tensor<at::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(buf.storage()), buf.key_set(), buf.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(offset);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(size);
+    return t;
+  };
+  return {view(a, 0), view(b, na)};
+}
+// workspace of one call, returned to the caching allocator behind it on the same stream
+c10::DataPtr workspace(long floats) { return c10::hip::HIPCachingAllocator::get()->allocate(floats * 4); }
 
 int dt(const Tensor& t) { return t.scalar_type() == at::kBFloat16 ? 0 : 1; }
 bool bf16_or_f32(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat; }
@@ -121,8 +141,7 @@ variable_list once(variable_list grads, const char* name) {
 // ------------------------------------------------------------------------------------------------------------------ 8-bit checkpoint
 std::pair<Tensor, Tensor> act8_alloc(long M, long C, const Tensor& like) {
   const long Cp = (C + 31) / 32 * 32;
-  const auto opt = like.options().dtype(at::kByte).requires_grad(false);
-  return {at::empty({M, Cp}, opt), at::empty({M, Cp / 32}, opt)};
+  return {fresh({M, Cp}, at::kByte, like), fresh({M, Cp / 32}, at::kByte, like)};
 }
 
 std::pair<Tensor, Tensor> act8_pack(const Tensor& x) {
@@ -147,60 +166,67 @@ Tensor act8_unpack(const Tensor& codes, const Tensor& exps, std::vector<int64_t>
     bad_value("Act8.unpack: codes uint8 [" + std::to_string(M) + ", " + std::to_string(Cp) + "] and exps uint8 [" + std::to_string(M) + ", " +
               std::to_string(Cp / 32) + "], contiguous on one device, not " + shape_of(codes) + " and " + shape_of(exps));
   here(codes, "Act8.unpack");
-  Tensor out = at::empty(shape, codes.options().dtype(bf16 ? at::kBFloat16 : at::kFloat));
+  Tensor out = fresh(shape, bf16 ? at::kBFloat16 : at::kFloat, codes);
   const auto st = stream_of(codes);
   ran(aql_act8_unpack(ptr<uint8_t>(codes), ptr<uint8_t>(exps), codes.size(0), (int)C, out.data_ptr(), bf16 ? 0 : 1, C, st), "aql_act8_unpack", st);
   return out;
 }
 
 // -------------------------------------------------------------------------------------------------------- LayerNorm with weight gradients
+struct NormCall : torch::CustomClassHolder {   // what its backward pass needs besides tensors of the graph
+  std::vector<Tensor> leaves;
+  bool beta = false;
+};
+
 struct LayerNormTrain : torch::autograd::Function<LayerNormTrain> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& gamma, const std::optional<Tensor>& beta_, double eps, bool ckpt8, bool passthrough) {
     const Tensor beta = beta_ ? *beta_ : Tensor();
     const long M = x.size(0), C = x.size(1);
     const Rows r = rows2d(x);
-    Tensor y = at::empty({M, C}, x.options()), stats = at::empty({M, 2}, x.options().dtype(at::kFloat)), codes, exps;
+    Tensor y = fresh({M, C}, x.scalar_type(), x), stats = fresh({M, 2}, at::kFloat, x), codes, exps;
     if (ckpt8) std::tie(codes, exps) = act8_alloc(M, C, x);
     const auto st = stream_of(x);
     ran(aql_layernorm_train_fwd(r.t.data_ptr(), dt(x), M, (int)C, r.ld, gamma.data_ptr(), ptr(beta), dt(gamma), (float)eps, y.data_ptr(), C,
                                 ptr<float>(stats), ptr<uint8_t>(codes), ptr<uint8_t>(exps), st), "aql_layernorm_train_fwd", st);
     ctx->save_for_backward({ckpt8 ? Tensor() : r.t, codes, exps, gamma, stats});
-    ctx->saved_data["beta"] = beta.defined();
-    ctx->saved_data["leaves"] = std::vector<Tensor>{leaf(x), leaf(gamma), leaf(beta)};
+    auto c = c10::make_intrusive<NormCall>();
+    c->beta = beta.defined();
+    c->leaves = {leaf(x), leaf(gamma), leaf(beta)};
+    ctx->saved_data["call"] = c10::IValue::make_capsule(std::move(c));
     if (passthrough) return {y, x.view_as(x)};
     return {y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const variable_list s = ctx->get_saved_variables();
     const Tensor &x = s[0], &codes = s[1], &exps = s[2], &gamma = s[3], &stats = s[4];
+    const auto c = c10::static_intrusive_pointer_cast<NormCall>(ctx->saved_data["call"].toCapsule());
     const long M = stats.size(0), C = gamma.size(0);
-    const bool want_g = ctx->needs_input_grad(1), want_b = ctx->saved_data["beta"].toBool() && ctx->needs_input_grad(2);
+    const bool want_g = ctx->needs_input_grad(1), want_b = c->beta && ctx->needs_input_grad(2);
     if (!g[0].defined()) {   // only the pass-through output was used
       const Tensor z;
       return {g.size() > 1 ? g[1] : z, z, z, z, z, z};
     }
     here(g[0], "layernorm_train backward");
-    leaves_ok(ctx->saved_data["leaves"].toTensorVector(), g[0], "layernorm_train");
+    leaves_ok(c->leaves, g[0], "layernorm_train");
     Tensor dx, dg, db;
     {
       at::AutoGradMode off(false);
-      const auto f32 = g[0].options().dtype(at::kFloat);
-      dx = at::empty({M, C}, g[0].options());
+      dx = fresh({M, C}, g[0].scalar_type(), g[0]);
       if (M == 0) {
+        const auto f32 = g[0].options().dtype(at::kFloat);
         if (want_g) dg = at::zeros({C}, f32);
         if (want_b) db = at::zeros({C}, f32);
       } else {
         const Rows dy = rows2d(g[0]);
         Rows dres;
         if (g.size() > 1 && g[1].defined()) dres = rows2d(g[1]);
-        if (want_g) dg = at::empty({C}, f32);
-        if (want_b) db = at::empty({C}, f32);
+        std::tie(dg, db) = fresh_pair(want_g, {C}, want_b, {C}, dx);
         const long n = aql_layernorm_train_scratch_floats(M, (int)C);
-        const Tensor scratch = at::empty({n}, f32);
+        const c10::DataPtr scratch = workspace(n);
         const auto st = stream_of(dx);
         ran(aql_layernorm_train_bwd(ptr(x), ptr<uint8_t>(codes), ptr<uint8_t>(exps), dy.t.data_ptr(), ptr(dres.t), dt(dx), M, (int)C,
                                     x.defined() && M > 1 ? x.stride(0) : C, dy.ld, dres.ld, gamma.data_ptr(), dt(gamma), ptr<float>(stats), dx.data_ptr(), C,
-                                    ptr<float>(dg), ptr<float>(db), ptr<float>(scratch), n, st), "aql_layernorm_train_bwd", st);
+                                    ptr<float>(dg), ptr<float>(db), (float*)scratch.get(), n, st), "aql_layernorm_train_bwd", st);
       }
       if (gamma.scalar_type() != at::kFloat) {
         if (dg.defined()) dg = dg.to(gamma.scalar_type());
@@ -289,8 +315,8 @@ struct Call : torch::CustomClassHolder {   // what a backward pass of adapter_li
 std::pair<Tensor, Tensor> product(const Rows& x, const Tensor& w, const Tensor& bias, const Rows& res, const Tensor& a, const Tensor& b, const Bank& bank,
                                   Plan& plan, long unit, long N, long K, int parts) {
   const long M = x.t.size(0);
-  Tensor y = at::empty({M, N}, x.t.options().requires_grad(false)), T;
-  if (plan.nseg) T = at::empty({M, parts, bank.R}, y.options());
+  Tensor y = fresh({M, N}, at::kBFloat16, x.t), T;
+  if (plan.nseg) T = fresh({M, parts, bank.R}, at::kBFloat16, y);
   const auto st = stream_of(y);
   ran(aql_adapter_linear(ptr<bf16_t>(x.t), x.ld, ptr<bf16_t>(w), K, ptr<bf16_t>(bias), ptr<bf16_t>(res.t), res.ld, ptr<bf16_t>(y), N, M, (int)N, (int)K,
                          ptr<bf16_t>(a), ptr<bf16_t>(b), ptr<int>(bank.ranks), ptr<float>(bank.scales), (int)bank.R, plan.part(0), (int)unit, plan.nseg,
@@ -299,7 +325,7 @@ std::pair<Tensor, Tensor> product(const Rows& x, const Tensor& w, const Tensor& 
 }
 
 Tensor down(const Rows& x, const Tensor& codes, const Tensor& exps, long M, long K, const Tensor& a, const Bank& bank, Plan& plan, long unit) {
-  Tensor T = at::empty({M, 3, bank.R}, a.options());
+  Tensor T = fresh({M, 3, bank.R}, at::kBFloat16, a);
   const auto st = stream_of(T);
   ran(aql_adapter_down(ptr<bf16_t>(x.t), x.ld, ptr<uint8_t>(codes), ptr<uint8_t>(exps), M, (int)K, ptr<bf16_t>(a), ptr<int>(bank.ranks), ptr<float>(bank.scales),
                        (int)bank.R, plan.part(0), (int)unit, plan.nseg, plan.slots(unit), ptr<bf16_t>(T), 3, st), "aql_adapter_down", st);
@@ -309,18 +335,15 @@ Tensor down(const Rows& x, const Tensor& codes, const Tensor& exps, long M, long
 // fp32 gradients of the stacks: dA [G, r, K] where want_a, dB [G, N, r] where want_b
 void wgrad(const Tensor& dT, const Rows& x, const Tensor& codes, const Tensor& exps, bool want_a, const Tensor& T, const Rows& dy, bool want_b, long M,
            const Bank& bank, const Plan& plan, long unit, Tensor& dA, Tensor& dB) {
-  const auto f32 = bank.scales.options();
-  if (want_a) dA = at::empty({bank.G, bank.r, bank.K}, f32);
-  if (want_b) dB = at::empty({bank.G, bank.N, bank.r}, f32);
+  std::tie(dA, dB) = fresh_pair(want_a, {bank.G, bank.r, bank.K}, want_b, {bank.G, bank.N, bank.r}, bank.scales);
   const long rows = plan.live_units * unit;
   const int n = aql_adapter_wgrad_scratch_floats(rows, plan.nused, want_a ? (int)bank.K : 0, want_b ? (int)bank.N : 0, (int)bank.R);
   if (n < 0) throw AqlErr("adapter_linear: the weight gradients' workspace passes 2^31 elements; train fewer rows or adapters per call");
-  Tensor scratch;
-  if (n) scratch = at::empty({n}, f32);
+  const c10::DataPtr scratch = workspace(n);
   const auto st = stream_of(bank.scales);
   ran(aql_adapter_wgrad(ptr<bf16_t>(dT), ptr<bf16_t>(x.t), x.ld, ptr<uint8_t>(codes), ptr<uint8_t>(exps), (int)bank.K, ptr<float>(dA), ptr<bf16_t>(T),
                         ptr<bf16_t>(dy.t), dy.ld, (int)bank.N, ptr<float>(dB), M, (int)bank.G, (int)bank.R, (int)bank.r, ptr<int>(bank.ranks), plan.part(1),
-                        plan.part(2), plan.part(3), plan.nused, plan.nslot, (int)unit, rows, ptr<float>(scratch), n, st), "aql_adapter_wgrad", st);
+                        plan.part(2), plan.part(3), plan.nused, plan.nslot, (int)unit, rows, (float*)scratch.get(), n, st), "aql_adapter_wgrad", st);
 }
 
 struct AdapterLinear : torch::autograd::Function<AdapterLinear> {
@@ -358,7 +381,7 @@ struct AdapterLinear : torch::autograd::Function<AdapterLinear> {
     {
       at::AutoGradMode off(false);
       if (c->M == 0) {
-        if (want_x) out[0] = at::empty({0, c->K}, g[0].options());
+        if (want_x) out[0] = fresh({0, c->K}, at::kBFloat16, g[0]);
         if (want_a) out[1] = at::zeros({bank.G, bank.r, bank.K}, bank.scales.options());
         if (want_b) out[2] = at::zeros({bank.G, bank.N, bank.r}, bank.scales.options());
       } else {

@@ -900,7 +900,8 @@ __global__ __launch_bounds__(256) void wgrad_reduce_kernel(const Grad da, const 
 // positions per chunk: whole tiles of 64
 int wgrad_chunk(long rows, int C, int R) {
   const long tiles = (long)((C + 127) / 128) * (R <= 32 ? 1 : (R + 63) / 64);
-  long want = 288 / tiles;   // workgroups of one gradient; dA and dB run together, three workgroups fit on a CU
+  // at most 256 workgroups for one gradient, two for each CU for both (4096 x 640, rank 320, with the sum: 27.6 us; 288: 30.4, 384: 29.0, 192: 31.6)
+  long want = 256 / tiles;
   if (want < 1) want = 1;
   long ch = (rows + want - 1) / want;
   ch = (ch + 63) / 64 * 64;
@@ -981,19 +982,22 @@ extern "C" int aql_adapter_linear(const bf16_t* X, long ldx, const bf16_t* W, lo
 #define AQL_TILE(BM, BN, WGM, WGN, ...) \
   hipLaunchKernelGGL((tile_kernel<BM, BN, WGM, WGN, __VA_ARGS__>), dim3((unsigned)(((M + BM - 1) / BM) * ((N + BN - 1) / BN))), dim3(WGM * WGN * 64), 0, stream, a)
     // Which tile (us without adapters, all tiles measured at each size): 256 x 320 where the width allows it and every CU gets one (4096 x 10240 x
-    // 1280: 99, 128 x 160 141, 128 x 128 141); else 128 rows by 160 or 128 columns, whichever needs less time for its rounds of two tiles per CU
-    // (9001 x 1280 x 1280: 37.7 with 128, 40.9 with 160), the former as 128 x 320 where that divides the width (16384 x 640 x 2560: 52.3 / 54.7;
-    // 32768 x 320 x 320: 13.0 / 16.1); smaller ones where those leave CUs idle (2048 x 1280 x 1280: 13.2 with 64 x 128, 14.8 with 128 x 128;
-    // 1001 x 640 x 768: 6.0 with 64 x 64, 6.6 with 64 x 128).  256 x 320 with requests of whole 256-row tiles: no tile meets two adapters, and the
-    // kernel need not find out (109 / 115 with rank 32).
+    // 1280: 99, 256 x 192 116, 128 x 320 142, 128 x 128 145).  Where 128 x 128 still gives every CU one: the least of rounds x time per round -- one
+    // 256 x 192 per CU, 29.5 us at K = 1280; one 128 x 320 (where that divides the width) or two 128 x 160, 29.2; two 128 x 128, 28.2, one 14.1
+    // (9001 x 1280 x 1280, in this order: 31.9, 50, 37.1; 16384 x 640 x 640: 19.4, 18.6, 21.0; 20480 x 640 x 640: 31.9, 31.2, 25.0; 32768 x 320 x 320 with 128 x
+    // 160: 16.1, 128 x 320: 13.0).  Smaller ones where those leave CUs idle (2048 x 1280 x 1280: 13.2 with 64 x 128, 14.8 with 128 x 128; 1001 x 640 x
+    // 768: 6.0 with 64 x 64, 6.6 with 64 x 128).  256 x 320 with requests of whole 256-row tiles: no tile meets two adapters, and the kernel need not
+    // find out (109 / 115 with rank 32).
     const auto tiles = [&](long bm, long bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
+    const long t192 = (tiles(256, 192) + 255) / 256 * 295, t160 = (tiles(128, 160) + 511) / 512 * 292, t128 = (tiles(128, 128) + 255) / 256 * 141;
     if (N % 320 == 0 && tiles(256, 320) >= 256 && (runs == 0 || unit % 256 == 0)) AQL_TILE(256, 320, 2, 4, 2, ONE);
     else if (N % 320 == 0 && tiles(256, 320) >= 256) AQL_TILE(256, 320, 2, 4, 2, FIND);
-    else if (tiles(128, 128) >= 256 && (tiles(128, 160) + 511) / 512 * 160 <= (tiles(128, 128) + 511) / 512 * 128) {
-      if (N % 320 == 0) AQL_TILE(128, 320, 2, 4, 2);
+    else if (tiles(128, 128) >= 256) {
+      if (t128 <= t160 && t128 <= t192) AQL_TILE(128, 128, 2, 4, 2);
+      else if (t192 < t160) AQL_TILE(256, 192, 4, 2, 2);
+      else if (N % 320 == 0) AQL_TILE(128, 320, 2, 4, 2);
       else AQL_TILE(128, 160, 2, 2, 2);
     }
-    else if (tiles(128, 128) >= 256) AQL_TILE(128, 128, 2, 4, 2);
     else if (tiles(64, 128) >= 256) AQL_TILE(64, 128, 2, 4, 3);
     else AQL_TILE(64, 64, 2, 2, 3);
 #undef AQL_TILE

@@ -35,6 +35,7 @@ CASES = {
     "whole_wide_tiles": ((8, 16384), [1, 0, -1, 2, 2, 0, 1, -1], 72, 1280, 24),
     "columns_of_160": ([13000, 8700], [1, 0], 64, 480, 72),
     "columns_of_320": ([20000, 12700], [1, 0], 64, 320, 72),
+    "columns_of_192": ([4000, 1, 3500, 1500], [1, 0, 2, 1], 72, 1280, 24),
     "two_rounds": ([20000, 13000], [1, 0], 64, 320, 72),
     "neighbours_of_one_adapter": ([16, 16, 16, 300], [1, 1, 0, 0], 64, 64, 12),
     "many_rows_many_adapters": ([1] * 300, [(7 * i) % 40 for i in range(300)], 320, 640, 16),

@@ -24,6 +24,7 @@ class AdapterBank:
     have changed (ops.adapter_linear calls it; writes through ``.data``, and an optimizer step inside a captured graph, need
     ``refresh(force=True)`` behind them)."""
 
+    @torch.inference_mode(False)
     def __init__(self, down, up, ranks=None, scales=None, trainable=False, device="cuda"):
         dev = torch.device(device)
         if dev.type != "cuda":
@@ -57,10 +58,14 @@ class AdapterBank:
             self.down = nn.Parameter(down.detach().to(device=dev, dtype=torch.float32, copy=True))
             self.up = nn.Parameter(up.detach().to(device=dev, dtype=torch.float32, copy=True))
         else:
-            self.down, self.up = down.detach().to(dev), up.detach().to(dev)
+            # (a copy of an inference tensor: `refresh` goes by version counters)
+            self.down, self.up = (t.detach().to(dev, copy=t.is_inference()) for t in (down, up))
         self.refresh()
         if trainable:
             self.lay_out_transposed()
+
+    def __reduce__(self):                    # copied and pickled by what it was made from (a U-Net that carries banks can be, too)
+        return AdapterBank, (self.down.detach(), self.up.detach(), self.ranks, self.scales, self.trainable, str(self.device))
 
     @classmethod
     def from_layers(cls, layers, trainable=False, device="cuda"):
@@ -124,8 +129,9 @@ class RequestPlan:
             raise ValueError("RequestPlan: adapters are numbered from 0; -1 is none")
         self.equal = lengths is None
         self.adapters, self.device = [int(a) for a in ids], dev
+        self.lengths = None if self.equal else [int(x) for x in lengths]
         self.requests = int(ids.size)
-        n = np.ones(ids.size, dtype=np.int64) if self.equal else np.asarray([int(x) for x in lengths], dtype=np.int64)
+        n = np.ones(ids.size, dtype=np.int64) if self.equal else np.asarray(self.lengths, dtype=np.int64)
         if n.size != ids.size or (n.size and n.min() < 0):
             raise ValueError("RequestPlan: one length of 0 or more for each request")
         if int(n.sum()) >= (1 << 31) - 256:
@@ -157,3 +163,6 @@ class RequestPlan:
         h.equal, h.max_id = self.equal, self.max_id
         h.nseg = int(seg.size) if self.max_id >= 0 else 0              # no adapters at all: no segments
         h.nused, h.nslot = int(used.size), int(slot.size)
+
+    def __reduce__(self):
+        return RequestPlan, (self.adapters, self.lengths, str(self.device))

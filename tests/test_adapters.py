@@ -3,7 +3,9 @@
 Tolerances.  u = 2^-24.  A dot product of n terms in fp32, in whatever order, is off by at most n u sum|terms|.  T (and dT) enters the product with
 B (A) as bf16: half a step, 2^-8 relative.  The output is rounded to bf16 once: 2^-8 of its value.  dA and dB are fp32 sums of products with
 T (dT) split into three bf16 parts that hold 24 bits (u relative)."""
+import copy
 import os
+import pickle
 import shutil
 import subprocess
 import sys
@@ -436,6 +438,42 @@ def test_two_threads_with_one_bank_and_one_plan():
     assert not errors, errors
     for a, b in zip(want, got):
         assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+@gpu
+@pytest.mark.parametrize("trainable", [False, True])
+def test_banks_and_plans_are_copied_and_pickled(trainable):
+    d, lengths, rows, ids, equal = make("ragged", 12)
+    packed, bank, plan = handles(d, lengths, ids, equal, trainable)
+    x = d["x"].to(DEV)
+    with torch.no_grad():
+        want = ops.adapter_linear(x, packed, bank, plan)
+        for b, p in ((copy.deepcopy(bank), copy.deepcopy(plan)), (pickle.loads(pickle.dumps(bank)), pickle.loads(pickle.dumps(plan)))):
+            assert b.down is not bank.down and b.down.data_ptr() != bank.down.data_ptr() and len(b.parameters()) == len(bank.parameters())
+            assert torch.equal(ops.adapter_linear(x, packed, b, p), want)
+
+
+@gpu
+def test_inference_mode():
+    d, lengths, rows, ids, equal = make("ragged", 13)
+    packed, bank, plan = handles(d, lengths, ids, equal, False)
+    x = d["x"].to(DEV)
+    gamma = torch.ones(x.shape[1], device=DEV, requires_grad=True)
+    with torch.no_grad():
+        want, norm = ops.adapter_linear(x, packed, bank, plan), ops.layernorm_train(x, gamma)
+    for trainable in (False, True):
+        with torch.inference_mode():
+            xi = d["x"].to(DEV)
+            _, bank, plan = handles({k: v.clone() if torch.is_tensor(v) else v for k, v in d.items()}, lengths, ids, equal, trainable)
+            moved = adapters.AdapterBank(d["down"].to(DEV), d["up"].to(DEV), ranks=d["ranks"], scales=d["scales"])
+            for b in (bank, moved):
+                assert torch.equal(ops.adapter_linear(xi, packed, b, plan), want)
+            for ckpt8 in (False, True):
+                y, skip = ops.layernorm_train_res(xi, gamma, ckpt8=ckpt8)
+                assert torch.equal(y, norm) and torch.equal(skip, xi)
+            assert torch.equal(ops.act8_pack(xi).unpack(), ops.act8_pack(x).unpack())
+    y = ops.adapter_linear(x, packed, bank, plan)               # a bank made there trains outside
+    torch.autograd.grad(y, bank.parameters(), d["dy"].to(DEV))
 
 
 @gpu

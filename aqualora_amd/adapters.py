@@ -53,13 +53,13 @@ class AdapterBank:
         h.a = torch.zeros(self.G, self.R, self.K, dtype=torch.bfloat16, device=dev)
         h.b = torch.zeros(self.G, self.N, self.R, dtype=torch.bfloat16, device=dev)
         self._transposed, self._lock = False, threading.Lock()
-        self._ver = None
         if trainable:
             self.down = nn.Parameter(down.detach().to(device=dev, dtype=torch.float32, copy=True))
             self.up = nn.Parameter(up.detach().to(device=dev, dtype=torch.float32, copy=True))
         else:
             # (a copy of an inference tensor: `refresh` goes by version counters)
             self.down, self.up = (t.detach().to(dev, copy=t.is_inference()) for t in (down, up))
+        h.down, h.up = self.down, self.up
         self.refresh()
         if trainable:
             self.lay_out_transposed()
@@ -86,17 +86,16 @@ class AdapterBank:
         return [self.down, self.up] if self.trainable else []
 
     def refresh(self, force=False):
-        ver = (self.down._version, self.up._version)
-        if ver == self._ver and not force:
-            return
         h, r, live = self.handle, self.rank, self._live
+        if h.fresh() and not force:
+            return
         with torch.no_grad():                # in place: a captured graph keeps reading these buffers
             h.a[:, :r].copy_(torch.where(live[:, :, None], self.down, torch.zeros((), dtype=self.down.dtype, device=self.device)))
             h.b[:, :, :r].copy_(torch.where(live[:, None, :], self.up, torch.zeros((), dtype=self.up.dtype, device=self.device)))
             if self._transposed:
                 h.at.copy_(h.a.transpose(1, 2))
                 h.bt.copy_(h.b.transpose(1, 2))
-        self._ver = ver
+        h.seen()
         h.serial += 1                        # a backward pass refuses weights that changed since its forward pass
 
     def lay_out_transposed(self):

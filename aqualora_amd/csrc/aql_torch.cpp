@@ -258,8 +258,13 @@ py::object layernorm_train(const Tensor& x, const Tensor& gamma, const std::opti
 // ------------------------------------------------------------------------------------------------------- adapters of many requests
 struct Bank {   // the device side of adapters.AdapterBank
   Tensor a, b, at, bt, ranks, scales;
+  Tensor down, up;              // what a .. bt are laid out from, and its versions then
+  int64_t down_seen = -1, up_seen = -1;
   long G = 0, r = 0, R = 0, K = 0, N = 0, serial = 0;
   bool trainable = false;
+
+  void seen() { down_seen = down._version(), up_seen = up._version(); }
+  bool fresh() const { return (int64_t)down._version() == down_seen && (int64_t)up._version() == up_seen; }
 };
 
 struct Plan {   // the device side of adapters.RequestPlan
@@ -402,9 +407,11 @@ struct AdapterLinear : torch::autograd::Function<AdapterLinear> {
   }
 };
 
-Tensor adapter_linear(const Tensor& x, const Tensor& w, const Tensor& wt, const std::optional<Tensor>& bias_, const std::shared_ptr<Bank>& bank,
-                      const std::shared_ptr<Plan>& plan, const Tensor& down, const Tensor& up,
-                      const std::optional<Tensor>& residual_, bool ckpt8) {
+// -> y, or nothing where the bank has to be laid out first
+std::optional<Tensor> adapter_linear(const Tensor& x, const Tensor& w, const Tensor& wt, const std::optional<Tensor>& bias_, const std::shared_ptr<Bank>& bank,
+                                     const std::shared_ptr<Plan>& plan, const std::optional<Tensor>& residual_, bool ckpt8) {
+  if (!bank->fresh() || (!bank->at.defined() && x.requires_grad() && at::GradMode::is_enabled())) return std::nullopt;
+  const Tensor &down = bank->down, &up = bank->up;
   const long N = w.size(0), K = w.size(1);
   if (x.dim() != 2 || x.scalar_type() != at::kBFloat16)
     bad_value("adapter_linear: expected bfloat16 [rows, " + std::to_string(K) + "], got " + c10::toString(x.scalar_type()) + " " + shape_of(x));
@@ -453,6 +460,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def(py::init<>())
       .def_readwrite("a", &Bank::a).def_readwrite("b", &Bank::b).def_readwrite("at", &Bank::at).def_readwrite("bt", &Bank::bt)
       .def_readwrite("ranks", &Bank::ranks).def_readwrite("scales", &Bank::scales)
+      .def_readwrite("down", &Bank::down).def_readwrite("up", &Bank::up).def("seen", &Bank::seen).def("fresh", &Bank::fresh)
       .def_readwrite("G", &Bank::G).def_readwrite("r", &Bank::r).def_readwrite("R", &Bank::R).def_readwrite("K", &Bank::K).def_readwrite("N", &Bank::N)
       .def_readwrite("serial", &Bank::serial).def_readwrite("trainable", &Bank::trainable);
   py::class_<Plan, std::shared_ptr<Plan>>(m, "Plan")

@@ -2073,10 +2073,14 @@ def adapter_linear(x2d, packed, bank, plan, residual=None, ckpt8=False):
     _plain(x2d, "adapter_linear")
     if residual is not None:
         _plain(residual, "adapter_linear")
-    bank.refresh()
-    if x2d.requires_grad and not bank.trainable and torch.is_grad_enabled():
-        bank.lay_out_transposed()
-    return L.native().adapter_linear(x2d, packed.w, packed.wt, packed.bias, bank.handle, plan.handle, bank.down, bank.up, residual, ckpt8)
+    args = x2d, packed.w, packed.wt, packed.bias, bank.handle, plan.handle, residual, ckpt8
+    y = L.native().adapter_linear(*args)
+    if y is None:                            # the bank's kernel copies do not fit the call yet: other weights, or a first input gradient
+        bank.refresh()
+        if x2d.requires_grad and torch.is_grad_enabled():
+            bank.lay_out_transposed()
+        y = L.native().adapter_linear(*args)
+    return y
 
 
 class GegluFn(torch.autograd.Function):

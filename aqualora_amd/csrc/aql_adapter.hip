@@ -897,22 +897,19 @@ __global__ __launch_bounds__(256) void wgrad_reduce_kernel(const Grad da, const 
   else wgrad_sum<true, VEC>(db, R, r_out, ranks, o, blockIdx.x - blocks_a);
 }
 
-// positions per chunk: whole tiles of 64
-int wgrad_chunk(long rows, int C, int R) {
-  const long tiles = (long)((C + 127) / 128) * (R <= 32 ? 1 : (R + 63) / 64);
-  // at most 256 workgroups for one gradient, two for each CU for both (4096 x 640, rank 320, with the sum: 27.6 us; 288: 30.4, 384: 29.0, 192: 31.6)
-  long want = 256 / tiles;
-  if (want < 1) want = 1;
-  long ch = (rows + want - 1) / want;
-  ch = (ch + 63) / 64 * 64;
+// positions per chunk, of both gradients (K, N: 0 for one that is not asked for): whole tiles of 64, at most 512 workgroups, two for each CU (4096 x 640,
+// rank 320, with the sum: 27.6 us; 576: 30.4, 768: 29.0, 384: 31.6)
+int wgrad_chunk(long rows, int K, int N, int R) {
+  const long tiles = (long)((K + 127) / 128 + (N + 127) / 128) * (R <= 32 ? 1 : (R + 63) / 64);
+  const long want = tiles < 512 ? 512 / tiles : 1;
+  const long ch = ((rows + want - 1) / want + 63) / 64 * 64;
   return (int)(ch < 64 ? 64 : ch > (1 << 20) ? (1 << 20) : ch);
 }
 
-// partial sums of one gradient, in floats
-double wgrad_floats(long rows, int nused, int C, int R) {
+// partial sums of one gradient with C columns, in floats
+double wgrad_floats(long rows, int nused, int C, int R, int chunk) {
   if (rows <= 0 || nused <= 0 || C <= 0 || R <= 0) return 0;
-  const int ch = wgrad_chunk(rows, C, R);
-  return (double)((rows + ch - 1) / ch + nused - 1) * R * C;
+  return (double)((rows + chunk - 1) / chunk + nused - 1) * R * C;
 }
 
 // T by 64-row tiles where a tile rarely meets a second adapter (each costs another pass over its rows) and the tiles fill the chip, by 16-row tiles
@@ -1024,7 +1021,11 @@ extern "C" int aql_adapter_down(const bf16_t* X, long ldx, const uint8_t* codes,
 // fp32 elements of the workspace of aql_adapter_wgrad (rows: those that have an adapter; nused: adapters that have rows; K, N: 0 for a gradient that is
 // not asked for), or -1: more than 2^31 - 1
 extern "C" int aql_adapter_wgrad_scratch_floats(long rows, int nused, int K, int N, int R) {
-  const double n = wgrad_floats(rows, nused, K, R) + wgrad_floats(rows, nused, N, R);
+  if (K < 0) K = 0;
+  if (N < 0) N = 0;
+  if (K + N == 0) return 0;
+  const int ch = wgrad_chunk(rows, K, N, R);
+  const double n = wgrad_floats(rows, nused, K, R, ch) + wgrad_floats(rows, nused, N, R, ch);
   return n < 2147483647.0 ? (int)n : -1;
 }
 
@@ -1046,18 +1047,18 @@ extern "C" int aql_adapter_wgrad(const bf16_t* dT, const bf16_t* X, long ldx, co
   uint32_t L = 0;   // 2^L >= unit: magic = floor(2^(31 + L) / unit) + 1 < 2^32, and the quotient is exact below 2^31
   while (rows && (1L << L) < unit) ++L;
   const Order o{perm, used_pos, slot, nused, rows ? nslot : 0, unit, rows ? (uint32_t)((1UL << (31 + L)) / (uint32_t)unit + 1) : 0u, L, rows};
-  const int rb = R <= 32 ? 32 : 64, tr = (R + rb - 1) / rb;
+  const int rb = R <= 32 ? 32 : 64, tr = (R + rb - 1) / rb, chunk = wgrad_chunk(rows, K, N, R);
   const auto job = [&](const bf16_t* U, const bf16_t* V, long ldv, int C, float* part, float* out) {
     Grad g{U, V, nullptr, nullptr, ldv, C, 64, 0, part, out};
     if (C && rows) {
-      g.chunk = wgrad_chunk(rows, C, R);
+      g.chunk = chunk;
       g.blocks = (int)((rows + g.chunk - 1) / g.chunk) * ((C + 127) / 128) * tr;
     }
     return g;
   };
   Grad a = job(dT, X, ldx, K, scratch, dA);
   a.codes = codes, a.exps = exps;
-  const Grad b = job(T, dY, lddy, N, scratch + (long)wgrad_floats(rows, nused, K, R), dB);
+  const Grad b = job(T, dY, lddy, N, scratch + (long)wgrad_floats(rows, nused, K, R, chunk), dB);
   if (rows) {
     const dim3 grid(a.blocks + b.blocks);
     if (R <= 32) {

@@ -549,6 +549,8 @@ def test_refusals_without_a_gpu():
     need = lib.aql_adapter_wgrad_scratch_floats(64, 2, 64, 64, 8)
     assert need > 0 and lib.aql_adapter_wgrad_scratch_floats(1 << 30, 60000, 1 << 14, 1 << 14, 1024) == -1
     assert 0 < lib.aql_adapter_wgrad_scratch_floats(64, 2, 64, 0, 8) < need
+    assert lib.aql_adapter_wgrad_scratch_floats(64, 2, -128, 64, 8) == lib.aql_adapter_wgrad_scratch_floats(64, 2, 0, 64, 8) > 0
+    assert lib.aql_adapter_wgrad_scratch_floats(64, 2, -5, -1, 8) == 0 == lib.aql_adapter_wgrad_scratch_floats(0, 0, 64, 64, 8)
 
     def wgrad(X=p, codes=None, r=8, rows=64, n=need, G=3, K=64, unit=1, dA=p, dB=p, dY=p, dT=p):
         return lib.aql_adapter_wgrad(dT, X, 64, codes, codes, K, dA, p, dY, 64, 64, dB, 64, G, 8, r, p, p, p, p, 2, 3, unit, rows, p, n, None)

@@ -980,19 +980,21 @@ extern "C" int aql_adapter_linear(const bf16_t* X, long ldx, const bf16_t* W, lo
   hipLaunchKernelGGL((tile_kernel<BM, BN, WGM, WGN, __VA_ARGS__>), dim3((unsigned)(((M + BM - 1) / BM) * ((N + BN - 1) / BN))), dim3(WGM * WGN * 64), 0, stream, a)
     // Which tile (us without adapters, all tiles measured at each size): 256 x 320 where the width allows it and every CU gets one (4096 x 10240 x
     // 1280: 99, 256 x 192 116, 128 x 320 142, 128 x 128 145).  Where 128 x 128 still gives every CU one: the least of rounds x time per round -- one
-    // 256 x 192 per CU, 29.5 us at K = 1280; one 128 x 320 (where that divides the width) or two 128 x 160, 29.2; two 128 x 128, 28.2, one 14.1
-    // (9001 x 1280 x 1280, in this order: 31.9, 50, 37.1; 16384 x 640 x 640: 19.4, 18.6, 21.0; 20480 x 640 x 640: 31.9, 31.2, 25.0; 32768 x 320 x 320 with 128 x
-    // 160: 16.1, 128 x 320: 13.0).  Smaller ones where those leave CUs idle (2048 x 1280 x 1280: 13.2 with 64 x 128, 14.8 with 128 x 128; 1001 x 640 x
-    // 768: 6.0 with 64 x 64, 6.6 with 64 x 128; both launches of 300 x 1280 x 5120: 31.3 with 64 x 32, 37.5 with 64 x 64).  256 x 320 with requests of
-    // whole 256-row tiles: no tile meets two adapters, and the kernel need not find out (109 / 115 with rank 32).
+    // 256 x 192 per CU, 29.5 us at K = 1280; one 128 x 320 (where that divides the width) or two 128 x 160, 29.2, a single 128 x 160, 19.8; two 128 x 128,
+    // 28.2, one 14.1 (9001 x 1280 x 1280 with 256 x 192, 128 x 320, 128 x 128: 31.9, 50, 37.1; 16384 x 640 x 640: 19.4, 18.6, 21.0; 20480 x 640 x 640: 31.9,
+    // 31.2, 25.0; 32768 x 320 x 320 with 128 x 160: 16.1, 128 x 320: 13.0; 4096 x 1280 x 1280 with 128 x 160: 19.8, 128 x 128: 21.5).  Smaller ones where
+    // those leave CUs idle (2048 x 1280 x 1280: 13.2 with 64 x 128, 14.8 with 128 x 128; 1001 x 640 x 768: 6.0 with 64 x 64, 6.6 with 64 x 128; both
+    // launches of 300 x 1280 x 5120: 31.3 with 64 x 32, 37.5 with 64 x 64).  256 x 320 with requests of whole 256-row tiles: no tile meets two
+    // adapters, and the kernel need not find out (109 / 115 with rank 32).
     const auto tiles = [&](long bm, long bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
-    const long t192 = (tiles(256, 192) + 255) / 256 * 295, t160 = (tiles(128, 160) + 511) / 512 * 292, t128 = (tiles(128, 128) + 255) / 256 * 141;
+    const long t192 = (tiles(256, 192) + 255) / 256 * 295, t160 = tiles(128, 160) <= 256 ? 198 : (tiles(128, 160) + 511) / 512 * 292;
+    const long t128 = (tiles(128, 128) + 255) / 256 * 141;
     if (N % 320 == 0 && tiles(256, 320) >= 256 && (runs == 0 || unit % 256 == 0)) AQL_TILE(256, 320, 2, 4, 2, ONE);
     else if (N % 320 == 0 && tiles(256, 320) >= 256) AQL_TILE(256, 320, 2, 4, 2, FIND);
     else if (tiles(128, 128) >= 256) {
       if (t128 <= t160 && t128 <= t192) AQL_TILE(128, 128, 2, 4, 2);
       else if (t192 < t160) AQL_TILE(256, 192, 4, 2, 2);
-      else if (N % 320 == 0) AQL_TILE(128, 320, 2, 4, 2);
+      else if (N % 320 == 0 && tiles(128, 160) > 256) AQL_TILE(128, 320, 2, 4, 2);
       else AQL_TILE(128, 160, 2, 2, 2);
     }
     else if (tiles(64, 128) >= 256) AQL_TILE(64, 128, 2, 4, 3);

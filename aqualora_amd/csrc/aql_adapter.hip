@@ -912,23 +912,24 @@ double wgrad_floats(long rows, int nused, int C, int R, int chunk) {
   return (double)((rows + chunk - 1) / chunk + nused - 1) * R * C;
 }
 
-// T by 64-row tiles where a tile rarely meets a second adapter (each costs another pass over its rows) and the tiles fill the chip, by 16-row tiles
-// otherwise.  Measured (us, 64-row / 16-row tiles): 32768 x 320, rank 32: 5.3 / 9.8; 9001 x 1280, rank 64: 10.0 / 19.9; 4096 x 640, rank 320:
-// 7.6 / 17.6; 4096 x 1280, rank 32 (64 tiles): 6.9 / 6.0; 1001 x 768, rank 64 (16 tiles): 6.7 / 6.3; 1000 x 2560, rank 32 (16 tiles): 10.7 / 9.0.
+// T by 64-row tiles where a tile rarely meets a second adapter (each costs another pass over its rows) and the tiles fill the chip or 16-row tiles are more
+// than one for each CU, by 16-row tiles otherwise.  Measured (us, 64-row / 16-row tiles): 32768 x 320, rank 32: 5.3 / 9.8; 9001 x 1280, rank 64: 10.0 /
+// 19.9; 4096 x 640, rank 320: 7.6 / 17.6; 4096 x 1280, rank 32 (64 tiles): 6.9 / 6.0; 1001 x 768, rank 64 (16 tiles): 6.7 / 6.3; 1000 x 2560, rank 32 (16
+// tiles): 10.7 / 9.0; with the second launch 4678 x 1896, rank 64 (74 tiles, 293 16-row workgroups): 21.1 / 32.6; 1000 x 640, rank 320 (80, 315): 10.9 / 16.6.
 void launch_down(const DownArgs& a, int runs, int slots, hipStream_t st) {
   const long tiles = (a.M + 63) / 64 * (a.R <= 32 ? 1 : (a.R + 63) / 64);
-  if (a.M / runs >= 64 && tiles >= 96) {
+  const int t16 = (a.R + 15) / 16;
+  // few workgroups: fewer adapter rows each, so that more CUs share the loads (8 x 1280, rank 32: 3.8 us with 16 rows, 5.0 with 32; 64 x 1280, rank 64:
+  // 4.3 / 5.5 / 8.0 with 16 / 32 / 64); many: more, so that X is read less often (9001 x 1280 codes, rank 64: 30 / 23 / 20)
+  const long b16 = (a.M + 15) / 16 * t16;
+  const int rt = t16 == 1 || b16 <= 256 ? 1 : t16 == 2 || b16 <= 512 ? 2 : 4;
+  if (a.M / runs >= 64 && (tiles >= 96 || (a.M + 15) / 16 * ((t16 + rt - 1) / rt) > 256)) {
     if (a.codes && a.R <= 32) hipLaunchKernelGGL((down8_tile_kernel<32>), dim3((unsigned)tiles, 2), dim3(256), 0, st, a);
     else if (a.codes) hipLaunchKernelGGL((down8_tile_kernel<64>), dim3((unsigned)tiles, 2), dim3(256), 0, st, a);
     else if (a.R <= 32) hipLaunchKernelGGL((down_tile_kernel<32, 4>), dim3((unsigned)tiles, 2), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((down_tile_kernel<64, 4>), dim3((unsigned)tiles, 2), dim3(256), 0, st, a);
     return;
   }
-  const int t16 = (a.R + 15) / 16;
-  // few workgroups: fewer adapter rows each, so that more CUs share the loads (8 x 1280, rank 32: 3.8 us with 16 rows, 5.0 with 32; 64 x 1280, rank 64:
-  // 4.3 / 5.5 / 8.0 with 16 / 32 / 64); many: more, so that X is read less often (9001 x 1280 codes, rank 64: 30 / 23 / 20)
-  const long b16 = (a.M + 15) / 16 * t16;
-  const int rt = t16 == 1 || b16 <= 256 ? 1 : t16 == 2 || b16 <= 512 ? 2 : 4;
   const dim3 grid((unsigned)((a.M + 15) / 16), slots, (t16 + rt - 1) / rt);
 #define AQL_DOWN(RT)                                                                          \
   do {                                                                                        \

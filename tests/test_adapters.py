@@ -43,6 +43,7 @@ CASES = {
     "many_rows_many_adapters": ([1] * 300, [(7 * i) % 40 for i in range(300)], 320, 640, 16),
     "wide_few_rows": ([60, 4], [1, 0], 72, 10240, 24),
     "few_tiles": ([200, 1, 99], [1, 2, 0], 200, 1280, 24),
+    "few_tiles_of_t": ([3000, 1001, 677], [1, 0, 2], 136, 160, 64),
     "no_adapters": ([3, 270], [-1, -1], 64, 72, 8),
 }
 

@@ -446,8 +446,10 @@ __device__ __forceinline__ bool tile_body(const LinArgs& a, char* lds, long m0, 
       g = next_adapter<BM>(ids, g, lane);
       left = g < 0 ? 1 << 30 : rk;
       if (g >= 0) {
-        sx.begin(a.T + m0 * a.P * a.R, (long)a.P * a.R, a.R, tid, [&](int r) { return ids[r] == g; });
-        sw.begin(a.B + ((long)g * a.N + n0) * a.R, a.R, a.R, tid, [&](int r) { return r < nlive; });
+        int t2 = tid;
+        asm volatile("" : "+v"(t2));   // (made anew, as in products)
+        sx.begin(a.T + m0 * a.P * a.R, (long)a.P * a.R, a.R, t2, [&](int r) { return ids[r] == g; });
+        sw.begin(a.B + ((long)g * a.N + n0) * a.R, a.R, a.R, t2, [&](int r) { return r < nlive; });
       }
     }
     --left;
@@ -491,19 +493,22 @@ __device__ __forceinline__ bool tile_body(const LinArgs& a, char* lds, long m0, 
     for (int t = 0; t < n; ++t) products<BM, BN, WGM, WGN, true>(ring.turn(issue), wave, lane, acc);
   }
   ring.drain();
+  int l2 = lane;
+  asm volatile("" : "+v"(l2));   // (what the stores need is made anew: kept over the loops it would spill)
+  const int i2 = l2 & 15, q2 = l2 >> 4;
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
-    const long m = w0 + i * 16 + i16;
+    const long m = w0 + i * 16 + i2;
     if (m >= a.M) continue;
 #pragma unroll
     for (int p = 0; p < FP; ++p) {
-      const int n = v0 + p * 32 + q * 8;
+      const int n = v0 + p * 32 + q2 * 8;
       if (n >= a.N) continue;
       const f32x4_t v = acc[i][2 * p], w = acc[i][2 * p + 1];
       *reinterpret_cast<uint4*>(a.Y + m * a.ldy + n) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3]));
     }
     if constexpr (FO) {
-      const int n = v0 + FP * 32 + q * 4;
+      const int n = v0 + FP * 32 + q2 * 4;
       if (n >= a.N) continue;
       const f32x4_t v = acc[i][FN - 1];
       *reinterpret_cast<uint2*>(a.Y + m * a.ldy + n) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
@@ -924,10 +929,11 @@ void launch_down(const DownArgs& a, int runs, int slots, hipStream_t st) {
   const long b16 = (a.M + 15) / 16 * t16;
   const int rt = t16 == 1 || b16 <= 256 ? 1 : t16 == 2 || b16 <= 512 ? 2 : 4;
   if (a.M / runs >= 64 && (tiles >= 96 || (a.M + 15) / 16 * ((t16 + rt - 1) / rt) > 256)) {
-    if (a.codes && a.R <= 32) hipLaunchKernelGGL((down8_tile_kernel<32>), dim3((unsigned)tiles, 2), dim3(256), 0, st, a);
-    else if (a.codes) hipLaunchKernelGGL((down8_tile_kernel<64>), dim3((unsigned)tiles, 2), dim3(256), 0, st, a);
-    else if (a.R <= 32) hipLaunchKernelGGL((down_tile_kernel<32, 4>), dim3((unsigned)tiles, 2), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((down_tile_kernel<64, 4>), dim3((unsigned)tiles, 2), dim3(256), 0, st, a);
+    const dim3 grid((unsigned)tiles, a.rows.unit % 64 ? 2 : 1);   // whole tiles of one adapter need no second workgroup
+    if (a.codes && a.R <= 32) hipLaunchKernelGGL((down8_tile_kernel<32>), grid, dim3(256), 0, st, a);
+    else if (a.codes) hipLaunchKernelGGL((down8_tile_kernel<64>), grid, dim3(256), 0, st, a);
+    else if (a.R <= 32) hipLaunchKernelGGL((down_tile_kernel<32, 4>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((down_tile_kernel<64, 4>), grid, dim3(256), 0, st, a);
     return;
   }
   const dim3 grid((unsigned)((a.M + 15) / 16), slots, (t16 + rt - 1) / rt);

@@ -1,5 +1,6 @@
 // 8-bit activation checkpoints (format: aql_act8.cuh): codes int8 [M][Cp], exponent bytes [M][Cp / 32], Cp = C rounded up to 32.
-// Both kernels are one pass over the data, bound by HBM: a thread takes 8 columns, a quad of lanes one block of 32.
+// Both kernels are one pass over the data, bound by HBM: a thread takes 8 columns, a quad of lanes one block of 32 (65536 x 640 bf16: pack 20.8 us,
+// unpack 19.8 us, 6.1 and 6.4 TB/s of 127 MB that partly stay in the last-level cache; a copy of 2 GiB runs at 4.9).
 #include "aql_act8.cuh"
 
 using namespace act8;

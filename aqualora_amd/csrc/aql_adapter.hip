@@ -84,7 +84,7 @@ struct DownArgs {
   Rows rows;
 };
 
-// Few rows or short requests.  One workgroup: 16 rows x 16 RT adapter rows of ONE adapter (blockIdx.y counts the adapters that the row
+// Few rows or short requests: bound by the latency of row -> adapter -> loads (8 x 1280, rank 32: 4.0 us).  One workgroup: 16 rows x 16 RT adapter rows of ONE adapter (blockIdx.y counts the adapters that the row
 // tile meets); its NW wavefronts split the contraction and join in LDS.  Fragments come straight from memory, four steps of 32 columns at a time
 // (all their loads in flight together): lane (i = lane & 15, q = lane >> 4) holds row i, columns k + 8 q .. k + 8 q + 7 of either operand, and
 // gets T[m = lane & 15][r = 4 q + e] back.
@@ -177,7 +177,8 @@ struct LinArgs {
 
 // ------------------------------------------------------------------------------------------- few rows: 16 x 16 NF tiles, split contraction
 // Eight wavefronts split the contraction of one tile (and the tile's (adapter, rank step) pairs) and join in LDS: with few rows the launch is
-// bound by the latency of the weight loads, so the loads of a tile are spread over as many wavefronts as it can feed and issued UN steps at a time.
+// bound by the latency of the weight loads, so the loads of a tile are spread over as many wavefronts as it can feed and issued UN steps at a time
+// (8 x 1280 x 1280, eight adapters: 5.3 us, 3.3 of them without adapters; 193 x 1280 x 320, 48 adapters: 8.0).
 template <int NF>
 __global__ __launch_bounds__(512) void skinny_kernel(const LinArgs a) {
   constexpr int UN = 4;
@@ -391,7 +392,9 @@ __device__ __forceinline__ bool one_adapter(const int* ids, int g, int live, int
 
 // WGM x WGN wavefronts, BM x BN outputs.  The low-rank term of each adapter that the tile meets goes through the same ring, behind the projection's
 // own columns: R further columns of the contraction, the adapter's rows of T against its B.  (Fragments of T and B
-// straight from memory instead cost a load latency per 32 columns of rank: 28 against 18 us at 4096 x 640 x 640, rank 320.)
+// straight from memory instead cost a load latency per 32 columns of rank: 28 against 18 us at 4096 x 640 x 640, rank 320.)  Large calls are bound by the
+// matrix cores and the LDS reads that feed them (4096 x 10240 x 1280, rank 32: 109 us, 1.0 PFLOP/s), small ones by the latency of their stages
+// (1001 x 640 x 768, rank 64: 8.6 us for 12 + 1 stages).
 // What the tile may meet: ANY adapters; ONE or none (the caller knows); or FIND out -- where it is not one or none, false comes back and nothing is written.
 enum Meets { ANY, ONE, FIND };
 template <int BM, int BN, int WGM, int WGN, int NSTG, Meets MEETS>
@@ -562,7 +565,8 @@ __device__ __forceinline__ void store_tile(const DownArgs& a, const f32x4_t (&ac
   }
 }
 
-// T = s A x for many rows of long requests: 64 rows x BN adapter rows per workgroup, once for each adapter that the rows meet (mostly one)
+// T = s A x for many rows of long requests: 64 rows x BN adapter rows per workgroup, once for each adapter that the rows meet (mostly one).  Bound by reading
+// X once per BN adapter rows (32768 x 2560, rank 32: 38.6 us, 4.4 TB/s; 32768 x 320: 5.7 us, 3.7 TB/s)
 template <int BN, int NSTG>
 __global__ __launch_bounds__(256) void down_tile_kernel(const DownArgs a) {
   constexpr int BM = 64, FM = 2, FN = BN / 32, STAGE = (BM + BN) * 128;
@@ -706,7 +710,8 @@ __global__ __launch_bounds__(256) void down8_tile_kernel(const DownArgs a) {
 // The rows of all adapters in sorted order (adapter by adapter) are one axis of `rows` positions, cut into chunks of `chunk` positions.  A workgroup
 // takes one chunk x 128 columns of V x RB columns of U; where adapters change inside its chunk it finishes one and begins the next.  Piece
 // (chunk b, j-th used adapter) is partial sum b + j: along the axis every new piece raises b or j.  A second launch adds an adapter's partial
-// sums in their order: no atomics, the same bits every time.
+// sums in their order: no atomics, the same bits every time.  Bound by the latency of a tile's loads and LDS reads (4096 x 640 and 640, rank 320: 22.0 us, 460
+// TFLOP/s, and 5.2 for the sums).
 struct Order {
   const int* perm;       // [rows / unit] the unit of rows at each position of the axis, in units
   const int* used_pos;   // [nused + 1] first position of the j-th used adapter, in units

@@ -178,7 +178,7 @@ struct LinArgs {
 // ------------------------------------------------------------------------------------------- few rows: 16 x 16 NF tiles, split contraction
 // Eight wavefronts split the contraction of one tile (and the tile's (adapter, rank step) pairs) and join in LDS: with few rows the launch is
 // bound by the latency of the weight loads, so the loads of a tile are spread over as many wavefronts as it can feed and issued UN steps at a time
-// (8 x 1280 x 1280, eight adapters: 5.3 us, 3.3 of them without adapters; 193 x 1280 x 320, 48 adapters: 8.0).
+// (8 x 1280 x 1280, eight adapters: 5.3 us, a whole call without adapters 3.7; 193 x 1280 x 320, 48 adapters: 8.0).
 template <int NF>
 __global__ __launch_bounds__(512) void skinny_kernel(const LinArgs a) {
   constexpr int UN = 4;

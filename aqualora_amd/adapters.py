@@ -89,13 +89,14 @@ class AdapterBank:
         h, r, live = self.handle, self.rank, self._live
         if h.fresh() and not force:
             return
+        h.begin_layout()                     # behind the other streams' reads
         with torch.no_grad():                # in place: a captured graph keeps reading these buffers
             h.a[:, :r].copy_(torch.where(live[:, :, None], self.down, torch.zeros((), dtype=self.down.dtype, device=self.device)))
             h.b[:, :, :r].copy_(torch.where(live[:, None, :], self.up, torch.zeros((), dtype=self.up.dtype, device=self.device)))
             if self._transposed:
                 h.at.copy_(h.a.transpose(1, 2))
                 h.bt.copy_(h.b.transpose(1, 2))
-        h.seen()
+        h.end_layout()
         h.serial += 1                        # a backward pass refuses weights that changed since its forward pass
 
     def lay_out_transposed(self):
@@ -109,6 +110,7 @@ class AdapterBank:
             if self._transposed:
                 return
             h = self.handle
+            h.reads()
             h.at, h.bt = h.a.transpose(1, 2).contiguous(), h.b.transpose(1, 2).contiguous()
             torch.cuda.current_stream(self.device).synchronize()      # once: later calls may come on other streams
             self._transposed = True

@@ -64,6 +64,14 @@ void here(const Tensor& t, const char* name) {
 }
 aql_stream_t stream_of(const Tensor& t) { return (aql_stream_t)c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 
+void hip_ok(hipError_t e, const char* what) {
+  if (e != hipSuccess) throw AqlErr(std::string(what) + ": " + hipGetErrorString(e));
+}
+bool capturing(const c10::hip::HIPStream& s) {
+  hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+  return hipStreamIsCapturing(s.stream(), &cs) == hipSuccess && cs != hipStreamCaptureStatusNone;
+}
+
 // at::empty without the dispatcher's way to it: a backward pass allocates up to seven tensors
 Tensor fresh(at::IntArrayRef size, at::ScalarType type, const Tensor& like) { return at::detail::empty_cuda(size, type, like.device(), std::nullopt); }
 // two fp32 tensors in one allocation (a pair of gradients: they live and end together); an unwanted one stays undefined
@@ -111,8 +119,7 @@ Tensor leaf(const Tensor& t) { return t.defined() && t.is_leaf() && t.requires_g
 // the same leaf still lives) would draw that stream into the capture, which ends the process: refused instead.
 void leaves_ok(const std::vector<Tensor>& leaves, const Tensor& g, const char* name) {
   const auto here = c10::hip::getCurrentHIPStream(g.get_device());
-  hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-  if (hipStreamIsCapturing(here.stream(), &cs) != hipSuccess || cs == hipStreamCaptureStatusNone) return;
+  if (!capturing(here)) return;
   for (const Tensor& t : leaves) {
     if (!t.defined()) continue;
     const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
@@ -265,6 +272,57 @@ struct Bank {   // the device side of adapters.AdapterBank
 
   void seen() { down_seen = down._version(), up_seen = up._version(); }
   bool fresh() const { return (int64_t)down._version() == down_seen && (int64_t)up._version() == up_seen; }
+
+  // The stacks are written in place, by whichever stream calls first after a change, and read by all.  A stream's first read behind a layout waits for its event,
+  // and a layout waits for every stream that has read since the last one.  (What runs inside a graph is ordered by whoever replays it.)
+  std::optional<c10::hip::HIPStream> home;    // stream of the last layout
+  std::vector<c10::hip::HIPStream> readers;   // streams that have read since then
+  hipEvent_t laid = nullptr, mark = nullptr;  // behind the last layout; for one wait at a time
+  std::mutex guard;                           // of these: backward passes come from the engine's threads
+
+  Bank() = default;
+  Bank(const Bank&) = delete;
+  ~Bank() {
+    for (hipEvent_t e : {laid, mark})
+      if (e) (void)hipEventDestroy(e);
+  }
+  c10::hip::HIPStream current() const { return c10::hip::getCurrentHIPStream(a.get_device()); }
+  // ahead of kernels on the current stream that read the stacks
+  void reads() {
+    const auto s = current();
+    const std::lock_guard<std::mutex> lock(guard);
+    for (const auto& r : readers)
+      if (r == s) return;
+    if (capturing(s)) return;
+    if (home && *home != s) hip_ok(hipStreamWaitEvent(s.stream(), laid, 0), "AdapterBank");
+    readers.push_back(s);
+  }
+  // around the copies of a layout on the current stream
+  void begin_layout() {
+    const auto s = current();
+    if (capturing(s)) return;
+    const std::lock_guard<std::mutex> lock(guard);
+    const c10::DeviceGuard device(a.device());
+    for (hipEvent_t* e : {&laid, &mark})
+      if (!*e) hip_ok(hipEventCreateWithFlags(e, hipEventDisableTiming), "AdapterBank");
+    if (home && *home != s) hip_ok(hipStreamWaitEvent(s.stream(), laid, 0), "AdapterBank");
+    for (const auto& r : readers) {
+      if (r == s) continue;
+      if (capturing(r)) throw AqlErr("AdapterBank: changed weights cannot be laid out while a stream that has read the old ones is being captured");
+      hip_ok(hipEventRecord(mark, r.stream()), "AdapterBank");
+      hip_ok(hipStreamWaitEvent(s.stream(), mark, 0), "AdapterBank");
+    }
+  }
+  void end_layout() {
+    const auto s = current();
+    const std::lock_guard<std::mutex> lock(guard);
+    if (!capturing(s)) {
+      hip_ok(hipEventRecord(laid, s.stream()), "AdapterBank");
+      home = s;
+      readers.clear();
+    }
+    seen();
+  }
 };
 
 struct Plan {   // the device side of adapters.RequestPlan
@@ -390,6 +448,7 @@ struct AdapterLinear : torch::autograd::Function<AdapterLinear> {
         if (want_a) out[1] = at::zeros({bank.G, bank.r, bank.K}, bank.scales.options());
         if (want_b) out[2] = at::zeros({bank.G, bank.N, bank.r}, bank.scales.options());
       } else {
+        c->bank->reads();
         const Rows dy = gemm_rows(g[0]);
         Tensor dT, T = s[1];
         Rows x;
@@ -428,6 +487,7 @@ std::optional<Tensor> adapter_linear(const Tensor& x, const Tensor& w, const Ten
   here(x, "adapter_linear");
   if (bank->a.device() != x.device() || plan->table.device() != x.device() || w.device() != x.device() || (res.defined() && res.device() != x.device()))
     bad_value("adapter_linear: input, projection, adapters, plan and residual must live on one device");
+  bank->reads();
   const bool train = bank->trainable && at::GradMode::is_enabled() && (down.requires_grad() || up.requires_grad());
   if (at::GradMode::is_enabled() && (train || x.requires_grad() || (res.defined() && res.requires_grad()))) {
     auto c = c10::make_intrusive<Call>();
@@ -460,7 +520,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def(py::init<>())
       .def_readwrite("a", &Bank::a).def_readwrite("b", &Bank::b).def_readwrite("at", &Bank::at).def_readwrite("bt", &Bank::bt)
       .def_readwrite("ranks", &Bank::ranks).def_readwrite("scales", &Bank::scales)
-      .def_readwrite("down", &Bank::down).def_readwrite("up", &Bank::up).def("seen", &Bank::seen).def("fresh", &Bank::fresh)
+      .def_readwrite("down", &Bank::down).def_readwrite("up", &Bank::up).def("fresh", &Bank::fresh)
+      .def("reads", &Bank::reads).def("begin_layout", &Bank::begin_layout).def("end_layout", &Bank::end_layout)
       .def_readwrite("G", &Bank::G).def_readwrite("r", &Bank::r).def_readwrite("R", &Bank::R).def_readwrite("K", &Bank::K).def_readwrite("N", &Bank::N)
       .def_readwrite("serial", &Bank::serial).def_readwrite("trainable", &Bank::trainable);
   py::class_<Plan, std::shared_ptr<Plan>>(m, "Plan")

@@ -1,0 +1,89 @@
+"""What an AdapterBank keeps between calls -- the bf16 stacks that the kernels read -- under streams, threads, captures and optimizers: a call sees the
+parameters as they are, whoever laid the stacks out.  Comparisons are bit for bit with a bank that was made from the same weights."""
+import pytest
+import torch
+
+from aqualora_amd import adapters, ops
+
+DEV = "cuda"
+SLEEP = 50_000_000     # cycles: 20 ms or more, longer than the host needs for what is queued behind it
+gpu = pytest.mark.gpu
+
+
+class Site:
+    """A small projection with three adapters, and banks of two sets of weights."""
+
+    def __init__(self, seed=0):
+        gen = torch.Generator().manual_seed(seed)
+        rn = lambda *s: torch.randn(s, generator=gen)  # noqa: E731
+        K, N, r, G = 320, 256, 16, 3
+        bf = torch.bfloat16
+        self.packed = ops.PackedLinear(rn(N, K).to(DEV) / K ** 0.5, rn(N).to(DEV))
+        self.old, self.new = ((rn(G, r, K).to(bf).float() / r, (0.2 * rn(G, N, r)).to(bf).float()) for _ in range(2))
+        self.plan = adapters.RequestPlan([0, 2, -1, 1], [70, 1, 30, 99])
+        self.x, self.dy = rn(200, K).to(DEV, bf), rn(200, N).to(DEV, bf)
+
+    def bank(self, weights, trainable=True):
+        return adapters.AdapterBank(*weights, ranks=[16, 12, 16], scales=[1.0, 0.5, 1.25], trainable=trainable)
+
+    def call(self, bank):
+        return ops.adapter_linear(self.x, self.packed, bank, self.plan)
+
+    def step(self, bank):
+        x = self.x.detach().requires_grad_(True)
+        y = ops.adapter_linear(x, self.packed, bank, self.plan)
+        return (y.detach(),) + torch.autograd.grad(y, (x, bank.down, bank.up), self.dy)
+
+
+def put(bank, weights):
+    """An eager step of an optimizer."""
+    with torch.no_grad():
+        bank.down.copy_(weights[0])
+        bank.up.copy_(weights[1])
+
+
+def same(a, b):
+    return all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@gpu
+def test_other_streams_wait_for_a_layout():
+    """The parameters change, both streams are ordered behind that; one stream's call lays the bank out (late: its stream is busy), the other's call comes next."""
+    s = Site()
+    bank = s.bank(s.old)
+    want = s.step(s.bank(s.new))
+    new = [w.to(DEV) for w in s.new]
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    for first, second in ((one, two), (torch.cuda.current_stream(), one), (two, torch.cuda.current_stream())):
+        put(bank, [w.to(DEV) for w in s.old])
+        s.step(bank)
+        put(bank, new)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(first):
+            torch.cuda._sleep(SLEEP)
+            a = s.step(bank)
+        with torch.cuda.stream(second):
+            b = s.step(bank)
+        torch.cuda.synchronize()
+        assert same(a, want) and same(b, want)
+
+
+@gpu
+def test_a_layout_waits_for_the_streams_that_still_read():
+    """A stream is late with its pass over the old weights; another stream's call lays the new ones out."""
+    s = Site(1)
+    old, new = s.step(s.bank(s.old)), s.step(s.bank(s.new))
+    to = [w.to(DEV) for w in s.new]
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    for late, next_ in ((one, two), (torch.cuda.current_stream(), one), (one, torch.cuda.current_stream())):
+        bank = s.bank(s.old)
+        s.call(bank)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(late):
+            torch.cuda._sleep(SLEEP)
+            a = s.step(bank)
+        with torch.cuda.stream(next_):
+            put(bank, to)
+            b = s.step(bank)
+        torch.cuda.synchronize()
+        assert same(a, old) and same(b, new)

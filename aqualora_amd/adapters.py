@@ -89,15 +89,17 @@ class AdapterBank:
         h, r, live = self.handle, self.rank, self._live
         if h.fresh() and not force:
             return
-        h.begin_layout()                     # behind the other streams' reads
-        with torch.no_grad():                # in place: a captured graph keeps reading these buffers
-            h.a[:, :r].copy_(torch.where(live[:, :, None], self.down, torch.zeros((), dtype=self.down.dtype, device=self.device)))
-            h.b[:, :, :r].copy_(torch.where(live[:, None, :], self.up, torch.zeros((), dtype=self.up.dtype, device=self.device)))
-            if self._transposed:
-                h.at.copy_(h.a.transpose(1, 2))
-                h.bt.copy_(h.b.transpose(1, 2))
-        h.end_layout()
-        h.serial += 1                        # a backward pass refuses weights that changed since its forward pass
+        with self._lock:                     # of threads that come together the first lays out
+            if h.fresh() and not force:
+                return
+            h.begin_layout()                 # behind what other threads and streams still read; backward passes of older calls are refused from here on
+            with torch.no_grad():            # in place: a captured graph keeps reading these buffers
+                h.a[:, :r].copy_(torch.where(live[:, :, None], self.down, torch.zeros((), dtype=self.down.dtype, device=self.device)))
+                h.b[:, :, :r].copy_(torch.where(live[:, None, :], self.up, torch.zeros((), dtype=self.up.dtype, device=self.device)))
+                if self._transposed:
+                    h.at.copy_(h.a.transpose(1, 2))
+                    h.bt.copy_(h.b.transpose(1, 2))
+            h.end_layout()
 
     def lay_out_transposed(self):
         """B^T [G, R, N] and A^T [G, K, R], the stacks as the backward-data pass reads them: at once for a trainable bank, for others when an input

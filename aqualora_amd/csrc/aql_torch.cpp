@@ -13,6 +13,7 @@
 #include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPStream.h>
 
+#include <condition_variable>
 #include <cstdlib>
 #include <memory>
 #include <mutex>
@@ -267,18 +268,25 @@ struct Bank {   // the device side of adapters.AdapterBank
   Tensor a, b, at, bt, ranks, scales;
   Tensor down, up;              // what a .. bt are laid out from, and its versions then
   int64_t down_seen = -1, up_seen = -1;
-  long G = 0, r = 0, R = 0, K = 0, N = 0, serial = 0;
+  long G = 0, r = 0, R = 0, K = 0, N = 0;
   bool trainable = false;
 
-  void seen() { down_seen = down._version(), up_seen = up._version(); }
   bool fresh() const { return (int64_t)down._version() == down_seen && (int64_t)up._version() == up_seen; }
 
-  // The stacks are written in place, by whichever stream calls first after a change, and read by all.  A stream's first read behind a layout waits for its event,
-  // and a layout waits for every stream that has read since the last one.  (What runs inside a graph is ordered by whoever replays it.)
+  // The stacks are written in place, by whichever call comes first after a change, and read by all, from any thread and stream.
+  //   Threads: `busy` calls are queueing kernels that read the stacks; a layout begins by raising `serial` and making the stacks stale, so that no further call enters,
+  //   and then waits for the ones inside.  (A backward pass enters by the serial of its forward pass; the versions are noted ahead of the copies.)
+  //   Streams: the first read on a stream behind a layout waits for its event, and a layout waits for every stream that has read since the last one.
+  // (What runs inside a graph is ordered by whoever replays it.)
+  std::mutex guard;
+  std::condition_variable quiet;
+  int busy = 0;
+  long serial = 0;
+  static thread_local const Bank* inside;     // the bank that this thread is queueing reads of
+  int64_t down_next = -1, up_next = -1;       // versions that the layout in progress will have seen
   std::optional<c10::hip::HIPStream> home;    // stream of the last layout
   std::vector<c10::hip::HIPStream> readers;   // streams that have read since then
   hipEvent_t laid = nullptr, mark = nullptr;  // behind the last layout; for one wait at a time
-  std::mutex guard;                           // of these: backward passes come from the engine's threads
 
   Bank() = default;
   Bank(const Bank&) = delete;
@@ -287,21 +295,28 @@ struct Bank {   // the device side of adapters.AdapterBank
       if (e) (void)hipEventDestroy(e);
   }
   c10::hip::HIPStream current() const { return c10::hip::getCurrentHIPStream(a.get_device()); }
-  // ahead of kernels on the current stream that read the stacks
-  void reads() {
-    const auto s = current();
-    const std::lock_guard<std::mutex> lock(guard);
+  // ahead of kernels on the current stream that read the stacks (guard held)
+  void read_on(const c10::hip::HIPStream& s) {
     for (const auto& r : readers)
       if (r == s) return;
     if (capturing(s)) return;
     if (home && *home != s) hip_ok(hipStreamWaitEvent(s.stream(), laid, 0), "AdapterBank");
     readers.push_back(s);
   }
-  // around the copies of a layout on the current stream
+  void reads() {
+    const std::lock_guard<std::mutex> lock(guard);
+    read_on(current());
+  }
+  // around the copies of a layout on the current stream; one at a time (adapters.AdapterBank sees to that)
   void begin_layout() {
     const auto s = current();
+    if (inside == this) throw AqlErr("AdapterBank: changed weights cannot be laid out from inside a call that uses the bank (a hook of its saved tensors)");
+    std::unique_lock<std::mutex> lock(guard);
+    down_next = down._version(), up_next = up._version();
+    down_seen = up_seen = -1;
+    ++serial;
+    quiet.wait(lock, [&] { return busy == 0; });
     if (capturing(s)) return;
-    const std::lock_guard<std::mutex> lock(guard);
     const c10::DeviceGuard device(a.device());
     for (hipEvent_t* e : {&laid, &mark})
       if (!*e) hip_ok(hipEventCreateWithFlags(e, hipEventDisableTiming), "AdapterBank");
@@ -321,7 +336,33 @@ struct Bank {   // the device side of adapters.AdapterBank
       home = s;
       readers.clear();
     }
-    seen();
+    down_seen = down_next, up_seen = up_next;
+  }
+};
+
+thread_local const Bank* Bank::inside = nullptr;
+
+// a call that queues kernels which read the stacks on the current stream; `in` is false where they are not what the call needs
+struct Reading {
+  Bank& bank;
+  bool in;
+  long serial;
+  const Bank* outer = Bank::inside;
+  explicit Reading(Bank& b, long want = -1) : bank(b) {   // want: the serial that the stacks must have (-1: that of the parameters' versions)
+    const std::lock_guard<std::mutex> lock(b.guard);
+    in = want < 0 ? b.fresh() : b.serial == want;
+    serial = b.serial;
+    if (!in) return;
+    b.read_on(b.current());
+    ++b.busy;
+    Bank::inside = &b;
+  }
+  Reading(const Reading&) = delete;
+  ~Reading() {
+    if (!in) return;
+    Bank::inside = outer;
+    const std::lock_guard<std::mutex> lock(bank.guard);
+    if (--bank.busy == 0) bank.quiet.notify_all();
   }
 };
 
@@ -440,7 +481,8 @@ struct AdapterLinear : torch::autograd::Function<AdapterLinear> {
     if (!g[0].defined()) return out;
     here(g[0], "adapter_linear backward");
     leaves_ok(c->leaves, g[0], "adapter_linear");
-    if (bank.serial != c->serial) throw AqlErr("adapter_linear: the bank's weights changed between the forward pass and its backward pass");
+    const Reading reading(*c->bank, c->serial);
+    if (!reading.in) throw AqlErr("adapter_linear: the bank's weights changed between the forward pass and its backward pass");
     {
       at::AutoGradMode off(false);
       if (c->M == 0) {
@@ -448,7 +490,6 @@ struct AdapterLinear : torch::autograd::Function<AdapterLinear> {
         if (want_a) out[1] = at::zeros({bank.G, bank.r, bank.K}, bank.scales.options());
         if (want_b) out[2] = at::zeros({bank.G, bank.N, bank.r}, bank.scales.options());
       } else {
-        c->bank->reads();
         const Rows dy = gemm_rows(g[0]);
         Tensor dT, T = s[1];
         Rows x;
@@ -469,7 +510,7 @@ struct AdapterLinear : torch::autograd::Function<AdapterLinear> {
 // -> y, or nothing where the bank has to be laid out first
 std::optional<Tensor> adapter_linear(const Tensor& x, const Tensor& w, const Tensor& wt, const std::optional<Tensor>& bias_, const std::shared_ptr<Bank>& bank,
                                      const std::shared_ptr<Plan>& plan, const std::optional<Tensor>& residual_, bool ckpt8) {
-  if (!bank->fresh() || (!bank->at.defined() && x.requires_grad() && at::GradMode::is_enabled())) return std::nullopt;
+  if (!bank->at.defined() && x.requires_grad() && at::GradMode::is_enabled()) return std::nullopt;
   const Tensor &down = bank->down, &up = bank->up;
   const long N = w.size(0), K = w.size(1);
   if (x.dim() != 2 || x.scalar_type() != at::kBFloat16)
@@ -487,11 +528,12 @@ std::optional<Tensor> adapter_linear(const Tensor& x, const Tensor& w, const Ten
   here(x, "adapter_linear");
   if (bank->a.device() != x.device() || plan->table.device() != x.device() || w.device() != x.device() || (res.defined() && res.device() != x.device()))
     bad_value("adapter_linear: input, projection, adapters, plan and residual must live on one device");
-  bank->reads();
+  const Reading reading(*bank);
+  if (!reading.in) return std::nullopt;
   const bool train = bank->trainable && at::GradMode::is_enabled() && (down.requires_grad() || up.requires_grad());
   if (at::GradMode::is_enabled() && (train || x.requires_grad() || (res.defined() && res.requires_grad()))) {
     auto c = c10::make_intrusive<Call>();
-    c->bank = bank, c->plan = plan, c->w = w, c->wt = wt, c->bias = bias, c->unit = unit, c->serial = bank->serial, c->M = M, c->N = N, c->K = K;
+    c->bank = bank, c->plan = plan, c->w = w, c->wt = wt, c->bias = bias, c->unit = unit, c->serial = reading.serial, c->M = M, c->N = N, c->K = K;
     return AdapterLinear::apply(x, down, up, residual_, c, ckpt8, train);
   }
   Rows r;
@@ -521,9 +563,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def_readwrite("a", &Bank::a).def_readwrite("b", &Bank::b).def_readwrite("at", &Bank::at).def_readwrite("bt", &Bank::bt)
       .def_readwrite("ranks", &Bank::ranks).def_readwrite("scales", &Bank::scales)
       .def_readwrite("down", &Bank::down).def_readwrite("up", &Bank::up).def("fresh", &Bank::fresh)
-      .def("reads", &Bank::reads).def("begin_layout", &Bank::begin_layout).def("end_layout", &Bank::end_layout)
+      .def("reads", &Bank::reads)
+      .def("begin_layout", &Bank::begin_layout, py::call_guard<py::gil_scoped_release>())   // (a call that it waits for may need the interpreter)
+      .def("end_layout", &Bank::end_layout)
       .def_readwrite("G", &Bank::G).def_readwrite("r", &Bank::r).def_readwrite("R", &Bank::R).def_readwrite("K", &Bank::K).def_readwrite("N", &Bank::N)
-      .def_readwrite("serial", &Bank::serial).def_readwrite("trainable", &Bank::trainable);
+      .def_readonly("serial", &Bank::serial).def_readwrite("trainable", &Bank::trainable);
   py::class_<Plan, std::shared_ptr<Plan>>(m, "Plan")
       .def(py::init<>())
       .def_readwrite("table", &Plan::table).def_readwrite("start", &Plan::start).def_readwrite("at", &Plan::at)

@@ -2074,13 +2074,14 @@ def adapter_linear(x2d, packed, bank, plan, residual=None, ckpt8=False):
     if residual is not None:
         _plain(residual, "adapter_linear")
     args = x2d, packed.w, packed.wt, packed.bias, bank.handle, plan.handle, residual, ckpt8
-    y = L.native().adapter_linear(*args)
-    if y is None:                            # the bank's kernel copies do not fit the call yet: other weights, or a first input gradient
-        bank.refresh()
+    for _ in range(16):
+        y = L.native().adapter_linear(*args)
+        if y is not None:
+            return y
+        bank.refresh()                       # the bank's kernel copies do not fit the call yet: other weights, or a first input gradient
         if x2d.requires_grad and torch.is_grad_enabled():
             bank.lay_out_transposed()
-        y = L.native().adapter_linear(*args)
-    return y
+    raise L.AqlError("adapter_linear: another thread keeps changing the bank's weights")
 
 
 class GegluFn(torch.autograd.Function):

@@ -1,5 +1,7 @@
 """What an AdapterBank keeps between calls -- the bf16 stacks that the kernels read -- under streams, threads, captures and optimizers: a call sees the
 parameters as they are, whoever laid the stacks out.  Comparisons are bit for bit with a bank that was made from the same weights."""
+import threading
+
 import pytest
 import torch
 
@@ -87,3 +89,83 @@ def test_a_layout_waits_for_the_streams_that_still_read():
             b = s.step(bank)
         torch.cuda.synchronize()
         assert same(a, old) and same(b, new)
+
+
+@gpu
+def test_threads_come_together_after_a_step():
+    """Two threads, each with a stream of its own, call forward and backward right after the parameters changed: one layout, no pass refused, the new weights in both."""
+    s = Site(2)
+    bank = s.bank(s.old)
+    weights = [[w.to(DEV) for w in ws] for ws in (s.old, s.new)]
+    want = [s.step(s.bank(ws)) for ws in (s.old, s.new)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    barrier, got, errors = threading.Barrier(3), [None, None], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(streams[i]):
+                for _ in range(60):
+                    barrier.wait(60)
+                    got[i] = s.step(bank)
+                    torch.cuda.current_stream().synchronize()
+                    barrier.wait(60)
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+            barrier.abort()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    try:
+        for k in range(60):
+            put(bank, weights[(k + 1) % 2])
+            serial = bank.handle.serial
+            torch.cuda.synchronize()
+            barrier.wait(60)
+            barrier.wait(60)
+            assert bank.handle.serial == serial + 1
+            assert all(same(g, want[(k + 1) % 2]) for g in got), k
+    except threading.BrokenBarrierError:
+        pass
+    except AssertionError:
+        barrier.abort()
+        raise
+    finally:
+        for t in threads:
+            t.join()
+    assert not errors, errors
+
+
+@gpu
+def test_a_change_under_a_layout_is_not_lost():
+    """The versions that a layout has seen are those from before its copies: a parameter changed right behind them is laid out by the next call."""
+    s = Site(3)
+    bank = s.bank(s.old)
+    new = [w.to(DEV) for w in s.new]
+
+    class Late:                                          # the handle, with another thread's write between the copies and their end
+        def __getattr__(self, name):
+            return getattr(handle, name)
+
+        def end_layout(self):
+            put(bank, new)
+            handle.end_layout()
+    handle = bank.handle
+    bank.handle = Late()
+    bank.refresh(force=True)
+    bank.handle = handle
+    assert torch.equal(s.call(bank), s.call(s.bank(s.new)))
+
+
+@gpu
+def test_a_layout_from_inside_a_call_is_refused():
+    s = Site(4)
+    bank = s.bank(s.old)
+
+    def pack(t):
+        bank.refresh(force=True)
+        return t
+    x = s.x.detach().requires_grad_(True)
+    with pytest.raises(RuntimeError, match="inside a call"):
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+            ops.adapter_linear(x, s.packed, bank, s.plan)
+    assert torch.equal(s.call(bank), s.call(s.bank(s.old)))

@@ -113,8 +113,9 @@ class AdapterBank:
                 return
             h = self.handle
             h.reads()
-            h.at, h.bt = h.a.transpose(1, 2).contiguous(), h.b.transpose(1, 2).contiguous()
+            at, bt = h.a.transpose(1, 2).contiguous(), h.b.transpose(1, 2).contiguous()
             torch.cuda.current_stream(self.device).synchronize()      # once: later calls may come on other streams
+            h.bt, h.at = bt, at                  # (calls go by `at`: it is there when both are complete)
             self._transposed = True
 
 

@@ -1,6 +1,7 @@
 """What an AdapterBank keeps between calls -- the bf16 stacks that the kernels read -- under streams, threads, captures and optimizers: a call sees the
 parameters as they are, whoever laid the stacks out.  Comparisons are bit for bit with a bank that was made from the same weights."""
 import threading
+import time
 
 import pytest
 import torch
@@ -169,3 +170,32 @@ def test_a_layout_from_inside_a_call_is_refused():
         with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
             ops.adapter_linear(x, s.packed, bank, s.plan)
     assert torch.equal(s.call(bank), s.call(s.bank(s.old)))
+
+
+@gpu
+def test_transposed_stacks_are_there_when_they_are_complete():
+    """One thread's call lays a frozen bank's transposed stacks out on a busy stream; another thread's call comes meanwhile."""
+    s = Site(5)
+
+    def step(bank):
+        x = s.x.detach().requires_grad_(True)
+        return torch.autograd.grad(ops.adapter_linear(x, s.packed, bank, s.plan), x, s.dy)
+    want = step(s.bank(s.old, False))
+    bank = s.bank(s.old, False)
+    torch.cuda.synchronize()
+    got = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                torch.cuda._sleep(SLEEP)
+            got.append(step(bank))
+            torch.cuda.current_stream().synchronize()
+    thread = threading.Thread(target=work)
+    thread.start()
+    time.sleep(0.02)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        got.append(step(bank))
+    thread.join()
+    torch.cuda.synchronize()
+    assert len(got) == 2 and all(same(g, want) for g in got)

@@ -22,7 +22,8 @@ class AdapterBank:
     multiplies it (None: 1).  The kernels read bf16 copies laid out once.  ``trainable``: ``down`` / ``up`` become fp32 parameters, their
     gradients are fp32, and the copies follow after an optimizer step: `refresh` lays them out again when the parameters' versions
     have changed (ops.adapter_linear calls it; writes through ``.data``, and an optimizer step inside a captured graph, need
-    ``refresh(force=True)`` behind them)."""
+    ``refresh(force=True)`` behind them).  A graph reads the stacks as they are at its replay: an eager step between replays needs `refresh` behind it;
+    a call in a capture that finds them stale is refused, and ``refresh(force=True)`` in a capture is for the replays of that graph alone."""
 
     @torch.inference_mode(False)
     def __init__(self, down, up, ranks=None, scales=None, trainable=False, device="cuda"):
@@ -92,6 +93,9 @@ class AdapterBank:
         with self._lock:                     # of threads that come together the first lays out
             if h.fresh() and not force:
                 return
+            if not force and torch.cuda.is_current_stream_capturing():
+                raise L.AqlError("AdapterBank: the weights have changed since they were laid out: call refresh() before the capture, or refresh(force=True) in it "
+                                 "for a graph that lays them out at every replay")
             h.begin_layout()                 # behind what other threads and streams still read; backward passes of older calls are refused from here on
             with torch.no_grad():            # in place: a captured graph keeps reading these buffers
                 h.a[:, :r].copy_(torch.where(live[:, :, None], self.down, torch.zeros((), dtype=self.down.dtype, device=self.device)))

@@ -72,6 +72,13 @@ bool capturing(const c10::hip::HIPStream& s) {
   hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
   return hipStreamIsCapturing(s.stream(), &cs) == hipSuccess && cs != hipStreamCaptureStatusNone;
 }
+// of the capture that a stream is in, never used again; 0: none
+unsigned long long capture_id(const c10::hip::HIPStream& s) {
+  hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  hip_ok(hipStreamGetCaptureInfo(s.stream(), &cs, &id), "hipStreamGetCaptureInfo");
+  return cs == hipStreamCaptureStatusActive ? id : 0;
+}
 
 // at::empty without the dispatcher's way to it: a backward pass allocates up to seven tensors
 Tensor fresh(at::IntArrayRef size, at::ScalarType type, const Tensor& like) { return at::detail::empty_cuda(size, type, like.device(), std::nullopt); }
@@ -271,19 +278,26 @@ struct Bank {   // the device side of adapters.AdapterBank
   long G = 0, r = 0, R = 0, K = 0, N = 0;
   bool trainable = false;
 
-  bool fresh() const { return (int64_t)down._version() == down_seen && (int64_t)up._version() == up_seen; }
+  // whether the stacks that a call on the current stream will read are those of the parameters
+  bool fresh() const {
+    const bool recorded = laid_in && capture_id(current()) == laid_in;   // a layout that the graph being captured holds goes before those outside
+    return (int64_t)down._version() == (recorded ? down_rec : down_seen) && (int64_t)up._version() == (recorded ? up_rec : up_seen);
+  }
 
   // The stacks are written in place, by whichever call comes first after a change, and read by all, from any thread and stream.
   //   Threads: `busy` calls are queueing kernels that read the stacks; a layout begins by raising `serial` and making the stacks stale, so that no further call enters,
   //   and then waits for the ones inside.  (A backward pass enters by the serial of its forward pass; the versions are noted ahead of the copies.)
   //   Streams: the first read on a stream behind a layout waits for its event, and a layout waits for every stream that has read since the last one.
   // (What runs inside a graph is ordered by whoever replays it.)
+  //   Captures: a layout in a capture changes nothing before a replay.  Only calls in that same capture go by it.
   std::mutex guard;
   std::condition_variable quiet;
   int busy = 0;
   long serial = 0;
   static thread_local const Bank* inside;     // the bank that this thread is queueing reads of
   int64_t down_next = -1, up_next = -1;       // versions that the layout in progress will have seen
+  unsigned long long laid_in = 0;             // the capture that holds the last recorded layout, and the versions that it has seen
+  int64_t down_rec = -1, up_rec = -1;
   std::optional<c10::hip::HIPStream> home;    // stream of the last layout
   std::vector<c10::hip::HIPStream> readers;   // streams that have read since then
   hipEvent_t laid = nullptr, mark = nullptr;  // behind the last layout; for one wait at a time
@@ -313,10 +327,10 @@ struct Bank {   // the device side of adapters.AdapterBank
     if (inside == this) throw AqlErr("AdapterBank: changed weights cannot be laid out from inside a call that uses the bank (a hook of its saved tensors)");
     std::unique_lock<std::mutex> lock(guard);
     down_next = down._version(), up_next = up._version();
-    down_seen = up_seen = -1;
     ++serial;
-    quiet.wait(lock, [&] { return busy == 0; });
     if (capturing(s)) return;
+    down_seen = up_seen = -1;
+    quiet.wait(lock, [&] { return busy == 0; });
     const c10::DeviceGuard device(a.device());
     for (hipEvent_t* e : {&laid, &mark})
       if (!*e) hip_ok(hipEventCreateWithFlags(e, hipEventDisableTiming), "AdapterBank");
@@ -331,11 +345,13 @@ struct Bank {   // the device side of adapters.AdapterBank
   void end_layout() {
     const auto s = current();
     const std::lock_guard<std::mutex> lock(guard);
-    if (!capturing(s)) {
-      hip_ok(hipEventRecord(laid, s.stream()), "AdapterBank");
-      home = s;
-      readers.clear();
+    if ((laid_in = capture_id(s))) {
+      down_rec = down_next, up_rec = up_next;
+      return;
     }
+    hip_ok(hipEventRecord(laid, s.stream()), "AdapterBank");
+    home = s;
+    readers.clear();
     down_seen = down_next, up_seen = up_next;
   }
 };

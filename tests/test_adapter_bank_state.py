@@ -199,3 +199,89 @@ def test_transposed_stacks_are_there_when_they_are_complete():
     thread.join()
     torch.cuda.synchronize()
     assert len(got) == 2 and all(same(g, want) for g in got)
+
+
+@gpu
+def test_a_capture_that_finds_the_bank_stale_is_refused():
+    s = Site(6)
+    bank = s.bank(s.old)
+    want = s.call(s.bank(s.new))
+    s.call(bank)
+    put(bank, [w.to(DEV) for w in s.new])
+    torch.cuda.synchronize()
+    with torch.no_grad():
+        with pytest.raises(RuntimeError, match="before the capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                s.call(bank)
+        torch.cuda.synchronize()
+        assert torch.equal(s.call(bank), want)           # nothing was marked
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):                    # and now there is nothing to lay out
+            bank.refresh()
+            y = s.call(bank)
+    for weights in (s.old, s.new, s.old):                # eager steps between the replays
+        put(bank, [w.to(DEV) for w in weights])
+        bank.refresh()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, s.call(s.bank(weights)))
+
+
+@gpu
+@pytest.mark.parametrize("aborted", [False, True])
+def test_a_layout_in_a_capture_is_for_its_replays(aborted):
+    s = Site(7)
+    bank = s.bank(s.old)
+    old, new = (s.call(s.bank(w)) for w in (s.old, s.new))
+    s.call(bank)
+    to = [w.to(DEV) for w in s.new]
+    put(bank, to)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad():
+        try:
+            with torch.cuda.graph(graph):
+                bank.refresh(force=True)
+                y = s.call(bank)
+                if aborted:
+                    raise KeyError
+        except KeyError:
+            pass
+        torch.cuda.synchronize()
+        assert torch.equal(s.call(bank), new)            # eager, ahead of the first replay
+        if aborted:
+            return
+        for weights, want in ((s.old, old), (s.new, new)):
+            for p, w in zip((bank.down, bank.up), weights):
+                p.data.copy_(w.to(DEV))                  # (no version tells of it)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, want) and torch.equal(s.call(bank), want)
+
+
+@gpu
+def test_two_training_steps_in_one_graph():
+    s = Site(8)
+    lr = 0.05
+
+    def two(bank):
+        out = []
+        for _ in range(2):
+            y = s.call(bank)
+            out += [y.detach(), *torch.autograd.grad(y, (bank.down, bank.up), s.dy)]
+            with torch.no_grad():
+                bank.down.sub_(lr * out[-2])
+                bank.up.sub_(lr * out[-1])
+            bank.refresh(force=True)
+        return out
+    eager, bank = s.bank(s.old), s.bank(s.old)
+    two(eager), two(bank)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = two(bank)
+    for k in range(3):
+        want = two(eager)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same(got, want), k
+        assert torch.equal(s.call(bank), s.call(eager))

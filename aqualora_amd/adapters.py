@@ -9,10 +9,23 @@ import threading
 import numpy as np
 import torch
 import torch.nn as nn
+from torch.optim.optimizer import register_optimizer_step_post_hook
 
 from . import _lib as L
 
 MAX_RANK = 1024
+
+
+def _count_fused_step(optimizer, args, kwargs):
+    """torch's fused optimizers write parameters without raising their versions, by which a bank tells that its weights have changed."""
+    for group in optimizer.param_groups:
+        if group.get("fused"):
+            for p in group["params"]:
+                if getattr(p, "_aql_bank_weights", False) and p.grad is not None:
+                    torch.autograd.graph.increment_version(p)
+
+
+_fused_hook = None
 
 
 class AdapterBank:
@@ -21,8 +34,8 @@ class AdapterBank:
     ``down`` [G, r, K] and ``up`` [G, N, r] in bf16 or fp32; ``ranks[g]`` <= r says how much of adapter g is used (None: all of it), ``scales[g]``
     multiplies it (None: 1).  The kernels read bf16 copies laid out once.  ``trainable``: ``down`` / ``up`` become fp32 parameters, their
     gradients are fp32, and the copies follow after an optimizer step: `refresh` lays them out again when the parameters' versions
-    have changed (ops.adapter_linear calls it; writes through ``.data``, and an optimizer step inside a captured graph, need
-    ``refresh(force=True)`` behind them).  A graph reads the stacks as they are at its replay: an eager step between replays needs `refresh` behind it;
+    have changed (ops.adapter_linear calls it; writes that raise no version -- through ``.data``, by collectives such as
+    ``dist.broadcast``, by an optimizer step inside a captured graph -- need ``refresh(force=True)`` behind them).  A graph reads the stacks as they are at its replay: an eager step between replays needs `refresh` behind it;
     a call in a capture that finds them stale is refused, and ``refresh(force=True)`` in a capture is for the replays of that graph alone."""
 
     @torch.inference_mode(False)
@@ -57,6 +70,10 @@ class AdapterBank:
         if trainable:
             self.down = nn.Parameter(down.detach().to(device=dev, dtype=torch.float32, copy=True))
             self.up = nn.Parameter(up.detach().to(device=dev, dtype=torch.float32, copy=True))
+            self.down._aql_bank_weights = self.up._aql_bank_weights = True
+            global _fused_hook
+            if _fused_hook is None:
+                _fused_hook = register_optimizer_step_post_hook(_count_fused_step)
         else:
             # (a copy of an inference tensor: `refresh` goes by version counters)
             self.down, self.up = (t.detach().to(dev, copy=t.is_inference()) for t in (down, up))

@@ -285,3 +285,30 @@ def test_two_training_steps_in_one_graph():
         torch.cuda.synchronize()
         assert same(got, want), k
         assert torch.equal(s.call(bank), s.call(eager))
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["single", "foreach", "fused"])
+@pytest.mark.parametrize("name", ["SGD", "Adam", "AdamW"])
+def test_a_bank_follows_every_form_of_an_optimizer(name, kind):
+    s = Site(9)
+    bank = s.bank(s.old)
+    opt = getattr(torch.optim, name)(bank.parameters(), lr=0.05, foreach=kind == "foreach", fused=kind == "fused")
+    for _ in range(3):
+        y = s.call(bank)
+        assert torch.equal(y, s.call(s.bank((bank.down.detach(), bank.up.detach()))))
+        before = bank.up.detach().clone()
+        bank.down.grad, bank.up.grad = torch.autograd.grad(y, (bank.down, bank.up), s.dy)
+        opt.step()
+        assert not torch.equal(bank.up.detach(), before)
+
+
+def test_fused_steps_raise_the_versions_of_bank_weights_only():
+    ps = [torch.nn.Parameter(torch.ones(4)) for _ in range(3)]
+    for p in ps[:2]:
+        p.grad = torch.ones(4)
+    ps[0]._aql_bank_weights = ps[2]._aql_bank_weights = True
+    opt = torch.optim.SGD(ps, lr=0.1, fused=True)
+    opt.register_step_post_hook(adapters._count_fused_step)
+    opt.step()
+    assert [p._version for p in ps] == [1, 0, 0] and all((p < 1).all() for p in ps[:2])      # (no gradient, no step)

@@ -140,6 +140,11 @@ class AdapterBank:
             self._transposed = True
 
 
+def banks_of(module):
+    """The banks on the hosts inside ``module``."""
+    return [m.adapter_bank for m in module.modules() if getattr(m, "adapter_bank", None) is not None]
+
+
 class RequestPlan:
     """Which rows use which adapter: request i has ``lengths[i]`` rows (None: all requests have the same number, whatever the rows of the call) and
     adapter ``adapters[i]`` (-1: none).  Requests follow each other in the rows.  The tables are built on the host once and live on the device;

@@ -29,6 +29,7 @@ import math
 import torch
 
 from . import _lib as L
+from .adapters import RequestPlan, banks_of
 from .inference import _cfg_scale, ddim_timesteps
 from .watermark import sd15_alphas_cumprod
 
@@ -396,6 +397,7 @@ class SamplerMachine:
         self.flag = torch.zeros(2, 5, dtype=torch.int32, device=dev)
         self.eps = None
         self.graph = None
+        self.banks = []           # under a RequestPlan: whose memory the graph reads
         self.use_graph = graph
         if self.scale2 is None:   # LoRA-free / fused U-Net: attn2's k|v of the text states once per prompt, not once per phase
             self.ctx._aql_kv_static = unet.text_kv(self.ctx)
@@ -420,6 +422,13 @@ class SamplerMachine:
     @torch.no_grad()
     def run(self, prog, noise_fn=None):
         """-> final fp32 latents.  ``noise_fn(i, like)`` supplies the N(0, 1) noise of ancestral phase i."""
+        if isinstance(self.scale2, RequestPlan):          # replays read the banks as they were laid out last: lay out what has changed since an earlier run
+            banks = banks_of(self.unet)
+            if len(banks) != len(self.banks) or any(a is not b for a, b in zip(banks, self.banks)):
+                self.graph = None                         # captured on banks that have been replaced
+            self.banks = banks
+            for bank in banks:
+                bank.refresh()
         self.x.mul_(prog.init_scale)
         # the first model input: a call without a model output that only writes uin = first_in_scale * x
         coef, flag = _call(no_eval=True, cx=1.0, nscale=prog.first_in_scale)

@@ -6,7 +6,9 @@ import time
 import pytest
 import torch
 
-from aqualora_amd import adapters, ops
+from aqualora_amd import adapters, inference, ksamplers, ops
+from aqualora_amd.unet import lora_keys
+from tests.common import ppft_inputs, tiny_lora, tiny_unet
 
 DEV = "cuda"
 SLEEP = 50_000_000     # cycles: 20 ms or more, longer than the host needs for what is queued behind it
@@ -312,3 +314,31 @@ def test_fused_steps_raise_the_versions_of_bank_weights_only():
     opt.register_step_post_hook(adapters._count_fused_step)
     opt.step()
     assert [p._version for p in ps] == [1, 0, 0] and all((p < 1).all() for p in ps[:2])      # (no gradient, no step)
+
+
+@gpu
+def test_a_sampling_machine_follows_the_banks():
+    """A second run of one machine: after a step on the banks, and after other banks were attached."""
+    unet = tiny_unet(DEV, torch.bfloat16)
+    keys = lora_keys(unet)
+    loras = [{f"{k}.{n}.weight": t for k, p in tiny_lora(keys, unet, rank=8, up_std=std).items() for n, t in zip(("down", "up"), p)} for std in (0.1, 0.2)]
+    inp = ppft_inputs(B=2, device=DEV)
+    unc = torch.zeros_like(inp["ctx"])
+    prog = ksamplers.program("euler", 3)
+    new = lambda: ksamplers.SamplerMachine(unet, inp["ctx"], unc, inp["z"], 3.0, scale=adapters.RequestPlan([1, 0]))  # noqa: E731
+
+    def again(m):
+        m.x.copy_(inp["z"])
+        return m.run(prog)
+    banks = inference.attach_adapters(unet, loras, trainable=True)
+    m = new()
+    first = m.run(prog)
+    assert torch.equal(again(m), first)
+    with torch.no_grad():
+        for bank in banks.values():
+            bank.up.mul_(0.5)
+    second = again(m)
+    assert torch.equal(second, new().run(prog)) and not torch.equal(second, first)
+    inference.attach_adapters(unet, loras[::-1])
+    third = again(m)
+    assert torch.equal(third, new().run(prog)) and not torch.equal(third, first)

@@ -8,6 +8,8 @@ sample latents with DDIM + classifier-free guidance.
                          steps_offset 1, eta 0, guidance 7.5 (recalled semantics; unpinned)
 The VAE decode that turns latents into pixels is outside this path.
 """
+from collections.abc import Mapping
+
 import torch
 
 from . import _lib as L
@@ -73,6 +75,9 @@ def attach_adapters(unet, lora_state_dicts, lora_scales=None, keys=None, trainab
     banks by site (``trainable``: their parameters learn)."""
     if not lora_state_dicts:
         raise ValueError("attach_adapters: no adapters")
+    for sd in lora_state_dicts:
+        if not isinstance(sd, Mapping):
+            raise ValueError(f"attach_adapters: state dicts, not {type(sd).__name__} (`create_watermark_lora` returns the message and the state dict)")
     keys = keys if keys is not None else load_unet_keys(unet)
     scales = [1.0] * len(lora_state_dicts) if lora_scales is None else list(lora_scales)
     banks = {}

@@ -1,0 +1,47 @@
+"""From one watermark LoRA and several messages to a U-Net that serves all of them: bake, attach, run; and what attach_adapters refuses."""
+import pytest
+import torch
+
+from aqualora_amd import adapters, inference, lora
+from aqualora_amd.checkpoint import lora_state_dict, site_to_ckpt_key
+from aqualora_amd.unet import lora_keys
+from aqualora_amd.watermark import MapperNet
+from oracle.ppft_oracle import UNetOracle
+from tests.common import TINY, ppft_inputs, tiny_lora, tiny_unet
+from tests.test_adapter_serving import single
+
+DEV = "cuda"
+gpu = pytest.mark.gpu
+
+
+@gpu
+def test_baked_messages_are_attached_and_served():
+    unet = tiny_unet(DEV, torch.bfloat16)
+    keys = lora_keys(unet)
+    lora.inject_lora(unet, 8, keys, {f"{k}.{n}.weight": t for k, p in tiny_lora(keys, unet, rank=8).items() for n, t in zip(("down", "up"), p)})
+    state_dict = lora_state_dict(unet, keys)
+    torch.manual_seed(3)
+    mapper = MapperNet(48, 8).to(DEV)
+    messages = ["01" * 24, "0011" * 12]
+    loras = [inference.create_watermark_lora(state_dict, mapper, msg)[1] for msg in messages]
+    unet = tiny_unet(DEV, torch.bfloat16)
+    inference.attach_adapters(unet, loras)
+    inp = ppft_inputs(B=3, device=DEV)
+    plan = adapters.RequestPlan([1, -1, 0])
+    with torch.no_grad():
+        got = unet(inp["z"], inp["t"], inp["ctx"], cross_attention_kwargs={"scale": plan}).sample.float()
+    # against the fp32 network with the baked weights; a U-Net that carries one of them alone rounds to bf16 at as many places (T once more): the norms of the
+    # two errors agree but for chance, 2 is allowed
+    b16 = lambda t: t.to(torch.bfloat16).float().cpu()  # noqa: E731
+    sd = {k: b16(v) for k, v in tiny_unet().state_dict().items()}
+    for baked, row in ((loras[1], 0), (loras[0], 2)):
+        lw = {k: tuple(b16(baked[f"{site_to_ckpt_key(k)}.{n}.weight"]) for n in ("down", "up")) for k in keys}
+        want = UNetOracle(sd, TINY, lw).forward(b16(inp["z"][[row]]), inp["t"][[row]].cpu(), b16(inp["ctx"][[row]]), scale=1.0)
+        err, err1 = (got[[row]].cpu() - want).norm(), (single(lw, inp, [row]).cpu() - want).norm()
+        assert err <= 2 * err1, (row, (err / want.norm()).item(), (err1 / want.norm()).item())
+
+
+def test_attach_adapters_takes_state_dicts():
+    unet = tiny_unet()
+    with pytest.raises(ValueError, match="state dicts"):
+        inference.attach_adapters(unet, [("01" * 24, {})])

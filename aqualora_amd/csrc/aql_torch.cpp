@@ -207,6 +207,7 @@ struct LayerNormTrain : torch::autograd::Function<LayerNormTrain> {
     auto c = c10::make_intrusive<NormCall>();
     c->beta = beta.defined();
     c->leaves = {leaf(x), leaf(gamma), leaf(beta)};
+    ctx->set_materialize_grads(false);   // an output that nothing used has no gradient, not one of zeros
     ctx->saved_data["call"] = c10::IValue::make_capsule(std::move(c));
     if (passthrough) return {y, x.view_as(x)};
     return {y};
@@ -217,9 +218,10 @@ struct LayerNormTrain : torch::autograd::Function<LayerNormTrain> {
     const auto c = c10::static_intrusive_pointer_cast<NormCall>(ctx->saved_data["call"].toCapsule());
     const long M = stats.size(0), C = gamma.size(0);
     const bool want_g = ctx->needs_input_grad(1), want_b = c->beta && ctx->needs_input_grad(2);
-    if (!g[0].defined()) {   // only the pass-through output was used
-      const Tensor z;
-      return {g.size() > 1 ? g[1] : z, z, z, z, z, z};
+    if (!g[0].defined()) {   // only the pass-through output was used: its gradient as it is, and the weights have no part in it
+      at::AutoGradMode off(false);
+      const auto zeros = [&](bool want) { return want ? at::zeros({C}, gamma.options()) : Tensor(); };
+      return {g.size() > 1 ? g[1] : Tensor(), zeros(want_g), zeros(want_b), Tensor(), Tensor(), Tensor()};
     }
     here(g[0], "layernorm_train backward");
     leaves_ok(c->leaves, g[0], "layernorm_train");
@@ -484,6 +486,7 @@ struct AdapterLinear : torch::autograd::Function<AdapterLinear> {
       ran(aql_act8_pack(x.t.data_ptr(), 0, c->M, (int)c->K, x.ld, ptr<uint8_t>(codes), ptr<uint8_t>(exps), st), "aql_act8_pack", st);
       keep = T = Tensor();
     }
+    ctx->set_materialize_grads(false);
     ctx->save_for_backward({keep, T, codes, exps});
     ctx->saved_data["call"] = c10::IValue::make_capsule(c);
     return y;

@@ -545,6 +545,8 @@ std::optional<Tensor> adapter_linear(const Tensor& x, const Tensor& w, const Ten
   if (res.defined() && (res.dim() != 2 || res.size(0) != M || res.size(1) != N || res.scalar_type() != at::kBFloat16))
     bad_value("adapter_linear: residual must be bfloat16 [" + std::to_string(M) + ", " + std::to_string(N) + "], not " + shape_of(res));
   here(x, "adapter_linear");
+  for (const Tensor* t : {&x, &res, &down, &up})   // (without reverse gradients no node is made that would refuse it)
+    if (t->defined() && t->_fw_grad(0).defined()) throw AqlErr("adapter_linear has no forward-mode derivative");
   if (bank->a.device() != x.device() || plan->table.device() != x.device() || w.device() != x.device() || (res.defined() && res.device() != x.device()))
     bad_value("adapter_linear: input, projection, adapters, plan and residual must live on one device");
   const Reading reading(*bank);

@@ -588,3 +588,18 @@ def test_refusals():
     for a in (([-2], [3]), ([0], [3, 4]), ([0], [-1])):
         with pytest.raises(ValueError):
             adapters.RequestPlan(*a)
+
+
+@gpu
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(grad):
+    """A tangent of any differentiable input is refused, not dropped, whether or not reverse gradients are asked for."""
+    d, lengths, rows, ids, equal = make("ragged", 14)
+    packed, bank, plan = handles(d, lengths, ids, equal, True)
+    x, res = d["x"].to(DEV), d["res"].to(DEV)
+    fw = torch.autograd.forward_ad
+    with torch.set_grad_enabled(grad), fw.dual_level():
+        for xd, rd in ((fw.make_dual(x, torch.ones_like(x)), res), (x, fw.make_dual(res, torch.ones_like(res)))):
+            with pytest.raises(RuntimeError):
+                ops.adapter_linear(xd, packed, bank, plan, residual=rd)
+        ops.adapter_linear(x, packed, bank, plan, residual=res)

@@ -16,7 +16,7 @@ from . import _lib as L
 from . import ops
 from .adapters import AdapterBank, RequestPlan
 from .checkpoint import site_to_ckpt_key
-from .lora import _walk, load_unet_keys
+from .lora import LoRACompatibleConv, LoRACompatibleLinear, _walk, load_unet_keys
 from .watermark import sd15_alphas_cumprod
 
 
@@ -80,9 +80,13 @@ def attach_adapters(unet, lora_state_dicts, lora_scales=None, keys=None, trainab
             raise ValueError(f"attach_adapters: state dicts, not {type(sd).__name__} (`create_watermark_lora` returns the message and the state dict)")
     keys = keys if keys is not None else load_unet_keys(unet)
     scales = [1.0] * len(lora_state_dicts) if lora_scales is None else list(lora_scales)
+    hosts = {key: _walk(unet, key) for key in keys}
+    for key, host in hosts.items():          # sites whose forward reads a bank: a linear, a 1x1 convolution -- but the U-Net runs all time_emb_proj as one projection
+        conv = isinstance(host, LoRACompatibleConv) and (host.kernel_size, host.stride, tuple(host.padding)) == ((1, 1), (1, 1), (0, 0))
+        if not (conv or isinstance(host, LoRACompatibleLinear)) or key.endswith("time_emb_proj"):
+            raise ValueError(f"attach_adapters: {key} does not run adapters (linears other than time_emb_proj and 1x1 convolutions do)")
     banks = {}
-    for key in keys:
-        host = _walk(unet, key)
+    for key, host in hosts.items():
         ck = site_to_ckpt_key(key)
         pairs = []
         for sd in lora_state_dicts:
@@ -94,7 +98,9 @@ def attach_adapters(unet, lora_state_dicts, lora_scales=None, keys=None, trainab
         pad = torch.nn.functional.pad
         down = torch.stack([pad(d, (0, 0, 0, r - d.shape[0])) for d, _ in pairs])
         up = torch.stack([pad(u, (0, r - u.shape[1])) for _, u in pairs])
-        host.adapter_bank = banks[key] = AdapterBank(down, up, ranks=ranks, scales=scales, trainable=trainable, device=host.weight.device)
+        banks[key] = AdapterBank(down, up, ranks=ranks, scales=scales, trainable=trainable, device=host.weight.device)
+    for key, host in hosts.items():
+        host.adapter_bank = banks[key]
     return banks
 
 

@@ -45,3 +45,33 @@ def test_attach_adapters_takes_state_dicts():
     unet = tiny_unet()
     with pytest.raises(ValueError, match="state dicts"):
         inference.attach_adapters(unet, [("01" * 24, {})])
+
+
+@pytest.mark.parametrize("kind", ["conv1", "downsamplers.0.conv", "time_emb_proj", "norm1"])
+def test_attach_adapters_refuses_sites_that_do_not_run_them(kind):
+    """3x3 convolutions, the time projections and modules without LoRA: refused before any site carries a bank."""
+    unet = tiny_unet()
+    good = lora_keys(unet)[0]
+    bad = next(n for n, _ in unet.named_modules() if n.endswith(kind))
+    with pytest.raises(ValueError, match="does not run adapters"):
+        inference.attach_adapters(unet, [{f"{k}.{n}.weight": torch.zeros(8, 8) for k in (good, bad) for n in ("down", "up")}], keys=[good, bad])
+    assert not adapters.banks_of(unet)
+
+
+@gpu
+def test_adapters_on_every_kind_of_site_that_runs_them():
+    """A linear outside the transformer blocks and a 1x1 shortcut: the bank changes the output of its own owner's image only."""
+    unet = tiny_unet(DEV, torch.bfloat16)
+    sites = ["time_embedding.linear_1"] + [n for n, m in unet.named_modules() if n.endswith("conv_shortcut") and m is not None][:1]
+    inp = ppft_inputs(B=2, device=DEV)
+    call = lambda scale: unet(inp["z"], inp["t"], inp["ctx"], cross_attention_kwargs={"scale": scale}).sample  # noqa: E731
+    gen = torch.Generator().manual_seed(4)
+    for site in sites:
+        w = unet.get_submodule(site).weight
+        lo = {f"{site}.down.weight": torch.randn(8, w.shape[1], generator=gen), f"{site}.up.weight": torch.randn(w.shape[0], 8, generator=gen)}
+        with torch.no_grad():
+            inference.attach_adapters(unet, [lo], keys=[site])
+            got = call(adapters.RequestPlan([-1, 0]))
+            off = call(adapters.RequestPlan([-1, -1]))
+        assert torch.equal(got[0], off[0]) and not torch.equal(got[1], off[1]), site
+        del unet.get_submodule(site).adapter_bank

@@ -154,6 +154,7 @@ variable_list once(variable_list grads, const char* name) {
 }
 
 // ------------------------------------------------------------------------------------------------------------------ 8-bit checkpoint
+constexpr long ACT8_COLUMNS = 1 << 24;   // the C entries' limit, checked ahead of their int
 std::pair<Tensor, Tensor> act8_alloc(long M, long C, const Tensor& like) {
   const long Cp = (C + 31) / 32 * 32;
   return {fresh({M, Cp}, at::kByte, like), fresh({M, Cp / 32}, at::kByte, like)};
@@ -162,6 +163,7 @@ std::pair<Tensor, Tensor> act8_alloc(long M, long C, const Tensor& like) {
 std::pair<Tensor, Tensor> act8_pack(const Tensor& x) {
   if (!bf16_or_f32(x)) bad_value(std::string("act8_pack: bfloat16 or float32, not ") + c10::toString(x.scalar_type()));
   if (x.dim() < 1 || x.size(-1) == 0) bad_value("act8_pack: expected [..., columns], got " + shape_of(x));
+  if (x.size(-1) > ACT8_COLUMNS) bad_value("act8_pack: at most " + std::to_string(ACT8_COLUMNS) + " columns, got " + shape_of(x));
   here(x, "act8_pack");
   at::AutoGradMode off(false);
   const long C = x.size(-1);
@@ -180,6 +182,7 @@ Tensor act8_unpack(const Tensor& codes, const Tensor& exps, std::vector<int64_t>
   if (C < 1 || !fits(codes, Cp) || !fits(exps, Cp / 32) || codes.device() != exps.device())
     bad_value("Act8.unpack: codes uint8 [" + std::to_string(M) + ", " + std::to_string(Cp) + "] and exps uint8 [" + std::to_string(M) + ", " +
               std::to_string(Cp / 32) + "], contiguous on one device, not " + shape_of(codes) + " and " + shape_of(exps));
+  if (C > ACT8_COLUMNS) bad_value("Act8.unpack: at most " + std::to_string(ACT8_COLUMNS) + " columns, not " + std::to_string(C));
   here(codes, "Act8.unpack");
   Tensor out = fresh(shape, bf16 ? at::kBFloat16 : at::kFloat, codes);
   const auto st = stream_of(codes);
@@ -538,6 +541,7 @@ std::optional<Tensor> adapter_linear(const Tensor& x, const Tensor& w, const Ten
   if (x.size(1) != K || bank->K != K || bank->N != N)
     bad_value("adapter_linear: input " + shape_of(x) + ", projection [" + std::to_string(N) + ", " + std::to_string(K) + "], adapters on [" +
               std::to_string(bank->N) + ", " + std::to_string(bank->K) + "]");
+  if (std::max(N, K) > 0x7fffffffL) bad_value("adapter_linear: projections of less than 2^31 rows and columns");
   if (plan->max_id >= bank->G)
     bad_value("adapter_linear: the plan names adapter " + std::to_string(plan->max_id) + ", the bank has " + std::to_string(bank->G));
   const long unit = plan->unit(M);

@@ -339,3 +339,13 @@ def test_c_entries_refuse_bad_arguments():
     assert lib.aql_act8_pack(p, 0, 4, 64, 60, p, p, None) != 0
     assert lib.aql_act8_unpack(None, p, 4, 64, p, 0, 64, None) != 0
     assert lib.aql_act8_pack(None, 0, 0, 64, 64, None, None, None) == 0   # no rows: nothing to do
+
+
+def test_act8_of_rows_beyond_the_format_is_refused():
+    """More columns than the kernels' 2^24, also where the count's low 32 bits would pass (a broadcast row: no memory)."""
+    for columns in ((1 << 24) + 1, (1 << 31) + 8, (1 << 32) + 5):
+        with pytest.raises(ValueError, match="columns"):
+            ops.act8_pack(torch.zeros(1, 1).expand(1, columns))
+        with pytest.raises(ValueError):
+            ops.Act8(torch.zeros(0, 1, dtype=torch.uint8).expand(0, (columns + 31) // 32 * 32), torch.zeros(0, 1, dtype=torch.uint8).expand(0, (columns + 31) // 32),
+                     (0, columns), torch.float32).unpack()

@@ -21,6 +21,8 @@ namespace {
 
 constexpr int BK = 64;
 constexpr uint32_t OOB = 0x80000000u;
+constexpr int SPAN = 0x40000000;     // bytes from a tile's first row that its buffer descriptor covers: 256 rows of any leading dimension below 2^21
+constexpr int MAX_R = 1 << 16;       // of the stacks: so that rows of T's three parts, and of B, do as well
 
 struct Rows {
   const int* id;   // adapter of each unit of rows; null: no adapters at all
@@ -281,7 +283,7 @@ struct Stage {
   // base: first row of the tile; live(r): whether row r of the tile is read (others are zeros)
   template <class L>
   __device__ __forceinline__ void begin(const bf16_t* base, long ld, int K, int tid, L live) {
-    rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t*>(base), 0, 0x40000000, 0x00020000);
+    rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t*>(base), 0, SPAN, 0x00020000);
     kc = ((tid & 7) ^ lds_mix(tid >> 3)) * 8;
 #pragma unroll
     for (int l = 0; l < NL; ++l) {
@@ -968,8 +970,8 @@ extern "C" int aql_adapter_linear(const bf16_t* X, long ldx, const bf16_t* W, lo
   AQL_CHECK_ARG(ldx >= K && ldw >= K && ldy >= N && (!residual || ldr >= N) && ldx % 8 == 0 && ldw % 8 == 0 && ldy % 8 == 0 && ldr % 8 == 0 && ldx < (1L << 21) &&
                     ldw < (1L << 21), "aql_adapter_linear: leading dimensions (multiples of 8, at least the width, below 2^21)");
   AQL_CHECK_ARG((((uintptr_t)X | (uintptr_t)W | (uintptr_t)bias | (uintptr_t)residual | (uintptr_t)Y) & 15) == 0, "aql_adapter_linear: operands must be 16-byte aligned");
-  AQL_CHECK_ARG(rows_ok(unit_id, runs, unit) && (runs == 0 || (A && B && ranks && scales && T && R > 0 && R % 8 == 0 && slots >= 1 && slots <= 16 && (parts == 1 || parts == 3))),
-                "aql_adapter_linear: bad adapters (R=%d: a multiple of 8) or rows", R);
+  AQL_CHECK_ARG(rows_ok(unit_id, runs, unit) && (runs == 0 || (A && B && ranks && scales && T && R > 0 && R <= MAX_R && R % 8 == 0 && slots >= 1 && slots <= 16 && (parts == 1 || parts == 3))),
+                "aql_adapter_linear: bad adapters (R=%d: a multiple of 8, at most %d) or rows", R, MAX_R);
   const Rows rows{runs ? unit_id : nullptr, unit};
   if (runs) {
     launch_down(DownArgs{X, nullptr, nullptr, A, ranks, scales, T, ldx, M, K, R, parts, rows}, runs, slots, stream);
@@ -1001,12 +1003,13 @@ extern "C" int aql_adapter_linear(const bf16_t* X, long ldx, const bf16_t* W, lo
     const auto tiles = [&](long bm, long bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
     const long t192 = (tiles(256, 192) + 255) / 256 * 295, t160 = tiles(128, 160) <= 256 ? 198 : (tiles(128, 160) + 511) / 512 * 292;
     const long t128 = (tiles(128, 128) + 255) / 256 * 141;
-    if (N % 320 == 0 && tiles(256, 320) >= 256 && (runs == 0 || unit % 256 == 0)) AQL_TILE(256, 320, 2, 4, 2, ONE);
-    else if (N % 320 == 0 && tiles(256, 320) >= 256) AQL_TILE(256, 320, 2, 4, 2, FIND);
+    const bool wide = N % 320 == 0 && 320 * ldw * 2 <= SPAN;   // (320 rows of W under one descriptor)
+    if (wide && tiles(256, 320) >= 256 && (runs == 0 || unit % 256 == 0)) AQL_TILE(256, 320, 2, 4, 2, ONE);
+    else if (wide && tiles(256, 320) >= 256) AQL_TILE(256, 320, 2, 4, 2, FIND);
     else if (tiles(128, 128) >= 256) {
       if (t128 <= t160 && t128 <= t192) AQL_TILE(128, 128, 2, 4, 2);
       else if (t192 < t160) AQL_TILE(256, 192, 4, 2, 2);
-      else if (N % 320 == 0 && tiles(128, 160) > 256) AQL_TILE(128, 320, 2, 4, 2);
+      else if (wide && tiles(128, 160) > 256) AQL_TILE(128, 320, 2, 4, 2);
       else AQL_TILE(128, 160, 2, 2, 2);
     }
     else if (tiles(64, 128) >= 256) AQL_TILE(64, 128, 2, 4, 3);
@@ -1022,7 +1025,7 @@ extern "C" int aql_adapter_linear(const bf16_t* X, long ldx, const bf16_t* W, lo
 extern "C" int aql_adapter_down(const bf16_t* X, long ldx, const uint8_t* codes, const uint8_t* exps, long M, int K, const bf16_t* A, const int* ranks,
                                 const float* scales, int R, const int* unit_id, int unit, int runs, int slots, bf16_t* T, int parts,
                                 hipStream_t stream) {
-  AQL_CHECK_ARG(M >= 0 && M < (1L << 31) - 256 && K > 0 && K % 8 == 0 && K < (1 << 21) && R > 0 && R % 8 == 0, "aql_adapter_down: bad shape M=%ld K=%d R=%d", M, K, R);
+  AQL_CHECK_ARG(M >= 0 && M < (1L << 31) - 256 && K > 0 && K % 8 == 0 && K < (1 << 21) && R > 0 && R <= MAX_R && R % 8 == 0, "aql_adapter_down: bad shape M=%ld K=%d R=%d", M, K, R);
   AQL_CHECK_ARG(rows_ok(unit_id, runs, unit), "aql_adapter_down: bad rows");
   if (M == 0 || runs == 0) return AQL_OK;
   AQL_CHECK_ARG(!codes == !exps && !X != !codes && (!X || (ldx >= K && ldx % 8 == 0 && ldx < (1L << 21) && ((uintptr_t)X & 15) == 0)) && A && ranks && scales && T && slots >= 1 && slots <= 16 && (parts == 1 || parts == 3),

@@ -222,13 +222,13 @@ int aql_groupnorm_silu_bwd(const bf16_t* x, const bf16_t* dy, int B, int HW, int
                            float* scratch, aql_stream_t stream);
 /* ---- low-rank adapters of many requests beside one projection (csrc/aql_adapter.hip) --------------------------------------------------
  *   T[m] = scales[g] A[g] x_m,   Y[m] = W x_m + bias + B[g] T[m] + residual[m],   g = the adapter of row m (none: Y = W x + bias + residual)
- * A: [G][R][K], B: [G][N][R] bf16, stacked at one rank R (a multiple of 8); rows of A / columns of B past ranks[g] are taken as zeros.
+ * A: [G][R][K], B: [G][N][R] bf16, stacked at one rank R (a multiple of 8, at most 65536); rows of A / columns of B past ranks[g] are taken as zeros.
  * Row m has adapter unit_id[m / unit] (-1: none); the M / unit (rounded up) ids are device memory and not checked against G here (the binding does).
  * runs: stretches of neighbouring rows with one adapter, 0: no adapters at all; slots (1..16): at least the adapters that any 16 rows
  * [16 i, 16 i + 16) meet; used: adapters that have rows (runs and used decide between forms only).  T: [M][parts][R] bf16, out: T rounded (parts = 1), or T = hi + mid + lo in three parts for a
  * later aql_adapter_wgrad (parts = 3); rows without an adapter are left as they are.
  * Backward data: the same entry with X = dY, W = W^T [K][N], A = B^T [G][R][N], B = A^T [G][K][R]: T is dT, Y is dX.
- * N, K, leading dimensions: multiples of 8; pointers 16-byte aligned.  One fp32 accumulator per output, rounded to bf16 once.          */
+ * N, K, leading dimensions: multiples of 8, those of X and W below 2^21; pointers 16-byte aligned.  One fp32 accumulator per output, rounded to bf16 once.          */
 int aql_adapter_linear(const bf16_t* X, long ldx, const bf16_t* W, long ldw, const bf16_t* bias, const bf16_t* residual, long ldr, bf16_t* Y,
                        long ldy, long M, int N, int K, const bf16_t* A, const bf16_t* B, const int* ranks, const float* scales, int R,
                        const int* unit_id, int unit, int runs, int slots, int used, bf16_t* T, int parts, aql_stream_t stream);

@@ -136,7 +136,7 @@ class AdapterBank:
             h.reads()
             at, bt = h.a.transpose(1, 2).contiguous(), h.b.transpose(1, 2).contiguous()
             torch.cuda.current_stream(self.device).synchronize()      # once: later calls may come on other streams
-            h.bt, h.at = bt, at                  # (calls go by `at`: it is there when both are complete)
+            h.publish(at, bt)
             self._transposed = True
 
 

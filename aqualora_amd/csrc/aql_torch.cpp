@@ -121,6 +121,11 @@ Rows gemm_rows(const Tensor& t) {
   return r;
 }
 
+// memory that kernels on stream s use: freed earlier, it is given out again behind them (nothing to do on the stream that it was allocated on)
+void used_on(const Tensor& t, const c10::hip::HIPStream& s) {
+  if (t.defined()) c10::hip::HIPCachingAllocator::recordStream(t.storage().data_ptr(), s);
+}
+
 Tensor leaf(const Tensor& t) { return t.defined() && t.is_leaf() && t.requires_grad() ? t : Tensor(); }
 
 // A leaf's accumulation node runs on the stream on which it was made.  A captured backward pass that reaches one made on another stream (an eager graph of
@@ -314,13 +319,23 @@ struct Bank {   // the device side of adapters.AdapterBank
       if (e) (void)hipEventDestroy(e);
   }
   c10::hip::HIPStream current() const { return c10::hip::getCurrentHIPStream(a.get_device()); }
+  void used_by(const c10::hip::HIPStream& s) const {
+    for (const Tensor* t : {&a, &b, &at, &bt, &ranks, &scales}) used_on(*t, s);
+  }
   // ahead of kernels on the current stream that read the stacks (guard held)
   void read_on(const c10::hip::HIPStream& s) {
     for (const auto& r : readers)
       if (r == s) return;
     if (capturing(s)) return;
     if (home && *home != s) hip_ok(hipStreamWaitEvent(s.stream(), laid, 0), "AdapterBank");
+    used_by(s);
     readers.push_back(s);
+  }
+  // the transposed stacks, complete
+  void publish(const Tensor& at_, const Tensor& bt_) {
+    const std::lock_guard<std::mutex> lock(guard);
+    at = at_, bt = bt_;
+    for (const auto& r : readers) used_by(r);
   }
   void reads() {
     const std::lock_guard<std::mutex> lock(guard);
@@ -335,6 +350,7 @@ struct Bank {   // the device side of adapters.AdapterBank
     ++serial;
     if (capturing(s)) return;
     down_seen = up_seen = -1;
+    used_by(s);
     quiet.wait(lock, [&] { return busy == 0; });
     const c10::DeviceGuard device(a.device());
     for (hipEvent_t* e : {&laid, &mark})
@@ -395,7 +411,8 @@ struct Plan {   // the device side of adapters.RequestPlan
   bool equal = false;
   std::vector<long> at;      // offsets of unit_id, perm, used_pos, slot in the table
   std::unordered_map<long, int> slots_by_unit;
-  std::mutex guard;          // of slots_by_unit: backward passes ask from the engine's threads
+  std::vector<c10::hip::HIPStream> readers;
+  std::mutex guard;          // of these two: backward passes ask from the engine's threads
 
   const int* part(int k) const { return (const int*)table.data_ptr() + at[k]; }
   long unit(long rows) const {   // rows per table unit for a call on `rows` rows
@@ -409,6 +426,15 @@ struct Plan {   // the device side of adapters.RequestPlan
     }
     if (rows % requests) bad_value("RequestPlan: " + std::to_string(rows) + " rows do not divide among " + std::to_string(requests) + " equal requests");
     return std::max(1L, rows / requests);
+  }
+  void reads() {   // ahead of kernels on the current stream that read the table
+    const auto s = c10::hip::getCurrentHIPStream(table.get_device());
+    const std::lock_guard<std::mutex> lock(guard);
+    for (const auto& r : readers)
+      if (r == s) return;
+    if (capturing(s)) return;
+    used_on(table, s);
+    readers.push_back(s);
   }
   int slots(long unit) {   // the most segments, and so adapters, that meet in 16 rows [16 i, 16 i + 16)
     const std::lock_guard<std::mutex> lock(guard);
@@ -555,6 +581,7 @@ std::optional<Tensor> adapter_linear(const Tensor& x, const Tensor& w, const Ten
     bad_value("adapter_linear: input, projection, adapters, plan and residual must live on one device");
   const Reading reading(*bank);
   if (!reading.in) return std::nullopt;
+  plan->reads();
   const bool train = bank->trainable && at::GradMode::is_enabled() && (down.requires_grad() || up.requires_grad());
   if (at::GradMode::is_enabled() && (train || x.requires_grad() || (res.defined() && res.requires_grad()))) {
     auto c = c10::make_intrusive<Call>();
@@ -585,7 +612,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("adapter_linear", &adapter_linear);
   py::class_<Bank, std::shared_ptr<Bank>>(m, "Bank")
       .def(py::init<>())
-      .def_readwrite("a", &Bank::a).def_readwrite("b", &Bank::b).def_readwrite("at", &Bank::at).def_readwrite("bt", &Bank::bt)
+      .def_readwrite("a", &Bank::a).def_readwrite("b", &Bank::b).def_readonly("at", &Bank::at).def_readonly("bt", &Bank::bt).def("publish", &Bank::publish)
       .def_readwrite("ranks", &Bank::ranks).def_readwrite("scales", &Bank::scales)
       .def_readwrite("down", &Bank::down).def_readwrite("up", &Bank::up).def("fresh", &Bank::fresh)
       .def("reads", &Bank::reads)

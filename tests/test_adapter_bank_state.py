@@ -342,3 +342,27 @@ def test_a_sampling_machine_follows_the_banks():
     inference.attach_adapters(unet, loras[::-1])
     third = again(m)
     assert torch.equal(third, new().run(prog)) and not torch.equal(third, first)
+
+
+@gpu
+@pytest.mark.parametrize("trainable", [False, True])
+def test_bank_and_plan_dropped_while_a_stream_still_reads(trainable):
+    """Made on one stream, used late on another and dropped at once: their memory is not given out again before that."""
+    s = Site(10)
+    x = s.x.detach().requires_grad_(True)
+    want = [ops.adapter_linear(x, s.packed, s.bank(s.new), s.plan)]
+    want = [want[0].detach(), *torch.autograd.grad(want[0], x, s.dy)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        bank, plan = s.bank(s.new, trainable), adapters.RequestPlan([0, 2, -1, 1], [70, 1, 30, 99])
+        sizes = [t.numel() * t.element_size() for t in (bank.handle.a, bank.handle.b, bank.handle.ranks, bank.handle.scales, plan.table)]
+        torch.cuda.synchronize()
+        with torch.cuda.stream(torch.cuda.Stream()):
+            torch.cuda._sleep(SLEEP)
+            y = ops.adapter_linear(x, s.packed, bank, plan)
+            dx, = torch.autograd.grad(y, x, s.dy)
+            y = y.detach()
+        del bank, plan
+        other = [torch.zeros(n, dtype=torch.uint8, device=DEV) for n in sizes * 3]      # (zeros: all of them adapter 0 of rank 0, if they were read)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[0]) and torch.equal(dx, want[1]) and len(other)

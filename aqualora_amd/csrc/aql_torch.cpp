@@ -13,6 +13,7 @@
 #include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
 #include <condition_variable>
 #include <cstdlib>
 #include <memory>
@@ -324,9 +325,7 @@ struct Bank {   // the device side of adapters.AdapterBank
   }
   // ahead of kernels on the current stream that read the stacks (guard held)
   void read_on(const c10::hip::HIPStream& s) {
-    for (const auto& r : readers)
-      if (r == s) return;
-    if (capturing(s)) return;
+    if (std::find(readers.begin(), readers.end(), s) != readers.end() || capturing(s)) return;
     if (home && *home != s) hip_ok(hipStreamWaitEvent(s.stream(), laid, 0), "AdapterBank");
     used_by(s);
     readers.push_back(s);
@@ -362,6 +361,7 @@ struct Bank {   // the device side of adapters.AdapterBank
       hip_ok(hipEventRecord(mark, r.stream()), "AdapterBank");
       hip_ok(hipStreamWaitEvent(s.stream(), mark, 0), "AdapterBank");
     }
+    if (std::find(readers.begin(), readers.end(), s) == readers.end()) readers.push_back(s);   // (for the next layout, if this one ends half way: out of memory)
   }
   void end_layout() {
     const auto s = current();
@@ -430,9 +430,7 @@ struct Plan {   // the device side of adapters.RequestPlan
   void reads() {   // ahead of kernels on the current stream that read the table
     const auto s = c10::hip::getCurrentHIPStream(table.get_device());
     const std::lock_guard<std::mutex> lock(guard);
-    for (const auto& r : readers)
-      if (r == s) return;
-    if (capturing(s)) return;
+    if (std::find(readers.begin(), readers.end(), s) != readers.end() || capturing(s)) return;
     used_on(table, s);
     readers.push_back(s);
   }

@@ -366,3 +366,34 @@ def test_bank_and_plan_dropped_while_a_stream_still_reads(trainable):
         other = [torch.zeros(n, dtype=torch.uint8, device=DEV) for n in sizes * 3]      # (zeros: all of them adapter 0 of rank 0, if they were read)
         torch.cuda.synchronize()
         assert torch.equal(y, want[0]) and torch.equal(dx, want[1]) and len(other)
+
+
+@gpu
+def test_a_layout_that_ends_half_way_is_finished_before_the_next():
+    """The first layout is late on its stream and fails between its copies; the next comes from another stream."""
+    s = Site(11)
+    bank = s.bank(s.old)
+    want = s.step(s.bank(s.new))
+    s.step(bank)
+    live = bank._live
+    put(bank, [w.to(DEV) for w in s.new])
+
+    class Fails:                                         # the copies of `down` are queued, those of `up` raise
+        calls = 0
+
+        def __getitem__(self, index):
+            Fails.calls += 1
+            if Fails.calls == 2:
+                raise MemoryError
+            return torch.zeros_like(live)[index]         # (other values than the right ones)
+    torch.cuda.synchronize()
+    bank._live = Fails()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        torch.cuda._sleep(SLEEP)
+        with pytest.raises(MemoryError):
+            s.call(bank)
+    bank._live = live
+    with torch.cuda.stream(torch.cuda.Stream()):
+        got = s.step(bank)
+    torch.cuda.synchronize()
+    assert same(got, want)

@@ -14,6 +14,7 @@ from torch.optim.optimizer import register_optimizer_step_post_hook
 from . import _lib as L
 
 MAX_RANK = 1024
+MAX_ADAPTERS = 65535
 
 
 def _count_fused_step(optimizer, args, kwargs):
@@ -50,8 +51,8 @@ class AdapterBank:
                 raise ValueError(f"AdapterBank: bfloat16 or float32 weights, not {t.dtype}")
         self.G, self.rank, self.K = down.shape
         self.N = up.shape[1]
-        if not (1 <= self.G <= 65535 and 1 <= self.rank <= MAX_RANK and self.K % 8 == 0 and self.N % 8 == 0 and self.K and self.N):
-            raise ValueError(f"AdapterBank: 1 to 65535 adapters of rank 1 to {MAX_RANK} on sides that are multiples of 8, "
+        if not (1 <= self.G <= MAX_ADAPTERS and 1 <= self.rank <= MAX_RANK and self.K % 8 == 0 and self.N % 8 == 0 and self.K and self.N):
+            raise ValueError(f"AdapterBank: 1 to {MAX_ADAPTERS} adapters of rank 1 to {MAX_RANK} on sides that are multiples of 8, "
                              f"not {self.G} of rank {self.rank} on [{self.N}, {self.K}]")
         self.ranks = [self.rank] * self.G if ranks is None else [int(r) for r in ranks]
         self.scales = [1.0] * self.G if scales is None else [float(s) for s in scales]
@@ -155,8 +156,8 @@ class RequestPlan:
         if dev.type != "cuda":
             raise L.AqlError("RequestPlan needs an MI355X (cuda device); there is no CPU path")
         ids = np.asarray([int(a) for a in adapters], dtype=np.int64)
-        if ids.size and ids.min() < -1:
-            raise ValueError("RequestPlan: adapters are numbered from 0; -1 is none")
+        if ids.size and (ids.min() < -1 or ids.max() >= MAX_ADAPTERS):
+            raise ValueError(f"RequestPlan: adapters are numbered from 0 to {MAX_ADAPTERS - 1}; -1 is none")
         self.equal = lengths is None
         self.adapters, self.device = [int(a) for a in ids], dev
         self.lengths = None if self.equal else [int(x) for x in lengths]

@@ -603,3 +603,10 @@ def test_forward_mode_is_refused(grad):
             with pytest.raises(RuntimeError):
                 ops.adapter_linear(xd, packed, bank, plan, residual=rd)
         ops.adapter_linear(x, packed, bank, plan, residual=res)
+
+
+def test_plans_of_adapters_that_no_bank_holds_are_refused():
+    """A bank has at most 65535 adapters; the tables are as long as the largest number, and 32 bits wide."""
+    for ids in ([0, 65535], [1 << 31], [(1 << 32) + 3], [-2], [0, -(1 << 32)]):
+        with pytest.raises(ValueError, match="numbered"):
+            adapters.RequestPlan(ids)

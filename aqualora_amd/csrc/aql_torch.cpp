@@ -75,6 +75,7 @@ bool capturing(const c10::hip::HIPStream& s) {
 }
 // of the capture that a stream is in, never used again; 0: none
 unsigned long long capture_id(const c10::hip::HIPStream& s) {
+  if (!capturing(s)) return 0;
   hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
   unsigned long long id = 0;
   hip_ok(hipStreamGetCaptureInfo(s.stream(), &cs, &id), "hipStreamGetCaptureInfo");

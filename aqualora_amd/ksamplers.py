@@ -425,7 +425,9 @@ class SamplerMachine:
         if isinstance(self.scale2, RequestPlan):          # replays read the banks as they were laid out last: lay out what has changed since an earlier run
             banks = banks_of(self.unet)
             if len(banks) != len(self.banks) or any(a is not b for a, b in zip(banks, self.banks)):
-                self.graph = None                         # captured on banks that have been replaced
+                if self.graph is not None:                # captured on banks that have been replaced: dropped when its last replay has ended
+                    torch.cuda.current_stream().synchronize()
+                self.graph = None
             self.banks = banks
             for bank in banks:
                 bank.refresh()

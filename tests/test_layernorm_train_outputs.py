@@ -54,3 +54,14 @@ def test_neither_output_of_a_chain_is_lost():
         ref, slack = reference(x, x, g, b, dy if use[0] else zero, dres if use[1] else None, 1e-5)
         check("dx", xd.grad, ref[1], slack[1], torch.float32)
         check("dgamma", gd.grad, ref[2], slack[2], torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(grad):
+    x, g, b, dy, _ = (t.to(DEV) for t in inputs(5, 64, torch.float32, 34))
+    fw = torch.autograd.forward_ad
+    with torch.set_grad_enabled(grad), fw.dual_level():
+        for args in ((fw.make_dual(x, dy), g, b), (x, fw.make_dual(g, b), b), (x, g, fw.make_dual(b, g))):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                ops.layernorm_train(*args)

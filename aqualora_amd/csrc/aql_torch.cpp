@@ -144,6 +144,15 @@ void leaves_ok(const std::vector<Tensor>& leaves, const Tensor& g, const char* n
   }
 }
 
+// A saved tensor as it was saved, whatever hooks of saved tensors made of it meanwhile (moved to the host and back, other strides): the kernels go by its address.
+// `rows`: with its row stride, else contiguous
+Tensor intact(const Tensor& t, at::IntArrayRef size, at::ScalarType type, const Tensor& like, const char* name, bool rows = false) {
+  if (!t.defined()) return t;
+  if (t.device() != like.device() || t.scalar_type() != type || t.sizes() != size || t.layout() != at::kStrided)
+    throw AqlErr(std::string(name) + ": a tensor saved for the backward pass came back as " + c10::toString(t.scalar_type()) + " " + shape_of(t) + " on " + t.device().str());
+  return rows ? t : t.contiguous();
+}
+
 // gradients of a backward pass under create_graph: they carry a node that refuses a second backward pass
 variable_list once(variable_list grads, const char* name) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -201,6 +210,8 @@ Tensor act8_unpack(const Tensor& codes, const Tensor& exps, std::vector<int64_t>
 struct NormCall : torch::CustomClassHolder {   // what its backward pass needs besides tensors of the graph
   std::vector<Tensor> leaves;
   bool beta = false;
+  long M = 0, C = 0;
+  at::ScalarType weights = at::kFloat;
 };
 
 struct LayerNormTrain : torch::autograd::Function<LayerNormTrain> {
@@ -215,7 +226,7 @@ struct LayerNormTrain : torch::autograd::Function<LayerNormTrain> {
                                 ptr<float>(stats), ptr<uint8_t>(codes), ptr<uint8_t>(exps), st), "aql_layernorm_train_fwd", st);
     ctx->save_for_backward({ckpt8 ? Tensor() : r.t, codes, exps, gamma, stats});
     auto c = c10::make_intrusive<NormCall>();
-    c->beta = beta.defined();
+    c->beta = beta.defined(), c->M = M, c->C = C, c->weights = gamma.scalar_type();
     c->leaves = {leaf(x), leaf(gamma), leaf(beta)};
     ctx->set_materialize_grads(false);   // an output that nothing used has no gradient, not one of zeros
     ctx->saved_data["call"] = c10::IValue::make_capsule(std::move(c));
@@ -224,13 +235,13 @@ struct LayerNormTrain : torch::autograd::Function<LayerNormTrain> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const variable_list s = ctx->get_saved_variables();
-    const Tensor &x = s[0], &codes = s[1], &exps = s[2], &gamma = s[3], &stats = s[4];
     const auto c = c10::static_intrusive_pointer_cast<NormCall>(ctx->saved_data["call"].toCapsule());
-    const long M = stats.size(0), C = gamma.size(0);
+    const long M = c->M, C = c->C;
     const bool want_g = ctx->needs_input_grad(1), want_b = c->beta && ctx->needs_input_grad(2);
     if (!g[0].defined()) {   // only the pass-through output was used: its gradient as it is, and the weights have no part in it
       at::AutoGradMode off(false);
-      const auto zeros = [&](bool want) { return want ? at::zeros({C}, gamma.options()) : Tensor(); };
+      if (!g.back().defined()) return variable_list(6);
+      const auto zeros = [&](bool want) { return want ? at::zeros({C}, g.back().options().dtype(c->weights)) : Tensor(); };
       return {g.size() > 1 ? g[1] : Tensor(), zeros(want_g), zeros(want_b), Tensor(), Tensor(), Tensor()};
     }
     here(g[0], "layernorm_train backward");
@@ -244,6 +255,12 @@ struct LayerNormTrain : torch::autograd::Function<LayerNormTrain> {
         if (want_g) dg = at::zeros({C}, f32);
         if (want_b) db = at::zeros({C}, f32);
       } else {
+        const char* name = "layernorm_train";
+        Rows x;
+        if (s[0].defined()) x = rows2d(intact(s[0], {M, C}, dx.scalar_type(), dx, name, true));
+        const long nb = (C + 31) / 32;
+        const Tensor codes = intact(s[1], {M, nb * 32}, at::kByte, dx, name), exps = intact(s[2], {M, nb}, at::kByte, dx, name);
+        const Tensor gamma = intact(s[3], {C}, c->weights, dx, name), stats = intact(s[4], {M, 2}, at::kFloat, dx, name);
         const Rows dy = rows2d(g[0]);
         Rows dres;
         if (g.size() > 1 && g[1].defined()) dres = rows2d(g[1]);
@@ -251,13 +268,13 @@ struct LayerNormTrain : torch::autograd::Function<LayerNormTrain> {
         const long n = aql_layernorm_train_scratch_floats(M, (int)C);
         const c10::DataPtr scratch = workspace(n);
         const auto st = stream_of(dx);
-        ran(aql_layernorm_train_bwd(ptr(x), ptr<uint8_t>(codes), ptr<uint8_t>(exps), dy.t.data_ptr(), ptr(dres.t), dt(dx), M, (int)C,
-                                    x.defined() && M > 1 ? x.stride(0) : C, dy.ld, dres.ld, gamma.data_ptr(), dt(gamma), ptr<float>(stats), dx.data_ptr(), C,
+        ran(aql_layernorm_train_bwd(ptr(x.t), ptr<uint8_t>(codes), ptr<uint8_t>(exps), dy.t.data_ptr(), ptr(dres.t), dt(dx), M, (int)C,
+                                    x.t.defined() ? x.ld : C, dy.ld, dres.ld, gamma.data_ptr(), dt(gamma), ptr<float>(stats), dx.data_ptr(), C,
                                     ptr<float>(dg), ptr<float>(db), (float*)scratch.get(), n, st), "aql_layernorm_train_bwd", st);
       }
-      if (gamma.scalar_type() != at::kFloat) {
-        if (dg.defined()) dg = dg.to(gamma.scalar_type());
-        if (db.defined()) db = db.to(gamma.scalar_type());
+      if (c->weights != at::kFloat) {
+        if (dg.defined()) dg = dg.to(c->weights);
+        if (db.defined()) db = db.to(c->weights);
       }
     }
     return once({dx, dg, db, Tensor(), Tensor(), Tensor()}, "layernorm_train");
@@ -538,14 +555,17 @@ struct AdapterLinear : torch::autograd::Function<AdapterLinear> {
         if (want_b) out[2] = at::zeros({bank.G, bank.N, bank.r}, bank.scales.options());
       } else {
         const Rows dy = gemm_rows(g[0]);
-        Tensor dT, T = s[1];
+        const char* name = "adapter_linear";
+        const long nb = (c->K + 31) / 32;
+        Tensor dT, T = intact(s[1], {c->M, 3, bank.R}, at::kBFloat16, dy.t, name);
+        const Tensor codes = intact(s[2], {c->M, nb * 32}, at::kByte, dy.t, name), exps = intact(s[3], {c->M, nb}, at::kByte, dy.t, name);
         Rows x;
-        if (s[0].defined()) x = {s[0], c->M > 1 ? s[0].stride(0) : c->K};
+        if (s[0].defined()) x = gemm_rows(intact(s[0], {c->M, c->K}, at::kBFloat16, dy.t, name, true));
         if (want_x) std::tie(out[0], dT) = product(dy, c->wt, Tensor(), Rows(), bank.bt, bank.at, bank, *c->plan, c->unit, c->K, c->N, c->train && want_a ? 3 : 1);
         if (c->train && (want_a || want_b)) {
           if (want_a && !dT.defined() && c->plan->nseg) dT = down(dy, Tensor(), Tensor(), c->M, c->N, bank.bt, bank, *c->plan, c->unit);
-          if (want_b && !T.defined() && c->plan->nseg) T = down(Rows(), s[2], s[3], c->M, c->K, bank.a, bank, *c->plan, c->unit);
-          wgrad(dT, x, s[2], s[3], want_a, T, dy, want_b, c->M, bank, *c->plan, c->unit, out[1], out[2]);
+          if (want_b && !T.defined() && c->plan->nseg) T = down(Rows(), codes, exps, c->M, c->K, bank.a, bank, *c->plan, c->unit);
+          wgrad(dT, x, codes, exps, want_a, T, dy, want_b, c->M, bank, *c->plan, c->unit, out[1], out[2]);
         }
       }
       if (want_r) out[3] = g[0];

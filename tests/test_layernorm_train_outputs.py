@@ -65,3 +65,20 @@ def test_forward_mode_is_refused(grad):
         for args in ((fw.make_dual(x, dy), g, b), (x, fw.make_dual(g, b), b), (x, g, fw.make_dual(b, g))):
             with pytest.raises((RuntimeError, NotImplementedError)):
                 ops.layernorm_train(*args)
+
+
+@gpu
+def test_a_node_behind_it_that_has_no_gradient():
+    class Stop(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, y):
+            return y * 2
+
+        @staticmethod
+        def backward(ctx, g):
+            return None
+    x, g, b, *_ = (t.to(DEV) for t in inputs(5, 64, torch.float32, 35))
+    x, g = x.requires_grad_(True), g.requires_grad_(True)
+    for f in (ops.layernorm_train, lambda *a: ops.layernorm_train_res(*a)[0]):
+        (Stop.apply(f(x, g, b)).sum() + 0 * x.sum()).backward()
+        assert (x.grad == 0).all() and g.grad is None

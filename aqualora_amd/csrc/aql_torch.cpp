@@ -579,6 +579,7 @@ std::optional<Tensor> adapter_linear(const Tensor& x, const Tensor& w, const Ten
                                      const std::shared_ptr<Plan>& plan, const std::optional<Tensor>& residual_, bool ckpt8) {
   if (!bank->at.defined() && x.requires_grad() && at::GradMode::is_enabled()) return std::nullopt;
   const Tensor &down = bank->down, &up = bank->up;
+  if (w.dim() != 2) bad_value("adapter_linear: the projection must be [N, K], not " + shape_of(w));
   const long N = w.size(0), K = w.size(1);
   if (x.dim() != 2 || x.scalar_type() != at::kBFloat16)
     bad_value("adapter_linear: expected bfloat16 [rows, " + std::to_string(K) + "], got " + c10::toString(x.scalar_type()) + " " + shape_of(x));
@@ -594,6 +595,9 @@ std::optional<Tensor> adapter_linear(const Tensor& x, const Tensor& w, const Ten
   if (res.defined() && (res.dim() != 2 || res.size(0) != M || res.size(1) != N || res.scalar_type() != at::kBFloat16))
     bad_value("adapter_linear: residual must be bfloat16 [" + std::to_string(M) + ", " + std::to_string(N) + "], not " + shape_of(res));
   here(x, "adapter_linear");
+  const auto operand = [&](const Tensor& t, at::IntArrayRef size) { return t.scalar_type() == at::kBFloat16 && t.sizes() == size && t.is_contiguous() && t.device() == x.device(); };
+  if (!operand(w, {N, K}) || !operand(wt, {K, N}) || (bias.defined() && !operand(bias, {N})))
+    bad_value("adapter_linear: the projection must be bfloat16 [" + std::to_string(N) + ", " + std::to_string(K) + "], its transpose and a bias of " + std::to_string(N) + ", contiguous on " + x.device().str());
   for (const Tensor* t : {&x, &res, &down, &up})   // (without reverse gradients no node is made that would refuse it)
     if (t->defined() && t->_fw_grad(0).defined()) throw AqlErr("adapter_linear has no forward-mode derivative");
   if (bank->a.device() != x.device() || plan->table.device() != x.device() || w.device() != x.device() || (res.defined() && res.device() != x.device()))

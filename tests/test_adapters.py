@@ -610,3 +610,19 @@ def test_plans_of_adapters_that_no_bank_holds_are_refused():
     for ids in ([0, 65535], [1 << 31], [(1 << 32) + 3], [-2], [0, -(1 << 32)]):
         with pytest.raises(ValueError, match="numbered"):
             adapters.RequestPlan(ids)
+
+
+@gpu
+def test_projections_that_do_not_fit_together_are_refused():
+    d, lengths, rows, ids, equal = make("ragged", 16)
+    packed, bank, plan = handles(d, lengths, ids, equal, False)
+    x = d["x"].to(DEV)
+    for name, value in (("bias", packed.bias[:-8]), ("bias", packed.bias.float()), ("bias", packed.bias.cpu()), ("wt", packed.wt[:, :-8].contiguous()), ("wt", packed.w.t()),
+                        ("w", packed.w.float()), ("w", packed.w[0])):
+        bad = copy.copy(packed)
+        setattr(bad, name, value)
+        with pytest.raises(ValueError):
+            ops.adapter_linear(x, bad, bank, plan)
+    bad = copy.copy(packed)
+    bad.bias = None
+    ops.adapter_linear(x, bad, bank, plan)
